@@ -24,7 +24,12 @@ LIB = os.path.join(HERE, "smoothquant", "libsqmp_w4a4.so")
 ARCH = os.environ.get("SQMP_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", INCLUDE,
-          "-Wno-unused-result"]
+          "-Wno-unused-result",
+          # no packed fp32 instructions (v_pk_{add,mul,fma}_f32): hipcc -O3 forms them from
+          # scalar float code by itself, and some of their operand forms have given wrong
+          # results on this hardware now and then (same roundings without them; the host pass
+          # warns that it does not know the feature)
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # SQMP_DIAG=1: also instantiate the timing-diagnostic kernel variants (wrong results by
 # design; never in the product build), into libsqmp_w4a4_diag.so (loaded by SQMP_DIAG_LIB=1)
 if os.environ.get("SQMP_DIAG") == "1":

@@ -104,10 +104,11 @@ template <> struct Dec<BF16> {
   typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
   __device__ static inline uint32_t prep(uint32_t sbits) { return sbits << 16; }
   // The nibbles as bytes (b: nibbles 0, 2, 4, 6; c: 1, 3, 5, 7), each to fp32 by one
-  // v_cvt_f32_ubyteN, then (n - 8) * s = fma(n, s, -8 s) on v_pk_fma_f32 -- n * s (4 x 8
+  // v_cvt_f32_ubyteN, then (n - 8) * s = fma(n, s, -8 s) -- n * s (4 x 8
   // significant bits) and -8 s are exact, so is their sum (code * s, <= 12 bits: no rounding,
   // and +0 for code 0 as the reference's 0 * s with s > 0) -- and one RNE cast per pair to bf16
-  // (v_cvt_pk_bf16_f32): D(code * s) as before, in 20 VALU per 8 values instead of 46.
+  // (v_cvt_pk_bf16_f32): D(code * s) as before, in 24 VALU per 8 values instead of 46 (the FMAs
+  // are scalar: the library is built without packed fp32 instructions).
   __device__ static inline u32x4 run(uint32_t w, uint32_t sf, const DecK&) {
     const float s = __uint_as_float(sf);
     const f2 s2 = {s, s}, m2 = {-8.0f * s, -8.0f * s};
