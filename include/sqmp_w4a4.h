@@ -257,7 +257,8 @@ int sqmp_gemm_f8_colmax(const void* a8, const float* ascale, const void* xs, con
  *   scale_t[n/WR][g][r][j] = wscale[g][WR (n/WR) + 16 j + r];
  *   sal_t[n/WR][S_pad/64][lane][j][s][e] = wsal[WR (n/WR) + 16 j + (lane & 15)]
  *     [64 kd + 8 (4 (q & 1) + 2 s + (q >> 1)) + e]  (the GEMM's fragment chunk order).
- * Rows >= N are zero. */
+ * Rows >= N are zero.  fp32 (J = 2 only): the operand of sqmp_gemv_w4 and
+ * sqmp_expert_linear_w4 for fp32 layers (sqmp_gemm_fq7 itself is fp16 / bf16). */
 int sqmp_fq7_sizes(int N, int Kp, int S_pad, int ngw, int J, size_t* codes_bytes,
                    size_t* scale_elems, size_t* sal_elems);
 int sqmp_pack_fq7(const void* codes, const void* wscale, const void* wsal, int dtype, int N,
@@ -411,6 +412,57 @@ int sqmp_pack_h2d(const void* planes, int Np, int L, void* wt, void* stream);
 int sqmp_gemm_h2d(const void* a2, int ldr, const int* aexp, const void* wt, const int* bexp,
                   const float* bias, float* y, int M, int N, int L, uint32_t* colmax,
                   void* stream);
+
+/* ---------------------------------------------------------------- few rows, experts, routing
+ * The decoding form of F.linear (fake_quant.py:306): y[M][N] = D( x . W^T + bias ) for at most
+ * SQMP_GEMV_MAX_ROWS rows, W = D(code * scale) and the exact salient columns, fp32 accumulation in
+ * a fixed order.  x: D rows of Kp + S_pad positions in packed order (SQMP_OUT_FP of
+ * sqmp_quant_act_v2, or sqmp_pack_rows), row stride ldx elements, 16-B aligned rows; no row
+ * beyond M is read.  codes_t / scale_t / sal_t: sqmp_pack_fq7 with J = 2.  Gw % 8 == 0. */
+#define SQMP_GEMV_MAX_ROWS 64
+int sqmp_gemv_w4(const void* x, long ldx, const void* codes_t, const void* scale_t,
+                 const void* sal_t, const void* bias, void* y, int dtype, int M, int N, int Kp,
+                 int S_pad, int Gw, int ngw, void* stream);
+
+/* Routing (the MixtralSparseMoeBlock that fake_quant.py:564-668 quantizes).  logits D [T][E], row
+ * stride ldl: per token the top_k largest (ties: the lowest index; NaN counts as the largest; -inf
+ * is never chosen) -> ids int32 [T][top_k] (-1: nothing chosen), weights fp32 [T][top_k] (their
+ * softmax over the chosen, or over all E with normalize = 0; 0 where nothing is chosen), and the
+ * plan: the chosen pairs f = token * top_k + j in stable order by expert, offsets int32 [E + 1],
+ * rows int32 [T top_k] (slot -> f, -1 behind the last pair), slots int32 [T top_k] (f -> slot, -1
+ * where nothing is chosen).  E <= 256, top_k <= 16.  workspace: sqmp_route_workspace_bytes. */
+size_t sqmp_route_workspace_bytes(int T, int E);
+int sqmp_route(const void* logits, long ldl, int dtype, int T, int E, int top_k, int normalize,
+               float* weights, int32_t* ids, int32_t* offsets, int32_t* rows, int32_t* slots,
+               void* workspace, size_t ws_bytes, void* stream);
+/* The plan alone; an id outside 0 .. E - 1 counts as nothing chosen. */
+int sqmp_plan_routes(const int32_t* ids, int T, int E, int top_k, int32_t* offsets, int32_t* rows,
+                     int32_t* slots, void* workspace, size_t ws_bytes, void* stream);
+
+/* Products grouped by expert: z[slot] = D( W_e x[row(slot)] ) for the slots offsets[e] ..
+ * offsets[e + 1] of every expert e; row(slot) = rows[slot] / top_k, or slot where rows is NULL.
+ * Operands: those of sqmp_gemv_w4, E weights one behind the other (sqmp_fq7_sizes apart).  act = 0:
+ * n_out == N.  act = 1 (silu) / 2 (gelu, the error-function form): the N weight rows are 16 gate
+ * and 16 up rows in turn, z = D( act(gate) * up ), n_out of the N / 2 columns are written.
+ * slots = rows of z (an upper bound of offsets[E]); rows of z behind offsets[E] are left as they
+ * were.  */
+int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* rows, int top_k,
+                          const int32_t* offsets, int E, const void* codes_t, const void* scale_t,
+                          const void* sal_t, void* y, int dtype, int slots, int N, int n_out,
+                          int Kp, int S_pad, int Gw, int ngw, int act, void* stream);
+
+/* y[t] = D( sum_j weights[t][j] * z[slots[t][j]] ), fp32 sums in the order of j; slots < 0 are
+ * skipped.  z D [slots][H], y D [T][H]. */
+int sqmp_combine(const void* z, int dtype, int T, int top_k, int H, const int32_t* slots,
+                 const float* weights, void* y, void* stream);
+
+/* The unquantized activation operand: out[i][p] = x[row(i)][amap[p]] (0 where amap[p] < 0),
+ * p < Kp, then the S salient columns and zeros up to S_pad.  offsets == NULL: row(i) = i for R
+ * rows.  Else the R output rows are slots (those behind offsets[E] are left as they were), row(i) =
+ * rows[i] / top_k or i (rows NULL), and the map is amap + e * map_stride for i's expert e. */
+int sqmp_pack_rows(const void* x, long ldx, int dtype, int R, const int32_t* amap, int Kp,
+                   const int32_t* salient, int S, int S_pad, const int32_t* rows, int top_k,
+                   const int32_t* offsets, int E, long map_stride, void* out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -950,7 +950,8 @@ extern "C" int sqmp_pack_fq7(const void* codes, const void* wscale, const void* 
   SQMP_DEVICE_GUARD(stream);
   if (!codes || !wscale || !codes_t || !scale_t || !sal_t || (S_pad > 0 && !wsal))
     return SQMP_EINVAL;
-  if (dtype != SQMP_F16 && dtype != SQMP_BF16) return SQMP_EUNSUPPORTED;
+  // fp32: the few-row kernels' operand (sqmp_gemv_w4), J = 2
+  if (dtype != SQMP_F16 && dtype != SQMP_BF16 && !(dtype == SQMP_F32 && J == 2)) return SQMP_EUNSUPPORTED;
   if (N <= 0 || Kp <= 0 || Kp % 64 || S_pad < 0 || S_pad % 64 || ngw <= 0) return SQMP_EINVAL;
   if (J != 2 && J != 4) return SQMP_EINVAL;
   hipStream_t s = (hipStream_t)stream;
@@ -963,6 +964,9 @@ extern "C" int sqmp_pack_fq7(const void* codes, const void* wscale, const void* 
   if (dtype == SQMP_F16)
     fq7::pack_scales_kernel<_Float16><<<dim3((unsigned)cdiv(ts, 256)), dim3(256), 0, s>>>(
         (const _Float16*)wscale, (_Float16*)scale_t, Np, ngw, J, ts);
+  else if (dtype == SQMP_F32)
+    fq7::pack_scales_kernel<float><<<dim3((unsigned)cdiv(ts, 256)), dim3(256), 0, s>>>(
+        (const float*)wscale, (float*)scale_t, Np, ngw, J, ts);
   else
     fq7::pack_scales_kernel<__bf16><<<dim3((unsigned)cdiv(ts, 256)), dim3(256), 0, s>>>(
         (const __bf16*)wscale, (__bf16*)scale_t, Np, ngw, J, ts);
@@ -972,6 +976,9 @@ extern "C" int sqmp_pack_fq7(const void* codes, const void* wscale, const void* 
     if (dtype == SQMP_F16)
       fq7::pack_sal_kernel<_Float16><<<dim3((unsigned)cdiv(tsl, 256)), dim3(256), 0, s>>>(
           (const _Float16*)wsal, (_Float16*)sal_t, N, S_pad, J, tsl);
+    else if (dtype == SQMP_F32)
+      fq7::pack_sal_kernel<float><<<dim3((unsigned)cdiv(tsl, 256)), dim3(256), 0, s>>>(
+          (const float*)wsal, (float*)sal_t, N, S_pad, J, tsl);
     else
       fq7::pack_sal_kernel<__bf16><<<dim3((unsigned)cdiv(tsl, 256)), dim3(256), 0, s>>>(
           (const __bf16*)wsal, (__bf16*)sal_t, N, S_pad, J, tsl);

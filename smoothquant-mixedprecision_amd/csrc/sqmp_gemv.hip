@@ -1,0 +1,253 @@
+// Few-row products with 4-bit weights: y[m][n] = D( sum_p x[m][p] W[n][p] + bias[n] ),
+// 1 <= m <= 64 rows (the decoding form of fake_quant.py:306's F.linear), and the same per expert
+// of a mixture (ragged rows).  W = D(code * scale) at the Kp coded positions, then the S_pad
+// exact salient columns.
+//
+// What bounds it: the weight bytes (N Kp / 2 codes + scales), read once.  So a wave streams
+// whole 1-KiB stages of the tile-major codes straight into registers, decodes them there and
+// feeds the MFMA with the tokens in the B slot -- up to 16 tokens cost what one does.  A
+// workgroup owns one block of 32 weight rows and its NW waves take the K stages round robin
+// (consecutive stages are consecutive memory), each with U stages of loads in flight; the NW
+// partial sums meet in LDS and are added in a fixed order, so results do not depend on timing.
+#include "sqmp_w4.h"
+
+namespace sqmp {
+namespace w4 {
+
+struct GemvArgs {
+  const void* x;          // D rows of Kp + S_pad positions, row stride ldx elements
+  long ldx;
+  const uint32_t* codes;  // tile-major operands of one weight, or of E of them
+  const void* scale;
+  const void* sal;
+  const void* bias;       // D [N] or NULL
+  void* y;                // D [M][N_out]
+  int M, N;               // rows (dense form); weight rows (gated: gate and up rows together)
+  int Kp, S_pad, Gw, ngw;
+  // expert form
+  const int32_t* rows;     // slot -> flat (token * top_k + j), or NULL: x row = slot
+  const int32_t* offsets;  // [E + 1]
+  int top_k;
+  int n_out;               // columns of y (gated: N / 2 rounded; else N)
+};
+
+// GB: 1 = groups of whole 64-position stages, 2 = groups of 32, 0 = any multiple of 8
+// MT: 16-row token tiles per pass; NW waves; U stages in flight; ACT / EXP: the expert forms
+template <class DT, int GB, int MT, int NW, int U, bool EXP, int ACT>
+__global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
+  typedef typename DT::T T;
+  constexpr int RS = 36;  // floats per token row of a partial (32 + 4: spreads the LDS banks)
+  __shared__ __attribute__((aligned(16))) float red[NW * MT * 16 * RS];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int r16 = lane & 15, q = lane >> 4;
+  const int nb = blockIdx.x;
+  const int nblk = (a.N + 255) / 256 * 8;  // 32-row blocks of one weight's operands
+  const int nkm = a.Kp / 64, nks = a.S_pad / 64;
+  int lo = 0, hi = a.M;
+  long wb = nb;
+  if constexpr (EXP) {
+    lo = a.offsets[blockIdx.y];
+    hi = a.offsets[blockIdx.y + 1];
+    wb += (long)blockIdx.y * nblk;
+  }
+  const uint32_t* codes = a.codes + wb * nkm * 256 + lane * 4;
+  const T* scale = (const T*)a.scale + wb * a.ngw * 32 + r16 * 2;
+  const T* sal = (const T*)a.sal + wb * (nks > 0 ? nks : 1) * 2048 + lane * 32;
+  const DecK dk = make_deck();
+  const int c0 = 4 * (q & 1) + (q >> 1);  // chunk of s = 0; s = 1: + 2
+
+  for (int m0 = lo; m0 < hi; m0 += 16 * MT) {
+    // this lane's tokens (rows past the end repeat the last one; their columns of C are dropped)
+    const T* xp[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = min(m0 + 16 * i + r16, hi - 1);
+      long xr = m;
+      if constexpr (EXP) {
+        if (a.rows) xr = a.rows[m] / a.top_k;
+      }
+      xp[i] = (const T*)a.x + xr * a.ldx + 8 * c0;
+    }
+    f32x4 acc[MT][2];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    struct Stage {
+      u32x4 w;
+      T s[GB == 0 ? 4 : 2];  // scales of the two row halves (GB 0: for either s)
+      Frag<DT> x[MT][2];
+    };
+    auto load = [&](int kt, Stage& st) {
+      st.w = *(const u32x4*)(codes + (long)kt * 256);
+      if constexpr (GB == 0) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int g = min((kt * 64 + 8 * (c0 + 2 * s)) / a.Gw, a.ngw - 1);
+          st.s[2 * s] = scale[(long)g * 32];
+          st.s[2 * s + 1] = scale[(long)g * 32 + 1];
+        }
+      } else {
+        const int g = GB == 1 ? min((kt * 64) / a.Gw, a.ngw - 1) : min(2 * kt + (q & 1), a.ngw - 1);
+        st.s[0] = scale[(long)g * 32];
+        st.s[1] = scale[(long)g * 32 + 1];
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) st.x[i][s] = load_frag<DT>(xp[i] + (long)kt * 64 + 16 * s);
+    };
+    auto compute = [&](const Stage& st) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const Frag<DT> w = decode<DT>(st.w[2 * j + s], st.s[GB == 0 ? 2 * s + j : j], dk);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) mfma<DT>(acc[i][j], w, st.x[i][s]);
+        }
+    };
+    int kt = wave;
+    for (; kt + (U - 1) * NW < nkm; kt += U * NW) {
+      Stage st[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) load(kt + u * NW, st[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) compute(st[u]);
+    }
+    for (; kt < nkm; kt += NW) {
+      Stage st;
+      load(kt, st);
+      compute(st);
+    }
+    // the exact salient columns: operand fragments as they are
+    for (int kd = wave; kd < nks; kd += NW) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        Frag<DT> x[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[i] = load_frag<DT>(xp[i] + (long)(nkm + kd) * 64 + 16 * s);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const Frag<DT> w = load_frag<DT>(sal + (long)kd * 2048 + j * 16 + s * 8);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) mfma<DT>(acc[i][j], w, x[i]);
+        }
+      }
+    }
+    // partial sums to LDS: red[wave][token][row of the block]
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        *(f32x4*)(red + ((wave * MT + i) * 16 + r16) * RS + 16 * j + 4 * q) = acc[i][j];
+    __syncthreads();
+    const int nm = min(16 * MT, hi - m0);
+    constexpr int NO = ACT == ACT_NONE ? 32 : 16;  // outputs per token of this block
+    for (int t = threadIdx.x; t < nm * NO; t += NW * 64) {
+      const int m = t / NO, r = t % NO;
+      const int n = nb * NO + r;
+      float v = 0.f, u = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        v += red[(w * MT * 16 + m) * RS + r];
+        if constexpr (ACT != ACT_NONE) u += red[(w * MT * 16 + m) * RS + r + 16];
+      }
+      if (n >= a.n_out) continue;
+      if constexpr (ACT != ACT_NONE) v = act_fn<ACT>(v) * u;
+      if (a.bias) v += DT::to_f(((const T*)a.bias)[n]);
+      ((T*)a.y)[(long)(m0 + m) * a.n_out + n] = DT::from_f(v);
+    }
+    __syncthreads();  // the next pass writes red again
+  }
+}
+
+template <class DT, int GB, bool EXP, int ACT>
+static int launch(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
+  const int nb = cdiv(a.N, 32);
+  const dim3 grid(nb, EXP ? E : 1);
+#define SQMP_GV(MT, NW, U) \
+  gemv_kernel<DT, GB, MT, NW, U, EXP, ACT><<<grid, dim3(NW * 64), 0, s>>>(a)
+  if (max_rows <= 16) SQMP_GV(1, 8, 4);
+  else if (max_rows <= 32) SQMP_GV(2, 8, 2);
+  else SQMP_GV(4, 8, 1);
+#undef SQMP_GV
+  SQMP_LAUNCH_CHECK();
+  return SQMP_OK;
+}
+
+template <class DT, bool EXP, int ACT>
+static int by_group(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
+  if (a.Gw % 64 == 0) return launch<DT, 1, EXP, ACT>(a, E, max_rows, s);
+  if (a.Gw == 32) return launch<DT, 2, EXP, ACT>(a, E, max_rows, s);
+  if (a.Gw % 8 == 0) return launch<DT, 0, EXP, ACT>(a, E, max_rows, s);
+  return SQMP_EUNSUPPORTED;
+}
+
+static int check_operand(const void* x, long ldx, int dtype, int N, int Kp, int S_pad, int Gw,
+                         int ngw) {
+  if (N <= 0 || Kp <= 0 || Kp % 128 || S_pad < 0 || S_pad % 64 || Gw <= 0 || ngw <= 0)
+    return SQMP_EINVAL;
+  if (dtype != SQMP_F32 && dtype != SQMP_F16 && dtype != SQMP_BF16) return SQMP_EUNSUPPORTED;
+  const long per16 = dtype == SQMP_F32 ? 4 : 8;  // whole 16-byte loads of x
+  if (ldx < (long)Kp + S_pad || ldx % per16 || (size_t)x % 16) return SQMP_EINVAL;
+  return SQMP_OK;
+}
+
+}  // namespace w4
+
+extern "C" int sqmp_gemv_w4(const void* x, long ldx, const void* codes_t, const void* scale_t,
+                            const void* sal_t, const void* bias, void* y, int dtype, int M, int N,
+                            int Kp, int S_pad, int Gw, int ngw, void* stream) {
+  SQMP_DEVICE_GUARD(stream);
+  if (!x || !codes_t || !scale_t || !y || (S_pad > 0 && !sal_t)) return SQMP_EINVAL;
+  if (M < 0 || M > SQMP_GEMV_MAX_ROWS) return SQMP_EINVAL;
+  const int st = w4::check_operand(x, ldx, dtype, N, Kp, S_pad, Gw, ngw);
+  if (st != SQMP_OK) return st;
+  if (M == 0) return SQMP_OK;
+  w4::GemvArgs a{};
+  a.x = x, a.ldx = ldx, a.codes = (const uint32_t*)codes_t, a.scale = scale_t, a.sal = sal_t;
+  a.bias = bias, a.y = y, a.M = M, a.N = N, a.n_out = N;
+  a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == SQMP_F32) return w4::by_group<F32, false, w4::ACT_NONE>(a, 1, M, s);
+  if (dtype == SQMP_F16) return w4::by_group<F16, false, w4::ACT_NONE>(a, 1, M, s);
+  return w4::by_group<BF16, false, w4::ACT_NONE>(a, 1, M, s);
+}
+
+extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* rows, int top_k,
+                                     const int32_t* offsets, int E, const void* codes_t,
+                                     const void* scale_t, const void* sal_t, void* y, int dtype,
+                                     int slots, int N, int n_out, int Kp, int S_pad, int Gw,
+                                     int ngw, int act, void* stream) {
+  SQMP_DEVICE_GUARD(stream);
+  if (!x || !offsets || !codes_t || !scale_t || !y || (S_pad > 0 && !sal_t)) return SQMP_EINVAL;
+  if (slots < 0 || E <= 0 || E > 65535 || top_k <= 0) return SQMP_EINVAL;
+  if (act < w4::ACT_NONE || act > w4::ACT_GELU) return SQMP_EINVAL;
+  // gated: blocks of 16 gate and 16 up rows, n_out of the outputs kept
+  if (act != w4::ACT_NONE ? (N % 32 || n_out <= N / 2 - 16 || n_out > N / 2) : n_out != N)
+    return SQMP_EINVAL;
+  const int st = w4::check_operand(x, ldx, dtype, N, Kp, S_pad, Gw, ngw);
+  if (st != SQMP_OK) return st;
+  if (slots == 0) return SQMP_OK;
+  w4::GemvArgs a{};
+  a.x = x, a.ldx = ldx, a.codes = (const uint32_t*)codes_t, a.scale = scale_t, a.sal = sal_t;
+  a.y = y, a.N = N, a.n_out = n_out, a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
+  a.rows = rows, a.offsets = offsets, a.top_k = top_k;
+  hipStream_t s = (hipStream_t)stream;
+  const int est = cdiv(slots, E) * 2;  // rows of a busy expert (any count is right)
+#define SQMP_EX(DTT)                                                                  \
+  switch (act) {                                                                      \
+    case w4::ACT_SILU: return w4::by_group<DTT, true, w4::ACT_SILU>(a, E, est, s);    \
+    case w4::ACT_GELU: return w4::by_group<DTT, true, w4::ACT_GELU>(a, E, est, s);    \
+    default: return w4::by_group<DTT, true, w4::ACT_NONE>(a, E, est, s);              \
+  }
+  if (dtype == SQMP_F32) SQMP_EX(F32)
+  if (dtype == SQMP_F16) SQMP_EX(F16)
+  SQMP_EX(BF16)
+#undef SQMP_EX
+}
+
+}  // namespace sqmp

@@ -1,0 +1,303 @@
+"""Mixture-of-experts blocks with 4-bit expert weights: routing, the products grouped by expert,
+the way back, and the module that replaces a model's fused experts.
+
+    r = route(logits, top_k)                     # or plan_routes(ids, weights, num_experts)
+    h = expert_linear(x, gate_up, r, act="silu")  # [tokens * top_k, I], rows in expert order
+    z = expert_linear(h, down, r, rows="slot")
+    y = combine(z, r)                             # [tokens, H]
+
+The reference swaps every expert's w1 / w2 / w3 for a W4A4Linear
+(/root/reference/smoothquant/fake_quant.py:564-668); transformers >= 5 holds them as two 3-D
+parameters, which `pack_experts` packs and W4A4Experts computes.  Inference only; every function
+launches HIP kernels on the current stream of its tensors' device, without host
+synchronisation, and raises on host tensors.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+from torch import nn
+
+from . import _lib, ops
+from ._lib import check, load
+
+MAX_EXPERTS, MAX_TOP_K = 256, 16
+ACTS = {None: 0, "silu": 1, "gelu": 2}
+
+
+# ------------------------------------------------------------------ routing
+@dataclass
+class Routing:
+    """Which experts the tokens go to, and the (token, expert) pairs in expert order.  A pair is
+    f = token * top_k + j; an id of -1 means that nothing was chosen there."""
+    ids: torch.Tensor       # int32 [T, top_k]
+    weights: torch.Tensor   # fp32 [T, top_k]
+    offsets: torch.Tensor   # int32 [E + 1]: slots of expert e are offsets[e] .. offsets[e + 1]
+    rows: torch.Tensor      # int32 [T * top_k]: slot -> pair (-1 behind the last)
+    slots: torch.Tensor     # int32 [T * top_k]: pair -> slot (-1: nothing chosen)
+    num_experts: int
+
+    @property
+    def tokens(self) -> int:
+        return self.ids.shape[0]
+
+    @property
+    def top_k(self) -> int:
+        return self.ids.shape[1]
+
+
+def _plan_buffers(T: int, k: int, E: int, dev):
+    n = load().sqmp_route_workspace_bytes(T, E)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    i32 = dict(dtype=torch.int32, device=dev)
+    return (torch.empty(E + 1, **i32), torch.empty(T * k, **i32), torch.empty(T * k, **i32), ws, n)
+
+
+def _check_sizes(what: str, E: int, k: int):
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"{what}: {E} experts, supported are 1 .. {MAX_EXPERTS}")
+    if not 1 <= k <= MAX_TOP_K:
+        raise ValueError(f"{what}: top_k {k}, supported are 1 .. {MAX_TOP_K}")
+
+
+def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
+    """The top_k largest logits of every token [T, E] (ties: the lowest index; NaN counts as the
+    largest, -inf is never chosen) with their softmax weights -- over the chosen ones, or
+    over all E with normalize=False -- and the plan of plan_routes.  A token whose logits are all
+    -inf (padding) goes to no expert."""
+    ops._require_gpu(logits, "route")
+    if logits.dim() != 2:
+        raise ValueError(f"route: logits must be [tokens, experts], got {tuple(logits.shape)}")
+    T, E = logits.shape
+    _check_sizes("route", E, top_k)
+    if top_k > E:
+        raise ValueError(f"route: top_k {top_k} of {E} experts")
+    dt = ops._dtype_code(logits.dtype)
+    if logits.stride(1) != 1 or logits.stride(0) < E:
+        logits = logits.contiguous()
+    dev = logits.device
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    offsets, rows, slots, ws, n = _plan_buffers(T, top_k, E, dev)
+    p = ops._p
+    check(load().sqmp_route(p(logits), max(logits.stride(0), E), dt, T, E, top_k, int(normalize),
+                            p(weights), p(ids), p(offsets), p(rows), p(slots), p(ws), n,
+                            ops._stream(logits)), "route")
+    return Routing(ids, weights, offsets, rows, slots, E)
+
+
+def plan_routes(ids: torch.Tensor, weights: torch.Tensor, num_experts: int) -> Routing:
+    """The plan for a routing chosen elsewhere: ids [T, top_k] (any integer type; a value outside
+    0 .. num_experts - 1 means that nothing was chosen), weights [T, top_k].  The pairs of an expert
+    keep the order of the tokens."""
+    ops._require_gpu(ids, "plan_routes")
+    if ids.dim() != 2 or ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+        raise ValueError(f"plan_routes: ids must be integers [tokens, top_k], got {ids.dtype} "
+                         f"{tuple(ids.shape)}")
+    if weights.shape != ids.shape or weights.device != ids.device:
+        raise ValueError(f"plan_routes: weights {tuple(weights.shape)} on {weights.device} do not "
+                         f"match ids {tuple(ids.shape)} on {ids.device}")
+    T, k = ids.shape
+    _check_sizes("plan_routes", num_experts, k)
+    if ids.dtype != torch.int32:
+        ids = (ids.long().clamp(-1, num_experts)).to(torch.int32)  # (no id may wrap into range)
+    ids = ids.contiguous()
+    offsets, rows, slots, ws, n = _plan_buffers(T, k, num_experts, ids.device)
+    p = ops._p
+    check(load().sqmp_plan_routes(p(ids), T, num_experts, k, p(offsets), p(rows), p(slots), p(ws),
+                                  n, ops._stream(ids)), "plan_routes")
+    return Routing(ids, weights.float().contiguous(), offsets, rows, slots, num_experts)
+
+
+# ------------------------------------------------------------------ packed experts
+@dataclass
+class PackedExperts:
+    """E packed 4-bit weights of one shape (the tile-major operands of sqmp_expert_linear_w4)."""
+    codes_t: torch.Tensor            # uint8 [E, ...]
+    scale_t: torch.Tensor            # D [E, ...]
+    sal_t: Optional[torch.Tensor]    # D [E, ...], None without salient columns
+    amap: torch.Tensor               # int32 [Kp], or [E, Kp] where every expert has its own order
+    salient: Optional[torch.Tensor]  # int32 [S]
+    num_experts: int
+    n_out: int                       # columns of the product (gated: of act(gate) * up)
+    N: int                           # packed weight rows
+    K: int
+    Kp: int
+    S: int
+    S_pad: int
+    Gw: int
+    ngw: int
+    dtype: torch.dtype
+    gated: bool
+    identity: bool                   # the operand is x itself (columns' order, K == Kp)
+
+
+def _interleave(t: torch.Tensor) -> torch.Tensor:
+    """[2 I, ...] (gate rows, then up rows) -> 16 gate and 16 up rows in turn, I padded to 16."""
+    inter = t.shape[0] // 2
+    pad = (inter + 15) // 16 * 16
+    full = t.new_zeros((2, pad) + t.shape[1:])
+    full[0, :inter], full[1, :inter] = t[:inter], t[inter:]
+    return full.view((2, pad // 16, 16) + t.shape[1:]).transpose(0, 1).reshape((2 * pad,) + t.shape[1:])
+
+
+def _pack_all(weights, E: int, rows: int, gated: bool) -> PackedExperts:
+    """weights: iterator over the E experts' PackedWeight (rows interleaved where gated)."""
+    pe, maps = None, []
+    for e, pw in enumerate(weights):
+        if not ops.gemv_eligible(pw):
+            raise ValueError("pack_experts: needs 4-bit codes in groups of a multiple of 8 columns "
+                             f"(n_bits {pw.n_bits}, group {pw.Gw})")
+        one = ops.tile_major(pw.codes, pw.wscale, pw.wsal, pw.N, pw.Kp, pw.S_pad, pw.ngw, pw.dtype,
+                             None if pe is None else (pe.codes_t[e], pe.scale_t[e],
+                                                      all_sal[e]))
+        if pe is None:
+            stacks = [torch.empty((E,) + t.shape, dtype=t.dtype, device=t.device) for t in one]
+            for st, t in zip(stacks, one):
+                st[0] = t
+            all_sal = stacks[2]
+            pe = PackedExperts(stacks[0], stacks[1], all_sal if pw.S_pad else None, pw.amap,
+                               pw.salient, E, rows // 2 if gated else rows, pw.N, pw.K, pw.Kp,
+                               pw.S, pw.S_pad, pw.Gw, pw.ngw, pw.dtype, gated, False)
+        maps.append(pw.amap)
+    amap = torch.stack(maps)
+    if bool((amap == amap[0]).all()):  # (also on the first use of another stream: a sync)
+        amap = amap[0].contiguous()
+        pe.identity = pe.S == 0 and pe.Kp == pe.K and bool(
+            torch.equal(amap, torch.arange(pe.K, dtype=torch.int32, device=amap.device)))
+    pe.amap = amap
+    return pe
+
+
+def _check_stack(what: str, w: torch.Tensor, gated: bool):
+    ops._require_gpu(w, what)
+    if w.dim() != 3 or 0 in w.shape:
+        raise ValueError(f"{what}: expected [experts, rows, columns], got {tuple(w.shape)}")
+    if w.shape[0] > MAX_EXPERTS:
+        raise ValueError(f"{what}: {w.shape[0]} experts, at most {MAX_EXPERTS}")
+    if gated and w.shape[1] % 2:
+        raise ValueError(f"{what}: a gated weight has an even number of rows, got {w.shape[1]}")
+
+
+def pack_experts(w: torch.Tensor, weight_quant: str = "per_channel", group_size: int = 128,
+                 salient: Optional[torch.Tensor] = None, gated: bool = False) -> PackedExperts:
+    """Quantize w D [E, N, K] to 4 bits expert by expert (ops.pack_weight).  gated: the rows are
+    [gate; up] halves (transformers' gate_up_proj); their statistics (per_tensor, the column
+    order of the sorted modes) are taken over both.  salient: one set of exact columns for all."""
+    _check_stack("pack_experts", w, gated)
+    if weight_quant == "none":
+        raise ValueError("pack_experts: needs a quantized weight")
+    it = (ops.pack_weight(_interleave(w[e]) if gated else w[e], weight_quant, 4, group_size, salient)
+          for e in range(w.shape[0]))
+    return _pack_all(it, w.shape[0], w.shape[1], gated)
+
+
+def pack_expert_codes(codes: torch.Tensor, scales: torch.Tensor, group_size: int,
+                      gated: bool = False) -> PackedExperts:
+    """As ops.pack_codes for codes int8 [E, N, K] and scales D [E, N, ceil(K / group_size)]."""
+    _check_stack("pack_expert_codes", codes, gated)
+    if scales.dim() != 3 or scales.shape[:2] != codes.shape[:2]:
+        raise ValueError(f"pack_expert_codes: scales {tuple(scales.shape)} do not match codes "
+                         f"{tuple(codes.shape)}")
+    pick = _interleave if gated else (lambda t: t)
+    it = (ops.pack_codes(pick(codes[e]), pick(scales[e]), group_size)
+          for e in range(codes.shape[0]))
+    return _pack_all(it, codes.shape[0], codes.shape[1], gated)
+
+
+# ------------------------------------------------------------------ products
+def _operand(x: torch.Tensor, pe: PackedExperts, r: Routing, by_slot: bool):
+    """(operand, its slot -> pair list or None): x itself where the kernels can read it, a packed
+    copy of its rows, or -- where every expert has its own column order -- of every slot's row."""
+    rows = None if by_slot else r.rows
+    if pe.identity and ops._operand_rows(x, pe.Kp):
+        return x, rows
+    if x.stride(1) != 1:
+        x = x.contiguous()
+    L = pe.Kp + pe.S_pad
+    own = pe.amap.dim() == 2
+    n = r.rows.shape[0] if own else x.shape[0]
+    out = torch.empty((n, L), dtype=x.dtype, device=x.device)
+    p = ops._p
+    check(load().sqmp_pack_rows(p(x), max(x.stride(0), 1), ops._dtype_code(x.dtype), n, p(pe.amap),
+                                pe.Kp, p(pe.salient), pe.S, pe.S_pad, p(rows) if own else None,
+                                r.top_k, p(r.offsets) if own else None, pe.num_experts,
+                                pe.Kp if own else 0, p(out), ops._stream(x)), "pack_rows")
+    return out, None if own else rows
+
+
+def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Optional[str] = None,
+                  rows: str = "token", out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """z [tokens * top_k, n_out], rows in expert order: D(W_e x) for every (token, expert) pair, or
+    D(act(gate) * up) of a gated weight (act "silu" / "gelu"; fp32 up to the one rounding).
+
+    x: [tokens, K] (rows="token") or [tokens * top_k, K] already in expert order (rows="slot").
+    Rows of z behind routing.offsets[-1] (tokens that go nowhere) are left as they were."""
+    ops._require_gpu(x, "expert_linear")
+    if act not in ACTS:
+        raise ValueError(f"expert_linear: act must be one of {sorted(map(str, ACTS))}, got {act!r}")
+    if (act is not None) != pe.gated:
+        raise ValueError("expert_linear: an activation goes with a gated weight, and a gated weight "
+                         f"with an activation (act={act!r}, gated={pe.gated})")
+    if rows not in ("token", "slot"):
+        raise ValueError(f"expert_linear: rows must be 'token' or 'slot', got {rows!r}")
+    if routing.num_experts != pe.num_experts:
+        raise ValueError(f"expert_linear: routing over {routing.num_experts} experts, weight of "
+                         f"{pe.num_experts}")
+    S = routing.rows.shape[0]
+    want = (S if rows == "slot" else routing.tokens, pe.K)
+    if tuple(x.shape) != want:
+        raise ValueError(f"expert_linear: x must be {list(want)}, got {list(x.shape)}")
+    if x.dtype != pe.dtype:
+        raise RuntimeError(f"expected input dtype {pe.dtype}, got {x.dtype}")
+    if x.device != pe.codes_t.device or routing.rows.device != x.device:
+        raise RuntimeError(f"expert_linear: x on {x.device}, weight on {pe.codes_t.device}, routing "
+                           f"on {routing.rows.device}")
+    if out is None:
+        out = torch.empty((S, pe.n_out), dtype=pe.dtype, device=x.device)
+    elif (tuple(out.shape) != (S, pe.n_out) or out.dtype != pe.dtype or out.device != x.device
+          or not out.is_contiguous()):
+        raise ValueError(f"expert_linear: out must be contiguous {pe.dtype} [{S}, {pe.n_out}] on "
+                         f"{x.device}")
+    if S == 0:
+        return out
+    a, pairs = _operand(x, pe, routing, rows == "slot")
+    p = ops._p
+    check(load().sqmp_expert_linear_w4(p(a), a.stride(0) if a.shape[0] > 1 else pe.Kp + pe.S_pad,
+                                       p(pairs), routing.top_k, p(routing.offsets), pe.num_experts,
+                                       p(pe.codes_t), p(pe.scale_t), p(pe.sal_t), p(out),
+                                       ops._dtype_code(pe.dtype), S, pe.N, pe.n_out, pe.Kp,
+                                       pe.S_pad, pe.Gw, pe.ngw, ACTS[act], ops._stream(x)),
+          "expert_linear")
+    return out
+
+
+def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y [tokens, H]: y[t] = D(sum_j weights[t, j] * z[slot of pair (t, j)]), fp32 sums in the
+    order of j; a token that goes nowhere gets zeros."""
+    ops._require_gpu(z, "combine")
+    T, k = routing.tokens, routing.top_k
+    if z.dim() != 2 or z.shape[0] != T * k or z.shape[1] == 0:
+        raise ValueError(f"combine: z must be [{T * k}, H], got {tuple(z.shape)}")
+    dt = ops._dtype_code(z.dtype)
+    if routing.slots.device != z.device:
+        raise RuntimeError(f"combine: z on {z.device}, routing on {routing.slots.device}")
+    z = z.contiguous()
+    H = z.shape[1]
+    if out is None:
+        out = torch.empty((T, H), dtype=z.dtype, device=z.device)
+    elif (tuple(out.shape) != (T, H) or out.dtype != z.dtype or out.device != z.device
+          or not out.is_contiguous()):
+        raise ValueError(f"combine: out must be contiguous {z.dtype} [{T}, {H}] on {z.device}")
+    if T == 0:
+        return out
+    p = ops._p
+    check(load().sqmp_combine(p(z), dt, T, k, H, p(routing.slots), p(routing.weights), p(out),
+                              ops._stream(z)), "combine")
+    return out
+
+
+__all__ = ["Routing", "route", "plan_routes", "PackedExperts", "pack_experts", "pack_expert_codes",
+           "expert_linear", "combine"]

@@ -200,7 +200,7 @@ _PW_KEY = ("w_codes", "w_scale", "w_salient", "w_perm", "w_amap", "w_amap_fq", "
 # W4A4Linear (fake_quant.py:209-374)
 # ----------------------------------------------------------------------------------------
 # the forward kernels a module's `kernel` attribute selects (W4A4Linear docstring)
-KERNELS = ("auto", "fq", "f8", "fqt")
+KERNELS = ("auto", "fq", "f8", "fqt", "gemv")
 
 
 class W4A4Linear(nn.Module):
@@ -216,6 +216,9 @@ class W4A4Linear(nn.Module):
             in ACTIVATION order -- 4-bit act codes decoded in the GEMM, the weight W_hat
             permuted per forward, no salient zero positions in the K loop; the same
             operands bit for bit, so "fq"'s numerics.
+      "gemv" decoding: up to ops.GEMV_MAX_ROWS rows on the few-row kernel ("fq"'s operands, fp32
+            sums in another order), more rows and the weights it does not take as "auto"
+            (use_gemv switches a model's layers).
     """
 
     def __init__(self, in_features, out_features, bias=True, act_quant="per_token",
@@ -520,14 +523,16 @@ class W4A4Linear(nn.Module):
         if bias is not None and bias.device != x.device:
             raise RuntimeError(f"bias on {bias.device}, input on {x.device}: move the module "
                                "to the input's device")
-        use_f8 = self.kernel == "f8" or (
-            self.kernel == "auto" and ops.f8_auto(pw, amode, bits) and ops.f8_input_ok(xc))
-        use_fqt = (not use_f8 and self.kernel in ("auto", "fqt")
-                   and ops.fqt_eligible(pw, amode, bits, ag, x2.shape[0],
-                                        force=self.kernel == "fqt")
+        use_gemv = (self.kernel == "gemv" and x2.shape[0] <= ops.GEMV_MAX_ROWS
+                    and ops.gemv_eligible(pw))
+        kernel = "fq" if use_gemv else "auto" if self.kernel == "gemv" else self.kernel
+        use_f8 = kernel == "f8" or (
+            kernel == "auto" and ops.f8_auto(pw, amode, bits) and ops.f8_input_ok(xc))
+        use_fqt = (not use_f8 and kernel in ("auto", "fqt")
+                   and ops.fqt_eligible(pw, amode, bits, ag, x2.shape[0], force=kernel == "fqt")
                    and ops.f8_input_ok(xc))
         # fp32 layers: the quantizer writes sqmp_gemm_h2d's two f16 planes itself
-        use_h2 = (not use_f8 and not use_fqt and self.kernel == "auto"
+        use_h2 = (not use_f8 and not use_fqt and kernel == "auto"
                   and ops.h2_planes_ok(pw, amode, x2.shape[0], ag))
         # the in-place quantization of the caller's x is the GEMM operand itself when the
         # packed order is the column order (ops.identity_layout): one quantizer pass, not two
@@ -548,7 +553,7 @@ class W4A4Linear(nn.Module):
         if mutate_input and not f8_write_x:
             ops.fake_quant_inplace(xc, amode, bits, ag, pw.amap_fq, pw.nonsal, 0)
         if inplace_op:
-            a = xc if xc.shape[0] % 256 == 0 else ops.padded_operand(xc)
+            a = xc if use_gemv or xc.shape[0] % 256 == 0 else ops.padded_operand(xc)
         if ospec is not None and self.salient_indices is not None and pw.N != pw.K:
             raise IndexError(                                                # :311-314
                 f"The shape of the mask [{pw.K}] at index 0 does not match the shape "
@@ -558,6 +563,7 @@ class W4A4Linear(nn.Module):
         # y into the output quantizer's workspace, which then skips its statistics pass
         fuse = (ospec is not None and ospec[0] in ("per_group", "per_tensor") and _OQ_FUSE
                 and (not use_f8 or ops.f8_colmax_ok(pw))       # the 16x16x128 FP8 kernel
+                and not use_gemv
                 and (not use_fqt or c4[1].dim() == 3)          # the tile-major fqt7 GEMM
                 and (self.salient_indices is None or pw.K - pw.S > 0))
         colmax = ops.out_quant_workspace(x2.shape[0], pw.N, x2.device)["buf"] if fuse else None
@@ -567,6 +573,8 @@ class W4A4Linear(nn.Module):
             y = ops.gemm_fqt(*c4, pw, bias, ag, colmax=colmax)
         elif use_h2:
             y = ops.gemm_h2_planes(a2, pw, bias, colmax=colmax)
+        elif use_gemv:
+            y = ops.gemv(a, pw, bias, packed=True)
         else:
             y = ops.gemm_fq(a, pw, bias, colmax=colmax)
         if ospec is not None:                                                # :308-316
@@ -717,6 +725,17 @@ def link_siblings(*modules):
     for m in mods:
         m.__dict__["_sqmp_group"] = g
     return g
+
+
+def use_gemv(model: nn.Module, enable: bool = True) -> int:
+    """Switch the W4A4Linear layers of `model` whose kernel is "auto" to "gemv" (enable=False:
+    back) and return how many changed: a model that decodes a few tokens at a time."""
+    was, now = ("auto", "gemv") if enable else ("gemv", "auto")
+    n = 0
+    for m in model.modules():
+        if isinstance(m, W4A4Linear) and m.kernel == was:
+            m.kernel, n = now, n + 1
+    return n
 
 
 # ----------------------------------------------------------------------------------------

@@ -96,6 +96,7 @@ class PackedWeight:
     h2d: Optional[torch.Tensor] = field(default=None)    # f16 tile-major planes (gemm_h2d)
     sib_maps: Optional[tuple] = field(default=None)      # sibling position map (sqmp_permute_act)
     ident: Optional[bool] = field(default=None)          # packed order == column order (identity_layout)
+    gemv: Optional[tuple] = field(default=None)          # (codes_t, scale_t, sal_t) of gemv
 
     @property
     def gemm_operand(self):
@@ -971,3 +972,163 @@ def f8_auto(pw: PackedWeight, act_quant: str, act_bits: int) -> bool:
     return F8_AUTO and pw.dtype == torch.float16 and f8_eligible(pw, act_quant, act_bits)
 
 
+# ----------------------------------------------------------------------------------------
+# few rows: the decoding form of the faithful product
+# ----------------------------------------------------------------------------------------
+GEMV_MAX_ROWS = 64  # SQMP_GEMV_MAX_ROWS
+
+
+def bpack_codes(codes: torch.Tensor) -> torch.Tensor:
+    """int codes [R, Kp] in -8 .. 7 (Kp % 64 == 0) -> uint8 [R, Kp / 2] in the packed layout of
+    include/sqmp_w4a4.h: dword (h * 4 + u) of a 64-position block holds positions
+    16 u + 8 h + e, even e in the low half-word, odd e in the high one, nibble = code + 8."""
+    R, Kp = codes.shape
+    n = (codes.to(torch.int8) + 8).view(R, Kp // 64, 4, 2, 8)
+    w = torch.zeros((R, Kp // 64, 2, 4), dtype=torch.int32, device=codes.device)
+    for e in range(8):
+        sh = (16 if e & 1 else 0) + 4 * (e >> 1)
+        w |= (n[..., e].transpose(2, 3).to(torch.int32) & 15) << sh
+    return w.view(R, Kp // 8).view(torch.uint8)
+
+
+def pack_codes(codes: torch.Tensor, scales: torch.Tensor, group_size: int) -> PackedWeight:
+    """A PackedWeight from 4-bit codes that exist already (a checkpoint quantized elsewhere):
+    codes int8 [N, K] in -8 .. 7, scales D [N, ceil(K / group_size)], W = D(code * scale) with
+    the groups over consecutive columns; no salient columns, the columns' own order."""
+    _require_gpu(codes, "pack_codes")
+    if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.int8:
+        raise ValueError("pack_codes: codes must be int8 [N, K], scales [N, groups]")
+    N, K = codes.shape
+    if N == 0 or K == 0 or group_size <= 0:
+        raise ValueError(f"pack_codes: empty weight [{N}, {K}] or group size {group_size}")
+    if scales.device != codes.device:
+        raise RuntimeError(f"pack_codes: codes on {codes.device}, scales on {scales.device}")
+    _dtype_code(scales.dtype)
+    if scales.shape != (N, (K + group_size - 1) // group_size):
+        raise ValueError(f"pack_codes: scales {tuple(scales.shape)} do not match codes "
+                         f"{tuple(codes.shape)} in groups of {group_size}")
+    dev, dt = codes.device, scales.dtype
+    wmode = _lib.W_PER_CHANNEL if scales.shape[1] == 1 else _lib.W_PER_GROUP_UNSORTED
+    Kp, Gw, ngw, S_pad = geometry(K, 0, wmode, group_size)
+    Np = pad_n(N)
+    full = torch.zeros((Np, Kp), dtype=torch.int8, device=dev)
+    full[:N, :K] = codes
+    wscale = torch.zeros((ngw, Np), dtype=dt, device=dev)
+    wscale[:scales.shape[1], :N] = scales.t()
+    perm, amap, amap_fq, nonsal = build_maps(K, None, dev, Kp)
+    pw = PackedWeight(bpack_codes(full), wscale, torch.empty((N, 0), dtype=dt, device=dev), perm,
+                      amap, amap_fq, nonsal, None, N, K, 0, S_pad, Kp, Gw, ngw, 4, wmode, dt)
+    pw.posmap = torch.arange(K, dtype=torch.int32, device=dev)
+    pw.sal_key = salient_key(K, None)
+    pw.ident = Kp == K
+    if Gw % (4 if dt == torch.float32 else 8):
+        pw.dense = dequant_weight_packed(pw)
+    return pw
+
+
+def tile_major(codes: torch.Tensor, wscale: torch.Tensor, wsal: torch.Tensor, N: int, Kp: int,
+               S_pad: int, ngw: int, dtype: torch.dtype, out=None):
+    """sqmp_pack_fq7 (J = 2) of a packed 4-bit weight: (codes_t, scale_t, sal_t), into `out`
+    where given."""
+    sizes = [ctypes.c_size_t() for _ in range(3)]
+    check(load().sqmp_fq7_sizes(N, Kp, S_pad, ngw, 2, *[ctypes.byref(v) for v in sizes]),
+          "fq7_sizes")
+    if out is None:
+        dev = codes.device
+        out = (torch.empty(sizes[0].value, dtype=torch.uint8, device=dev),
+               torch.empty(sizes[1].value, dtype=dtype, device=dev),
+               torch.empty(sizes[2].value, dtype=dtype, device=dev))
+    if tuple(t.numel() for t in out) != tuple(v.value for v in sizes):
+        raise ValueError("tile_major: operands of another size")
+    check(load().sqmp_pack_fq7(_p(codes), _p(wscale), _p(wsal) if S_pad else None,
+                               _dtype_code(dtype), N, Kp, S_pad, ngw, 2, *[_p(t) for t in out],
+                               _stream(codes)), "pack_fq7")
+    return out
+
+
+def gemv_eligible(pw: PackedWeight) -> bool:
+    """Whether gemv computes this weight: 4-bit codes in groups of whole 8 positions."""
+    return pw.n_bits == 4 and pw.dense is None and pw.Gw % 8 == 0
+
+
+def gemv_operands(pw: PackedWeight):
+    """(codes_t, scale_t, sal_t) of gemv: fq7_operands' copies where those are J = 2 (fp16 /
+    bf16), else its own; built once per packed weight.  Inside a HIP-graph capture nothing is
+    kept (the copy would be written at replay only): call gemv once before capturing."""
+    if pw.gemv is None and pw.fq7 is not None and pw.fq7[3] == 2:
+        pw.gemv = pw.fq7[:3]
+    if pw.gemv is not None:
+        return pw.gemv
+    ops_t = tile_major(pw.codes, pw.wscale, pw.wsal, pw.N, pw.Kp, pw.S_pad, pw.ngw, pw.dtype)
+    if torch.cuda.is_current_stream_capturing():
+        return ops_t
+    # (built on this stream, read later from any other)
+    torch.cuda.current_stream(pw.codes.device).synchronize()
+    pw.gemv = ops_t
+    if pw.fq7 is None and FQ7_J == 2 and pw.dtype != torch.float32:
+        pw.fq7 = ops_t + (2,)
+    return ops_t
+
+
+def _operand_rows(x2: torch.Tensor, width: int):
+    """Whether the kernels read x2's rows in place: unit column stride, 16-B aligned rows."""
+    per = 16 // x2.element_size()
+    return (x2.stride(1) == 1 and x2.data_ptr() % 16 == 0
+            and (x2.shape[0] == 1 or (x2.stride(0) >= width and x2.stride(0) % per == 0)))
+
+
+def pack_rows(x2: torch.Tensor, amap: torch.Tensor, Kp: int, salient: Optional[torch.Tensor],
+              S: int, S_pad: int) -> torch.Tensor:
+    """x [M, K] -> [M, Kp + S_pad]: the unquantized activation operand (columns gathered by amap,
+    then the salient columns)."""
+    if x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    out = torch.empty((x2.shape[0], Kp + S_pad), dtype=x2.dtype, device=x2.device)
+    check(load().sqmp_pack_rows(_p(x2), max(x2.stride(0), 1), _dtype_code(x2.dtype), x2.shape[0],
+                                _p(amap), Kp, _p(salient), S, S_pad, None, 1, None, 0, 0, _p(out),
+                                _stream(x2)), "pack_rows")
+    return out
+
+
+def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
+         packed: bool = False) -> torch.Tensor:
+    """y [M, N] = D(x . W_hat^T + bias) for M <= GEMV_MAX_ROWS rows (the decoding form of
+    gemm_fq: the same operands, fp32 sums in another fixed order).
+
+    x: [M, K] in the columns' order -- a 4-bit weight with D activations -- or, with `packed`,
+    the [M, Kp + S_pad] operand of quant_act_fp.  Any strides; rows that are not 16-B aligned,
+    and packed weights in an order of their own, are copied first (sqmp_pack_rows)."""
+    _require_gpu(x, "gemv")
+    if x.dim() != 2:
+        raise ValueError(f"gemv: x must have 2 dimensions, got {tuple(x.shape)}")
+    M = x.shape[0]
+    L = pw.Kp + pw.S_pad
+    if x.shape[1] != (L if packed else pw.K):
+        raise ValueError(f"gemv: x has {x.shape[1]} columns, the weight {L if packed else pw.K}")
+    if M > GEMV_MAX_ROWS:
+        raise ValueError(f"gemv: {M} rows, at most {GEMV_MAX_ROWS}")
+    if not gemv_eligible(pw):
+        raise ValueError(f"gemv: needs 4-bit codes in groups of a multiple of 8 columns (n_bits "
+                         f"{pw.n_bits}, group {pw.Gw})")
+    if x.dtype != pw.dtype:
+        raise RuntimeError(f"expected input dtype {pw.dtype}, got {x.dtype}")
+    if x.device != pw.codes.device:
+        raise RuntimeError(f"gemv: x on {x.device}, the weight on {pw.codes.device}")
+    if bias is not None:
+        if bias.dtype != pw.dtype or bias.device != x.device or bias.numel() != pw.N:
+            raise RuntimeError(f"gemv: bias {bias.dtype} [{bias.numel()}] on {bias.device} does "
+                               f"not match {pw.dtype} [{pw.N}] on {x.device}")
+        bias = bias.reshape(-1).contiguous()
+    y = torch.empty((M, pw.N), dtype=pw.dtype, device=x.device)
+    if M == 0:
+        return y
+    codes_t, scale_t, sal_t = gemv_operands(pw)
+    if not (packed or identity_layout(pw)):
+        x = pack_rows(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
+    elif not _operand_rows(x, L):
+        x = x.clone(memory_format=torch.contiguous_format)
+    check(load().sqmp_gemv_w4(_p(x), L if M == 1 else x.stride(0), _p(codes_t), _p(scale_t),
+                              _p(sal_t) if pw.S_pad else None, _p(bias), _p(y),
+                              _dtype_code(pw.dtype), M, pw.N, pw.Kp, pw.S_pad, pw.Gw, pw.ngw,
+                              _stream(x)), "gemv")
+    return y
