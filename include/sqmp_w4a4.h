@@ -445,11 +445,11 @@ int sqmp_plan_routes(const int32_t* ids, int T, int E, int top_k, int32_t* offse
  * n_out == N.  act = 1 (silu) / 2 (gelu, the error-function form): the N weight rows are 16 gate
  * and 16 up rows in turn, z = D( act(gate) * up ), n_out of the N / 2 columns are written.
  * slots = rows of z (an upper bound of offsets[E]); rows of z behind offsets[E] are left as they
- * were.  */
+ * were.  x_rows: rows of x. */
 int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* rows, int top_k,
                           const int32_t* offsets, int E, const void* codes_t, const void* scale_t,
-                          const void* sal_t, void* y, int dtype, int slots, int N, int n_out,
-                          int Kp, int S_pad, int Gw, int ngw, int act, void* stream);
+                          const void* sal_t, void* y, int dtype, int slots, int x_rows, int N,
+                          int n_out, int Kp, int S_pad, int Gw, int ngw, int act, void* stream);
 
 /* y[t] = D( sum_j weights[t][j] * z[slots[t][j]] ), fp32 sums in the order of j; slots < 0 are
  * skipped.  z D [slots][H], y D [T][H]. */

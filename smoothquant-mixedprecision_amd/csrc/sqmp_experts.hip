@@ -1,0 +1,307 @@
+// Products grouped by expert for many rows: z[slot] = D( W_e x[row(slot)] ) over the ragged
+// segments offsets[e] .. offsets[e + 1], W_e = D(code * scale) (+ exact salient columns), or
+// D( act(gate) * up ) for weights whose rows are 16 gate and 16 up rows in turn.
+//
+// What bounds it: the MFMA (2 slots N K flops), with the LDS reads of the activation tile close
+// behind.  A workgroup of 8 waves computes up to 256 slots of one expert by 256 weight rows:
+//   * each wave owns 32 weight rows; their codes and scales go straight from the tile-major
+//     operands to registers, two stages ahead, and are decoded there -- a decoded fragment feeds
+//     all the tile's tokens, and no weight passes through LDS;
+//   * the activation rows go to a three-slot LDS ring by LDS-DMA, gathered by the slot -> row
+//     list as they are loaded, so the tokens are never copied into expert order;
+//   * the last tile of an expert runs 64, 128 or 192 rows (TM), so a ragged segment wastes less
+//     than 64 rows of MFMA;
+//   * gate and up rows of one output are the two accumulators of one lane: the activation and the
+//     product happen in registers, half the output bytes, no second launch.
+// The grid holds every tile that any split of `slots` over the experts can need; the tiles that
+// exist are found from the offsets on the GPU (no host synchronisation), the rest return.
+#include "sqmp_w4_launch.h"
+
+namespace sqmp {
+namespace w4 {
+
+typedef int rsrc_t __attribute__((ext_vector_type(4)));
+
+__device__ inline rsrc_t make_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t a = (uint64_t)(size_t)base;
+  rsrc_t r;
+  r[0] = (int)__builtin_amdgcn_readfirstlane((uint32_t)a);
+  r[1] = (int)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xFFFFu);
+  r[2] = (int)__builtin_amdgcn_readfirstlane(bytes);
+  r[3] = 0x00020000;
+  return r;
+}
+
+// LDS-DMA of 16 B per lane to the wave-uniform LDS base + 16 * lane (no register output: nothing
+// of it is in flight that the compiler could reuse).  From asm, because the compiler would wait
+// for every LDS-DMA before the next LDS read; s_nop 0: the wait state after the M0 write.
+__device__ inline void dma16(const rsrc_t& r, uint32_t voff, uint32_t soff, unsigned char* lds) {
+  const uint32_t m0v = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m0v),
+               "v"(voff), "s"(r), "s"(soff)
+               : "memory", "m0");
+}
+template <int N>
+__device__ inline void vmwait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ inline void barrier() {
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");  // no LDS read moves above the barrier
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ inline int brev3(int c) { return ((c & 1) << 2) | (c & 2) | ((c >> 2) & 1); }
+
+constexpr int TILE_ROWS = 256;   // slots per tile
+constexpr int TILE_N = 256;      // weight rows per tile
+constexpr int RING = 3;
+
+// The tile of workgroup `bid`: expert e, slots [m0, m1), weight tile tn; false: no such tile.
+// Tiles are ordered by expert, groups of up to 4 row tiles, weight tile, row tile (the row tiles
+// of a group read the same weights), in contiguous runs per XCD.
+__device__ inline bool find_tile(const int32_t* offsets, int E, int tiles_n, int bid, int& e,
+                                 int& m0, int& m1, int& tn) {
+  const int lane = threadIdx.x & 63;
+  const int per = (E + 63) >> 6;  // experts per lane (E <= 256: at most 4)
+  const int e0 = lane * per;
+  int off[5], cnt = 0;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) off[i] = offsets[min(e0 + min(i, per), E)];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < per) cnt += (off[i + 1] - off[i] + TILE_ROWS - 1) / TILE_ROWS;
+  int incl = cnt;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += v;
+  }
+  const int nwg = __builtin_amdgcn_readfirstlane(__shfl(incl, 63, 64)) * tiles_n;
+  if (bid >= nwg) return false;
+  const int xcd = bid & 7, q = nwg >> 3, r = nwg & 7;
+  const int wg = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
+  // the lane, then the expert within it, whose tiles hold wg
+  const uint64_t mask = __ballot(incl * tiles_n > wg);
+  const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)mask) - 1);
+  int rem = wg - __shfl(incl - cnt, src, 64) * tiles_n;
+  int found = 0, lo = 0, hi = 0, done = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int a = __shfl(off[i], src, 64), b = __shfl(off[i + 1], src, 64);
+    const int t = i < per ? (b - a + TILE_ROWS - 1) / TILE_ROWS * tiles_n : 0;
+    if (!done && rem < t) found = src * per + i, lo = a, hi = b, done = 1;
+    if (!done) rem -= t;
+  }
+  const int tiles_m = (hi - lo + TILE_ROWS - 1) / TILE_ROWS;
+  const int gid = rem / (4 * tiles_n), first = gid * 4, gsz = min(tiles_m - first, 4);
+  const int in_g = rem - gid * 4 * tiles_n;
+  e = __builtin_amdgcn_readfirstlane(found);
+  m0 = __builtin_amdgcn_readfirstlane(lo + (first + in_g % gsz) * TILE_ROWS);
+  m1 = __builtin_amdgcn_readfirstlane(min(hi, lo + (first + in_g % gsz + 1) * TILE_ROWS));
+  tn = __builtin_amdgcn_readfirstlane(in_g / gsz);
+  return true;
+}
+
+// One tile of 16 I slots (I / 4 LDS-DMA pieces per wave and stage)
+template <class DT, int GB, bool GATED, int I>
+__device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int nm, int tn,
+                                unsigned char* lds) {
+  typedef typename DT::T T;
+  constexpr int J = 2, NA = I / 4, PF = I == 16 ? 2 : 3;
+  constexpr int SLOT = I * 16 * 128;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int r16 = lane & 15, q = lane >> 4;
+  const int nkm = a.Kp / 64, nks = a.S_pad / 64, nkt = nkm + nks;
+
+  // activation rows: piece i of a wave = rows 64 i + 8 wave + (lane >> 3); the lane brings the
+  // chunk that belongs at physical place lane & 7 of its row (chunk c at brev3(c) ^ (row / 2))
+  const T* xb = (const T*)a.x;
+  if (!a.rows) xb += (long)m0 * a.ldx;
+  const rsrc_t rA = make_rsrc(xb, 0xFFFFFFFFu);
+  uint32_t a_off[NA];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) {
+    const int row = 64 * i + 8 * wave + (lane >> 3);
+    const int rr = min(row, nm - 1);  // (rows past the segment repeat its last one)
+    const long xr = a.rows ? a.rows[m0 + rr] / a.top_k : rr;
+    a_off[i] = (uint32_t)(xr * a.ldx * (long)sizeof(T)) +
+               (uint32_t)(brev3((lane & 7) ^ ((row >> 1) & 7)) << 4);
+  }
+  auto issue_a = [&](int kt) {
+    unsigned char* slot = lds + (kt % RING) * SLOT + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) dma16(rA, a_off[i], (uint32_t)kt * 128, slot + i * 8192);
+  };
+
+  // weights
+  const long wb = (long)e * ((a.N + 255) / 256 * 8) + tn * 8 + wave;
+  const uint32_t* codes = a.codes + wb * nkm * 256 + lane * 4;
+  const T* scale = (const T*)a.scale + wb * a.ngw * 32 + r16 * 2;
+  struct Codes {
+    u32x4 w;
+    uint32_t s;
+  };
+  auto load_w = [&](int kt, Codes& c) {
+    c.w = *(const u32x4*)(codes + (long)kt * 256);
+    const int g = GB == 1 ? min((kt * 64) / a.Gw, a.ngw - 1) : min(2 * kt + (q & 1), a.ngw - 1);
+    c.s = *(const uint32_t*)(scale + (long)g * 32);
+  };
+
+  f32x4 acc[I][J];
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const DecK dk = make_deck();
+  uint32_t a_lo[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    a_lo[s] = (uint32_t)(r16 * 128 + ((brev3(4 * (q & 1) + 2 * s + (q >> 1)) ^ ((r16 >> 1) & 7)) << 4));
+  auto lda = [&](const unsigned char* slot, int t) {
+    return *(const u32x4*)(slot + (t % I) * 2048 + a_lo[t / I]);
+  };
+  // 2 I blocks (sub-step t / I, token tile t % I) with the fragments read PF blocks ahead
+  auto blocks = [&](const unsigned char* slot, auto bf, auto hook) {
+    u32x4 f[PF + 1];
+#pragma unroll
+    for (int t = 0; t < PF; ++t) f[t] = lda(slot, t);
+#pragma unroll
+    for (int t = 0; t < 2 * I; ++t) {
+      if (t + PF < 2 * I) f[(t + PF) % (PF + 1)] = lda(slot, t + PF);
+#pragma unroll
+      for (int j = 0; j < J; ++j) Mfma<DT>::run(acc[t % I][j], bf(t / I, j), f[t % (PF + 1)]);
+      hook(t);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // The decode of stage kt comes before the next activation loads are issued: the compiler waits
+  // for the codes by counting its own loads, and would otherwise wait for those as well.
+  Codes cs[2];
+  issue_a(0);
+  load_w(0, cs[0]);
+  if (nkt > 1) issue_a(1);
+  load_w(1, cs[1]);  // (nkm is even)
+  auto step = [&](int kt, Codes& c) {
+    uint32_t sp[J];
+    sp[0] = Dec<DT>::prep(c.s & 0xFFFFu), sp[1] = Dec<DT>::prep(c.s >> 16);
+    u32x4 bf[2][J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) bf[0][j] = Dec<DT>::run(c.w[2 * j], sp[j], dk);
+    // at most the NA youngest loads outstanding: stage kt's activations are older than those
+    if (kt + 1 < nkt) vmwait<NA>(); else vmwait<0>();
+    barrier();  // everyone's part of stage kt is in LDS, and nobody reads stage kt - 1 any more
+    if (kt + 2 < nkt) issue_a(kt + 2);
+    blocks(lds + (kt % RING) * SLOT, [&](int s, int j) -> const u32x4& { return bf[s][j]; },
+           [&](int t) {
+             if (t < J) bf[1][t] = Dec<DT>::run(c.w[2 * t + 1], sp[t], dk);
+           });
+    if (kt + 2 < nkm) load_w(kt + 2, c);
+  };
+  for (int kt = 0; kt < nkm; kt += 2) {
+    step(kt, cs[0]);
+    step(kt + 1, cs[1]);
+  }
+  // the exact salient columns: fragments as they are
+  for (int kd = 0; kd < nks; ++kd) {
+    const int kt = nkm + kd;
+    const T* sal = (const T*)a.sal + (wb * nks + kd) * 2048 + lane * 32;
+    u32x4 d[2][J];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int j = 0; j < J; ++j) d[s][j] = *(const u32x4*)(sal + j * 16 + s * 8);
+    if (kt + 1 < nkt) vmwait<NA>(); else vmwait<0>();
+    barrier();
+    if (kt + 2 < nkt) issue_a(kt + 2);
+    blocks(lds + (kt % RING) * SLOT, [&](int s, int j) -> const u32x4& { return d[s][j]; },
+           [](int) {});
+  }
+
+  // epilogue: the tile in LDS (16-B chunk c of row m at c ^ (m & 15)), then whole rows out
+  constexpr int TNO = GATED ? TILE_N / 2 : TILE_N;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  barrier();
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const int m = 16 * i + r16;
+#pragma unroll
+    for (int j = 0; j < (GATED ? 1 : J); ++j) {
+      const int nl = GATED ? 16 * wave + 4 * q : 32 * wave + 16 * j + 4 * q;
+      T v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float f = acc[i][j][r];
+        if constexpr (GATED)
+          f = (act == ACT_SILU ? act_fn<ACT_SILU>(f) : act_fn<ACT_GELU>(f)) * acc[i][1][r];
+        v[r] = DT::from_f(f);
+      }
+      *(uint64_t*)(lds + m * (TNO * 2) + (((nl >> 3) ^ (m & 15)) << 4) + (nl & 4) * 2) = *(const uint64_t*)v;
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  barrier();
+  constexpr int CPR = TNO / 8;
+  const int n0 = tn * TNO;
+  T* y = (T*)a.y + (long)m0 * a.n_out + n0;
+  const bool vec = a.n_out % 8 == 0 && (size_t)a.y % 16 == 0;
+  for (int k = threadIdx.x; k < nm * CPR; k += 512) {
+    const int m = k / CPR, c = k % CPR;
+    const u32x4 val = *(const u32x4*)(lds + m * (TNO * 2) + ((c ^ (m & 15)) << 4));
+    const int n = n0 + 8 * c;
+    if (vec) {
+      if (n < a.n_out) *(u32x4*)(y + (long)m * a.n_out + 8 * c) = val;
+    } else {
+      const T* v = (const T*)&val;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < a.n_out) y[(long)m * a.n_out + 8 * c + i] = v[i];
+    }
+  }
+}
+
+template <class DT, int GB, bool GATED>
+__global__ __launch_bounds__(512, 1) void expert_tiles_kernel(const GemvArgs a, int E, int tiles_n,
+                                                              int act) {
+  constexpr int EPI = TILE_ROWS * (GATED ? TILE_N / 2 : TILE_N) * 2;
+  constexpr int BYTES = RING * TILE_ROWS * 128 > EPI ? RING * TILE_ROWS * 128 : EPI;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[BYTES];
+  int e, m0, m1, tn;
+  if (!find_tile(a.offsets, E, tiles_n, blockIdx.x, e, m0, m1, tn)) return;
+  const int nm = m1 - m0;
+  if (nm > 192) run_tile<DT, GB, GATED, 16>(a, act, e, m0, nm, tn, lds);
+  else if (nm > 128) run_tile<DT, GB, GATED, 12>(a, act, e, m0, nm, tn, lds);
+  else if (nm > 64) run_tile<DT, GB, GATED, 8>(a, act, e, m0, nm, tn, lds);
+  else run_tile<DT, GB, GATED, 4>(a, act, e, m0, nm, tn, lds);
+}
+
+template <class DT, int GB>
+static int launch_tiles(const GemvArgs& a, int E, int slots, int act, hipStream_t s) {
+  const int tiles_n = cdiv(a.N, TILE_N);
+  const long tiles_m = (long)slots / TILE_ROWS + (slots < E ? slots : E);
+  const long grid = tiles_m * tiles_n;
+  if (grid > 0x7FFFFFFFL) return SQMP_EUNSUPPORTED;
+  if (act != ACT_NONE)
+    expert_tiles_kernel<DT, GB, true><<<dim3((unsigned)grid), dim3(512), 0, s>>>(a, E, tiles_n, act);
+  else
+    expert_tiles_kernel<DT, GB, false><<<dim3((unsigned)grid), dim3(512), 0, s>>>(a, E, tiles_n, act);
+  SQMP_LAUNCH_CHECK();
+  return SQMP_OK;
+}
+
+bool expert_tiles_ok(const GemvArgs& a, int dtype, int E, long x_rows) {
+  // fp16 / bf16, groups of 32 or of whole stages, a 32-bit offset to every activation
+  return (dtype == SQMP_F16 || dtype == SQMP_BF16) && (a.Gw % 64 == 0 || a.Gw == 32) && E <= 256 &&
+         (a.rows ? x_rows : TILE_ROWS) * a.ldx * 2 < 0xFFFF0000L;
+}
+
+int launch_expert_tiles(const GemvArgs& a, int dtype, int E, int slots, int act, hipStream_t s) {
+  if (dtype == SQMP_F16)
+    return a.Gw == 32 ? launch_tiles<F16, 2>(a, E, slots, act, s) : launch_tiles<F16, 1>(a, E, slots, act, s);
+  return a.Gw == 32 ? launch_tiles<BF16, 2>(a, E, slots, act, s) : launch_tiles<BF16, 1>(a, E, slots, act, s);
+}
+
+}  // namespace w4
+}  // namespace sqmp

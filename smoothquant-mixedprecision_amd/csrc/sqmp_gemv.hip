@@ -9,27 +9,10 @@
 // workgroup owns one block of 32 weight rows and its NW waves take the K stages round robin
 // (consecutive stages are consecutive memory), each with U stages of loads in flight; the NW
 // partial sums meet in LDS and are added in a fixed order, so results do not depend on timing.
-#include "sqmp_w4.h"
+#include "sqmp_w4_launch.h"
 
 namespace sqmp {
 namespace w4 {
-
-struct GemvArgs {
-  const void* x;          // D rows of Kp + S_pad positions, row stride ldx elements
-  long ldx;
-  const uint32_t* codes;  // tile-major operands of one weight, or of E of them
-  const void* scale;
-  const void* sal;
-  const void* bias;       // D [N] or NULL
-  void* y;                // D [M][N_out]
-  int M, N;               // rows (dense form); weight rows (gated: gate and up rows together)
-  int Kp, S_pad, Gw, ngw;
-  // expert form
-  const int32_t* rows;     // slot -> flat (token * top_k + j), or NULL: x row = slot
-  const int32_t* offsets;  // [E + 1]
-  int top_k;
-  int n_out;               // columns of y (gated: N / 2 rounded; else N)
-};
 
 // GB: 1 = groups of whole 64-position stages, 2 = groups of 32, 0 = any multiple of 8
 // MT: 16-row token tiles per pass; NW waves; U stages in flight; ACT / EXP: the expert forms
@@ -220,11 +203,11 @@ extern "C" int sqmp_gemv_w4(const void* x, long ldx, const void* codes_t, const 
 extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* rows, int top_k,
                                      const int32_t* offsets, int E, const void* codes_t,
                                      const void* scale_t, const void* sal_t, void* y, int dtype,
-                                     int slots, int N, int n_out, int Kp, int S_pad, int Gw,
+                                     int slots, int x_rows, int N, int n_out, int Kp, int S_pad, int Gw,
                                      int ngw, int act, void* stream) {
   SQMP_DEVICE_GUARD(stream);
   if (!x || !offsets || !codes_t || !scale_t || !y || (S_pad > 0 && !sal_t)) return SQMP_EINVAL;
-  if (slots < 0 || E <= 0 || E > 65535 || top_k <= 0) return SQMP_EINVAL;
+  if (slots < 0 || x_rows < 0 || E <= 0 || E > 65535 || top_k <= 0) return SQMP_EINVAL;
   if (act < w4::ACT_NONE || act > w4::ACT_GELU) return SQMP_EINVAL;
   // gated: blocks of 16 gate and 16 up rows, n_out of the outputs kept
   if (act != w4::ACT_NONE ? (N % 32 || n_out <= N / 2 - 16 || n_out > N / 2) : n_out != N)
@@ -237,6 +220,8 @@ extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* row
   a.y = y, a.N = N, a.n_out = n_out, a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
   a.rows = rows, a.offsets = offsets, a.top_k = top_k;
   hipStream_t s = (hipStream_t)stream;
+  if (w4::expert_tiles_ok(a, dtype, E, x_rows) && slots >= 16 * E)
+    return w4::launch_expert_tiles(a, dtype, E, slots, act, s);
   const int est = cdiv(slots, E) * 2;  // rows of a busy expert (any count is right)
 #define SQMP_EX(DTT)                                                                  \
   switch (act) {                                                                      \

@@ -100,7 +100,7 @@ SIGNATURES = {
     "sqmp_route": (_i, [_vp, _l, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "sqmp_plan_routes": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "sqmp_expert_linear_w4": (_i, [_vp, _l, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i,
-                                   _i, _i, _i, _i, _i, _vp]),
+                                   _i, _i, _i, _i, _i, _i, _vp]),
     "sqmp_combine": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "sqmp_pack_rows": (_i, [_vp, _l, _i, _i, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _l, _vp,
                             _vp]),

@@ -268,7 +268,7 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
     check(load().sqmp_expert_linear_w4(p(a), a.stride(0) if a.shape[0] > 1 else pe.Kp + pe.S_pad,
                                        p(pairs), routing.top_k, p(routing.offsets), pe.num_experts,
                                        p(pe.codes_t), p(pe.scale_t), p(pe.sal_t), p(out),
-                                       ops._dtype_code(pe.dtype), S, pe.N, pe.n_out, pe.Kp,
+                                       ops._dtype_code(pe.dtype), S, a.shape[0], pe.N, pe.n_out, pe.Kp,
                                        pe.S_pad, pe.Gw, pe.ngw, ACTS[act], ops._stream(x)),
           "expert_linear")
     return out
