@@ -299,5 +299,173 @@ def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = Non
     return out
 
 
+# ------------------------------------------------------------------ the module
+_TENSORS = ("codes_t", "scale_t", "sal_t", "amap", "salient")
+_INTS = ("num_experts", "n_out", "N", "K", "Kp", "S", "S_pad", "Gw", "ngw", "gated", "identity")
+# activation quantizers that look at one row at a time: they do not depend on which rows an expert
+# gets (the sorted and per_tensor ones take statistics over an expert's whole batch)
+ROW_ACTS = ("per_token", "per_group_unsorted")
+
+
+def _act_name(fn) -> str:
+    """The name of a gated MLP's activation module."""
+    name = type(fn).__name__
+    if isinstance(fn, nn.SiLU) or name == "SiLUActivation":
+        return "silu"
+    if (isinstance(fn, nn.GELU) and fn.approximate == "none") or name == "GELUActivation":
+        return "gelu"
+    raise ValueError(f"W4A4Experts: activation {name} (supported: silu, gelu)")
+
+
+class W4A4Experts(nn.Module):
+    """Drop-in for transformers' fused experts (gate_up_proj [E, 2 I, H], down_proj [E, H, I];
+    forward(hidden_states, top_k_index, top_k_weights)) with 4-bit weights and row-wise 4-bit
+    activations: what fake_quant.py:564-668 does to the experts' separate w1 / w3 / w2, as two
+    products grouped by expert.  act(gate) * up is formed in fp32 and rounded once (the reference
+    rounds gate, up and act(gate) to the model's type first); the experts' outputs are weighted and
+    summed in fp32."""
+
+    EXTRA_FORMAT = "sqmp-w4a4-experts/1"
+
+    def __init__(self, act: str = "silu", act_quant: Optional[str] = "per_token",
+                 quant_bits: int = 4, group_size: int = 128):
+        super().__init__()
+        if act not in ("silu", "gelu"):
+            raise ValueError(f"W4A4Experts: activation {act!r} (supported: silu, gelu)")
+        if act_quant is not None and act_quant not in ROW_ACTS:
+            raise ValueError(f"Invalid act_quant: {act_quant} (experts quantize row by row: "
+                             f"{', '.join(ROW_ACTS)} or None)")
+        if quant_bits != 4:
+            raise ValueError(f"quant_bits={quant_bits}: packed experts support 4 bits")
+        self.act, self.act_quant, self.quant_bits, self.group_size = act, act_quant, quant_bits, group_size
+        self.weight_quant = "None"
+        self._meta = None
+        for part in ("gate_up", "down"):
+            for n in _TENSORS:
+                self.register_buffer(f"{part}_{n}", None)
+
+    # -------------------------------------------------------------- packing
+    @staticmethod
+    def from_float(module, weight_quant="per_channel", act_quant="per_token", importance=None,
+                   salient_prop=0, quant_bits=4, group_size=128):
+        """module: the fused experts.  importance [H] picks the salient columns of gate_up_proj
+        (one set for all experts, as W4A4Linear picks them)."""
+        for n in ("gate_up_proj", "down_proj", "act_fn"):
+            if not hasattr(module, n):
+                raise ValueError(f"W4A4Experts: {type(module).__name__} has no fused {n}")
+        new = W4A4Experts(_act_name(module.act_fn), act_quant, quant_bits, group_size)
+        if not torch.cuda.is_available():
+            raise RuntimeError("W4A4Experts packing needs a ROCm GPU (no CPU implementation)")
+        gate_up, down = module.gate_up_proj.data, module.down_proj.data
+        dev = gate_up.device
+        salient = None
+        if importance is not None and salient_prop > 0:
+            order = torch.argsort(importance, descending=True, stable=True)
+            salient = order[:max(1, int(salient_prop * len(order)))]
+        gpu = dev if dev.type == "cuda" else torch.device("cuda")
+        new._install("gate_up", pack_experts(gate_up.to(gpu), weight_quant, group_size, salient, gated=True))
+        new._install("down", pack_experts(down.to(gpu), weight_quant, group_size))
+        new.weight_quant = weight_quant
+        return new if dev == gpu else new.to(dev)
+
+    def _install(self, part: str, pe: PackedExperts):
+        for n in _TENSORS:
+            setattr(self, f"{part}_{n}", getattr(pe, n))
+        meta = dict(self._meta or {}, dtype=pe.dtype)
+        meta.update({f"{part}_{n}": getattr(pe, n) for n in _INTS})
+        self._meta = meta
+        self.__dict__.pop("_packed", None)
+
+    def packed(self):
+        """(gate_up, down) as PackedExperts, and the column maps of the input's quantizer."""
+        b = tuple(getattr(self, f"{part}_{n}") for part in ("gate_up", "down") for n in _TENSORS)
+        c = self.__dict__.get("_packed")
+        if c is not None and all(x is y for x, y in zip(c[0], b)):
+            return c[1]
+        if self._meta is None:
+            raise RuntimeError("W4A4Experts has no packed weight")
+        pes = []
+        for part in ("gate_up", "down"):
+            kw = {n: getattr(self, f"{part}_{n}") for n in _TENSORS}
+            kw.update({n: self._meta[f"{part}_{n}"] for n in _INTS})
+            pes.append(PackedExperts(dtype=self._meta["dtype"], **kw))
+        dev = pes[0].codes_t.device
+        maps = [ops.build_maps(pe.K, pe.salient, dev)[2:] for pe in pes]
+        self.__dict__["_packed"] = (b, (pes[0], pes[1], maps))
+        return self.__dict__["_packed"][1]
+
+    # -------------------------------------------------------------- forward
+    def _quant(self, t2: torch.Tensor, pe: PackedExperts, maps) -> torch.Tensor:
+        if self.act_quant is not None:
+            ops.fake_quant_inplace(t2, self.act_quant, self.quant_bits, self.group_size, maps[0],
+                                   maps[1], pe.S)
+        return t2
+
+    @torch.no_grad()
+    def forward(self, hidden_states, top_k_index, top_k_weights):
+        ops._require_gpu(hidden_states, "W4A4Experts.forward")
+        gate_up, down, maps = self.packed()
+        x = hidden_states.reshape(-1, hidden_states.shape[-1])
+        if x.shape[1] != gate_up.K:
+            raise ValueError(f"W4A4Experts: hidden size {x.shape[1]}, packed for {gate_up.K}")
+        if x.dtype != gate_up.dtype:
+            raise RuntimeError(f"expected input dtype {gate_up.dtype}, got {x.dtype}")
+        if x.shape[0] == 0:
+            return torch.empty_like(hidden_states)
+        r = plan_routes(top_k_index, top_k_weights, gate_up.num_experts)
+        if r.tokens != x.shape[0]:
+            raise ValueError(f"W4A4Experts: {x.shape[0]} tokens, {r.tokens} routed")
+        if self.act_quant is not None:
+            x = x.clone(memory_format=torch.contiguous_format)  # (the caller's stays as it was)
+        h = expert_linear(self._quant(x, gate_up, maps[0]), gate_up, r, act=self.act)
+        z = expert_linear(self._quant(h, down, maps[1]), down, r, rows="slot")
+        return combine(z, r).view(hidden_states.shape)
+
+    # -------------------------------------------------------------- casts and persistence
+    def _apply(self, fn, recurse=True):
+        if self._meta is not None and self.gate_up_scale_t is not None:
+            dt = fn(torch.empty(0, dtype=self._meta["dtype"], device=self.gate_up_scale_t.device)).dtype
+            if dt != self._meta["dtype"]:
+                raise RuntimeError(f"W4A4Experts: packed in {self._meta['dtype']}; a cast to {dt} changes "
+                                   "the weights' values -- quantize the model in the target dtype")
+        return super()._apply(fn, recurse)
+
+    def get_extra_state(self):
+        m = self._meta
+        return {"format": self.EXTRA_FORMAT, "act": self.act, "act_quant": self.act_quant,
+                "quant_bits": self.quant_bits, "group_size": self.group_size,
+                "weight_quant": self.weight_quant,
+                "meta": None if m is None else {k: str(v).replace("torch.", "") if k == "dtype" else int(v)
+                                                for k, v in m.items()}}
+
+    def set_extra_state(self, state):
+        if not isinstance(state, dict) or state.get("format") != self.EXTRA_FORMAT:
+            raise RuntimeError(f"W4A4Experts: unsupported extra state {type(state)}")
+        for n in ("act", "act_quant", "quant_bits", "group_size", "weight_quant"):
+            setattr(self, n, state[n])
+        m = state["meta"]
+        if m is not None:
+            m = dict(m, dtype=getattr(torch, m["dtype"]))
+            for part in ("gate_up", "down"):
+                for n in ("gated", "identity"):
+                    m[f"{part}_{n}"] = bool(m[f"{part}_{n}"])
+        self._meta = m
+        self.__dict__.pop("_packed", None)
+
+    def _load_from_state_dict(self, sd, prefix, *args):
+        if prefix + "_extra_state" in sd:  # size the buffers (None in a fresh module)
+            for part in ("gate_up", "down"):
+                for n in _TENSORS:
+                    t = sd.get(f"{prefix}{part}_{n}")
+                    setattr(self, f"{part}_{n}", None if t is None else torch.empty_like(t))
+        super()._load_from_state_dict(sd, prefix, *args)
+
+    def __repr__(self):
+        m = self._meta or {}
+        return (f"W4A4Experts({m.get('gate_up_num_experts')} experts, {m.get('gate_up_K')} -> "
+                f"{m.get('gate_up_n_out')}, act={self.act}, weight_quant={self.weight_quant}, "
+                f"act_quant={self.act_quant}, salient={m.get('gate_up_S')})")
+
+
 __all__ = ["Routing", "route", "plan_routes", "PackedExperts", "pack_experts", "pack_expert_codes",
-           "expert_linear", "combine"]
+           "expert_linear", "combine", "W4A4Experts"]

@@ -796,12 +796,17 @@ def quantize_llama_like(model, weight_quant="per_channel", act_quant="per_token"
 
 def quantize_mixtral(model, weight_quant="per_channel", act_quant="per_token",
                      quantize_bmm_input=False, input_feat=None, salient_prop=0, quant_bits=4,
-                     group_size=128):
+                     group_size=128, quantize_experts=False):
     """fake_quant.py:564-668.  Experts are swapped where they are nn.Linear modules
-    (w1/w2/w3); transformers >= 5 fuses them into 3-D parameters, which stay unquantized."""
+    (w1/w2/w3); transformers >= 5 fuses them into 3-D parameters, which stay unquantized unless
+    quantize_experts swaps them for experts.W4A4Experts (its row-wise activation modes and 4 bits
+    only; salient columns of gate_up by the router's input statistic, the key `gate`)."""
     from transformers.models.mixtral import modeling_mixtral as mm
     kw = dict(weight_quant=weight_quant, act_quant=act_quant, salient_prop=salient_prop,
               quant_bits=quant_bits, group_size=group_size)
+    if quantize_experts:
+        from .experts import W4A4Experts
+        W4A4Experts(act_quant=act_quant, quant_bits=quant_bits)  # (refuses before anything is swapped)
     expert_cls = getattr(mm, "MixtralBLockSparseTop2MLP", None) or getattr(mm, "MixtralBlockSparseTop2MLP", None)
     for name, m in list(model.model.named_modules()):
         pre = "model." + name + "."
@@ -816,6 +821,10 @@ def quantize_mixtral(model, weight_quant="per_channel", act_quant="per_token",
             link_siblings(m.q_proj, m.k_proj, m.v_proj)
         elif isinstance(m, mm.MixtralSparseMoeBlock) and isinstance(getattr(m, "gate", None), nn.Linear):
             _swap(m, "gate", pre + "gate", input_feat, True, **kw)
+        if (quantize_experts and isinstance(m, mm.MixtralSparseMoeBlock)
+                and hasattr(getattr(m, "experts", None), "gate_up_proj")):
+            imp = _importance(input_feat, pre + "gate", True) if salient_prop else None
+            m.experts = W4A4Experts.from_float(m.experts, importance=imp, **kw)
     return model
 
 
@@ -840,8 +849,8 @@ def quantize_falcon(model, weight_quant="per_channel", act_quant="per_token",
 
 def quantize_model(model, weight_quant="per_channel", act_quant="per_token",
                    quantize_bmm_input=False, input_feat=None, salient_prop=None, quant_bits=4,
-                   group_size=128, min_prop=0, max_prop=0):
-    """fake_quant.py:734-799: dispatch on the HF model class."""
+                   group_size=128, min_prop=0, max_prop=0, quantize_experts=False):
+    """fake_quant.py:734-799: dispatch on the HF model class (quantize_experts: quantize_mixtral)."""
     if input_feat is None:
         input_feat = {}
     from transformers.models.falcon.modeling_falcon import FalconPreTrainedModel
@@ -857,7 +866,7 @@ def quantize_model(model, weight_quant="per_channel", act_quant="per_token",
     if isinstance(model, (LlamaPreTrainedModel, MistralPreTrainedModel)):
         return quantize_llama_like(model, **kw)
     if isinstance(model, MixtralPreTrainedModel):
-        return quantize_mixtral(model, **kw)
+        return quantize_mixtral(model, quantize_experts=quantize_experts, **kw)
     if isinstance(model, FalconPreTrainedModel):
         return quantize_falcon(model, **kw)
     raise ValueError(f"Unsupported model type: {type(model)}")
