@@ -53,13 +53,24 @@ __device__ inline void barrier() {
 }
 __device__ inline int brev3(int c) { return ((c & 1) << 2) | (c & 2) | ((c >> 2) & 1); }
 
-constexpr int TILE_ROWS = 256;   // slots per tile
 constexpr int TILE_N = 256;      // weight rows per tile
-constexpr int RING = 3;
+
+// A kernel of tiles of up to 16 IMAX slots: RING LDS stages of activations, DW stages of codes in
+// registers ahead, OCC waves per SIMD (two workgroups per CU at 4); SPLIT: waves 0-3 issue all
+// LDS-DMA and waves 4-7 run at a higher wave priority
+template <int IMAX_, int RING_, int DW_, int OCC_, bool SPLIT_>
+struct Shape {
+  static constexpr int IMAX = IMAX_, RING = RING_, DW = DW_, OCC = OCC_, ROWS = 16 * IMAX_;
+  static constexpr bool SPLIT = SPLIT_;
+};
+using Large = Shape<16, 4, 2, 1, true>;
+using Medium = Shape<8, 4, 2, 4, false>;
+using Small = Shape<4, 8, 4, 4, false>;
 
 // The tile of workgroup `bid`: expert e, slots [m0, m1), weight tile tn; false: no such tile.
 // Tiles are ordered by expert, groups of up to 4 row tiles, weight tile, row tile (the row tiles
 // of a group read the same weights), in contiguous runs per XCD.
+template <int TILE_ROWS>
 __device__ inline bool find_tile(const int32_t* offsets, int E, int tiles_n, int bid, int& e,
                                  int& m0, int& m1, int& tn) {
   const int lane = threadIdx.x & 63;
@@ -104,12 +115,13 @@ __device__ inline bool find_tile(const int32_t* offsets, int E, int tiles_n, int
 }
 
 // One tile of 16 I slots (I / 4 LDS-DMA pieces per wave and stage)
-template <class DT, int GB, bool GATED, int I>
+template <class DT, int GB, bool GATED, class SH, int I>
 __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int nm, int tn,
                                 unsigned char* lds) {
   typedef typename DT::T T;
-  constexpr int J = 2, NA = I / 4, PF = I == 16 ? 2 : 3;
-  constexpr int SLOT = I * 16 * 128;
+  constexpr int J = 2, NA = I / 4, PF = I == 16 || (I == 8 && SH::OCC == 4) ? 2 : 3;
+  constexpr int SLOT = I * 16 * 128, RING = SH::RING, DW = SH::DW;
+  constexpr int NO = SH::SPLIT ? 2 : 1;  // waves whose pieces a loading wave issues
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int r16 = lane & 15, q = lane >> 4;
@@ -120,19 +132,32 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
   const T* xb = (const T*)a.x;
   if (!a.rows) xb += (long)m0 * a.ldx;
   const rsrc_t rA = make_rsrc(xb, 0xFFFFFFFFu);
-  uint32_t a_off[NA];
+  uint32_t a_off[NO][NA];
 #pragma unroll
-  for (int i = 0; i < NA; ++i) {
-    const int row = 64 * i + 8 * wave + (lane >> 3);
-    const int rr = min(row, nm - 1);  // (rows past the segment repeat its last one)
-    const long xr = a.rows ? a.rows[m0 + rr] / a.top_k : rr;
-    a_off[i] = (uint32_t)(xr * a.ldx * (long)sizeof(T)) +
-               (uint32_t)(brev3((lane & 7) ^ ((row >> 1) & 7)) << 4);
-  }
+  for (int o = 0; o < NO; ++o)
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int row = 64 * i + 8 * ((wave + 4 * o) & 7) + (lane >> 3);
+      const int rr = min(row, nm - 1);  // (rows past the segment repeat its last one)
+      const long xr = a.rows ? a.rows[m0 + rr] / a.top_k : rr;
+      a_off[o][i] = (uint32_t)(xr * a.ldx * (long)sizeof(T)) +
+                    (uint32_t)(brev3((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    }
+  const bool loads = !SH::SPLIT || wave < 4;
   auto issue_a = [&](int kt) {
+    if (!loads) return;
     unsigned char* slot = lds + (kt % RING) * SLOT + wave * 1024;
 #pragma unroll
-    for (int i = 0; i < NA; ++i) dma16(rA, a_off[i], (uint32_t)kt * 128, slot + i * 8192);
+    for (int o = 0; o < NO; ++o)
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+        dma16(rA, a_off[o][i], (uint32_t)kt * 128, slot + o * 4096 + i * 8192);
+  };
+  // stage kt's activations of this wave are in LDS: at most the RING - 2 later stages' LDS-DMA
+  // (the youngest operations; codes loads among them only make it wait for more) are in flight
+  auto wait_a = [&](int kt) {
+    if (!loads) return;
+    if (nkt - 1 - kt >= RING - 2) vmwait<(RING - 2) * NO * NA>(); else vmwait<0>();
   };
 
   // weights
@@ -179,31 +204,32 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
 
   // The decode of stage kt comes before the next activation loads are issued: the compiler waits
   // for the codes by counting its own loads, and would otherwise wait for those as well.
-  Codes cs[2];
-  issue_a(0);
-  load_w(0, cs[0]);
-  if (nkt > 1) issue_a(1);
-  load_w(1, cs[1]);  // (nkm is even)
+  Codes cs[DW];
+#pragma unroll
+  for (int p = 0; p < (RING - 1 > DW ? RING - 1 : DW); ++p) {
+    if (p < RING - 1 && p < nkt) issue_a(p);
+    if (p < DW && p < nkm) load_w(p, cs[p]);
+  }
   auto step = [&](int kt, Codes& c) {
     uint32_t sp[J];
     sp[0] = Dec<DT>::prep(c.s & 0xFFFFu), sp[1] = Dec<DT>::prep(c.s >> 16);
     u32x4 bf[2][J];
 #pragma unroll
     for (int j = 0; j < J; ++j) bf[0][j] = Dec<DT>::run(c.w[2 * j], sp[j], dk);
-    // at most the NA youngest loads outstanding: stage kt's activations are older than those
-    if (kt + 1 < nkt) vmwait<NA>(); else vmwait<0>();
+    wait_a(kt);
     barrier();  // everyone's part of stage kt is in LDS, and nobody reads stage kt - 1 any more
-    if (kt + 2 < nkt) issue_a(kt + 2);
+    if (kt + RING - 1 < nkt) issue_a(kt + RING - 1);
     blocks(lds + (kt % RING) * SLOT, [&](int s, int j) -> const u32x4& { return bf[s][j]; },
            [&](int t) {
              if (t < J) bf[1][t] = Dec<DT>::run(c.w[2 * t + 1], sp[t], dk);
            });
-    if (kt + 2 < nkm) load_w(kt + 2, c);
+    if (kt + DW < nkm) load_w(kt + DW, c);
   };
-  for (int kt = 0; kt < nkm; kt += 2) {
-    step(kt, cs[0]);
-    step(kt + 1, cs[1]);
-  }
+  if (SH::SPLIT && wave >= 4) __builtin_amdgcn_s_setprio(1);
+  for (int kt = 0; kt < nkm; kt += DW)
+#pragma unroll
+    for (int u = 0; u < DW; ++u)
+      if (u < 2 || kt + u < nkm) step(kt + u, cs[u]);  // (nkm is even)
   // the exact salient columns: fragments as they are
   for (int kd = 0; kd < nks; ++kd) {
     const int kt = nkm + kd;
@@ -213,12 +239,13 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int j = 0; j < J; ++j) d[s][j] = *(const u32x4*)(sal + j * 16 + s * 8);
-    if (kt + 1 < nkt) vmwait<NA>(); else vmwait<0>();
+    wait_a(kt);
     barrier();
-    if (kt + 2 < nkt) issue_a(kt + 2);
+    if (kt + RING - 1 < nkt) issue_a(kt + RING - 1);
     blocks(lds + (kt % RING) * SLOT, [&](int s, int j) -> const u32x4& { return d[s][j]; },
            [](int) {});
   }
+  if (SH::SPLIT && wave >= 4) __builtin_amdgcn_s_setprio(0);
 
   // epilogue: the tile in LDS (16-B chunk c of row m at c ^ (m & 15)), then whole rows out
   constexpr int TNO = GATED ? TILE_N / 2 : TILE_N;
@@ -262,45 +289,59 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
   }
 }
 
-template <class DT, int GB, bool GATED>
-__global__ __launch_bounds__(512, 1) void expert_tiles_kernel(const GemvArgs a, int E, int tiles_n,
-                                                              int act) {
-  constexpr int EPI = TILE_ROWS * (GATED ? TILE_N / 2 : TILE_N) * 2;
-  constexpr int BYTES = RING * TILE_ROWS * 128 > EPI ? RING * TILE_ROWS * 128 : EPI;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[BYTES];
+template <class DT, int GB, bool GATED, class SH>
+__global__ __launch_bounds__(512, SH::OCC) void expert_tiles_kernel(const GemvArgs a, int E,
+                                                                    int tiles_n, int act) {
+  constexpr int RB = SH::RING * SH::ROWS * 128;
+  constexpr int EPI = SH::ROWS * (GATED ? TILE_N / 2 : TILE_N) * 2;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[RB > EPI ? RB : EPI];
   int e, m0, m1, tn;
-  if (!find_tile(a.offsets, E, tiles_n, blockIdx.x, e, m0, m1, tn)) return;
+  if (!find_tile<SH::ROWS>(a.offsets, E, tiles_n, blockIdx.x, e, m0, m1, tn)) return;
   const int nm = m1 - m0;
-  if (nm > 192) run_tile<DT, GB, GATED, 16>(a, act, e, m0, nm, tn, lds);
-  else if (nm > 128) run_tile<DT, GB, GATED, 12>(a, act, e, m0, nm, tn, lds);
-  else if (nm > 64) run_tile<DT, GB, GATED, 8>(a, act, e, m0, nm, tn, lds);
-  else run_tile<DT, GB, GATED, 4>(a, act, e, m0, nm, tn, lds);
+  if constexpr (SH::IMAX >= 16) {
+    if (nm > 192) return run_tile<DT, GB, GATED, SH, 16>(a, act, e, m0, nm, tn, lds);
+    if (nm > 128) return run_tile<DT, GB, GATED, SH, 12>(a, act, e, m0, nm, tn, lds);
+  }
+  if constexpr (SH::IMAX >= 8) {
+    if (nm > 64) return run_tile<DT, GB, GATED, SH, 8>(a, act, e, m0, nm, tn, lds);
+  }
+  run_tile<DT, GB, GATED, SH, 4>(a, act, e, m0, nm, tn, lds);
 }
 
-template <class DT, int GB>
+template <class DT, int GB, class SH>
 static int launch_tiles(const GemvArgs& a, int E, int slots, int act, hipStream_t s) {
   const int tiles_n = cdiv(a.N, TILE_N);
-  const long tiles_m = (long)slots / TILE_ROWS + (slots < E ? slots : E);
+  const long tiles_m = (long)slots / SH::ROWS + (slots < E ? slots : E);
   const long grid = tiles_m * tiles_n;
   if (grid > 0x7FFFFFFFL) return SQMP_EUNSUPPORTED;
   if (act != ACT_NONE)
-    expert_tiles_kernel<DT, GB, true><<<dim3((unsigned)grid), dim3(512), 0, s>>>(a, E, tiles_n, act);
+    expert_tiles_kernel<DT, GB, true, SH><<<dim3((unsigned)grid), dim3(512), 0, s>>>(a, E, tiles_n, act);
   else
-    expert_tiles_kernel<DT, GB, false><<<dim3((unsigned)grid), dim3(512), 0, s>>>(a, E, tiles_n, act);
+    expert_tiles_kernel<DT, GB, false, SH><<<dim3((unsigned)grid), dim3(512), 0, s>>>(a, E, tiles_n, act);
   SQMP_LAUNCH_CHECK();
   return SQMP_OK;
+}
+
+// The tile height: from the mean rows of an expert (a tile mostly filled by its expert's rows)
+template <class DT, int GB>
+static int by_shape(const GemvArgs& a, int E, int slots, int act, hipStream_t s) {
+  const char* k = knob("SQMP_EXPERT_ROWS");
+  const int rows = k ? atoi(k) : slots / E <= 64 ? 64 : slots / E <= 192 ? 128 : 256;
+  if (rows <= 64) return launch_tiles<DT, GB, Small>(a, E, slots, act, s);
+  if (rows <= 128) return launch_tiles<DT, GB, Medium>(a, E, slots, act, s);
+  return launch_tiles<DT, GB, Large>(a, E, slots, act, s);
 }
 
 bool expert_tiles_ok(const GemvArgs& a, int dtype, int E, long x_rows) {
   // fp16 / bf16, groups of 32 or of whole stages, a 32-bit offset to every activation
   return (dtype == SQMP_F16 || dtype == SQMP_BF16) && (a.Gw % 64 == 0 || a.Gw == 32) && E <= 256 &&
-         (a.rows ? x_rows : TILE_ROWS) * a.ldx * 2 < 0xFFFF0000L;
+         (a.rows ? x_rows : 256) * a.ldx * 2 < 0xFFFF0000L;
 }
 
 int launch_expert_tiles(const GemvArgs& a, int dtype, int E, int slots, int act, hipStream_t s) {
   if (dtype == SQMP_F16)
-    return a.Gw == 32 ? launch_tiles<F16, 2>(a, E, slots, act, s) : launch_tiles<F16, 1>(a, E, slots, act, s);
-  return a.Gw == 32 ? launch_tiles<BF16, 2>(a, E, slots, act, s) : launch_tiles<BF16, 1>(a, E, slots, act, s);
+    return a.Gw == 32 ? by_shape<F16, 2>(a, E, slots, act, s) : by_shape<F16, 1>(a, E, slots, act, s);
+  return a.Gw == 32 ? by_shape<BF16, 2>(a, E, slots, act, s) : by_shape<BF16, 1>(a, E, slots, act, s);
 }
 
 }  // namespace w4

@@ -193,6 +193,40 @@ def test_products_exact_sums(T, E, k, N, K, G, by_slot, dt):
     assert (z[n:] == 7.0).all()                       # rows behind the last pair: as they were
 
 
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("height", [64, 128, 256])
+def test_tile_heights_agree(height, dt, monkeypatch):
+    """Every tile height, on segments of 0, 1, and the sizes around a tile's, with salient columns and
+    an odd number of outputs: the same bits."""
+    from smoothquant import _lib
+    monkeypatch.setenv("SQMP_EXPERT_ROWS", str(height))
+    _lib.reload_knobs()
+    D, g = DT[dt], gen(height)
+    sizes = [0, 1, 63, 64, 65, 127, 0, 129, 192, 193, 255, 256, 257, 320, 513]
+    ids = torch.repeat_interleave(torch.arange(len(sizes), device="cuda"),
+                                  torch.tensor(sizes, device="cuda"))
+    ids = ids[torch.randperm(len(ids), generator=g, device="cuda")].view(-1, 1)
+    E, T, N, K, G = len(sizes), len(ids), 283, 640, 64
+    codes, scales = int_weight((E, N, K), G, D, g)
+    pe = experts.pack_expert_codes(codes, scales, G)
+    r = experts.plan_routes(ids, torch.ones(T, 1, device="cuda"), E)
+    x = int_rows(T, K, D, g)
+    want = plain_experts(x, values(codes, scales, G), r, False).float().to(D)
+    assert torch.equal(experts.expert_linear(x, pe, r), want)
+    # whole 8-column outputs and salient columns: small whole numbers quantize exactly
+    w = torch.randint(-7, 8, (E, 48, 256), generator=g, device="cuda").to(D)
+    w[:, :, :4] = 7
+    sal = torch.tensor([5, 9, 200], device="cuda")
+    w[:, :, sal] *= 3
+    ps = experts.pack_experts(w, "per_group_unsorted", 64, sal)
+    x = int_rows(T, 256, D, g)
+    w_hat = torch.stack([ops.dequant_weight(ops.pack_weight(w[e], "per_group_unsorted", 4, 64, sal))
+                         for e in range(E)]).double()
+    z = experts.expert_linear(x, ps, r).double()
+    y = plain_experts(x, w_hat, r, False)
+    assert (z - y).abs().max() <= HALF[D] * y.abs().max() * 1.01
+
+
 @pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("T,E,k,I,K,G", [(4, 8, 2, 40, 128, 64), (150, 4, 2, 257, 320, 64),
