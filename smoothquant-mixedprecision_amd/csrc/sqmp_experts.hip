@@ -322,11 +322,14 @@ static int launch_tiles(const GemvArgs& a, int E, int slots, int act, hipStream_
   return SQMP_OK;
 }
 
-// The tile height: from the mean rows of an expert (a tile mostly filled by its expert's rows)
+// The tile height, by the mean rows of an expert (64 / 128 / 256 rows, one box, 2 of 8 experts, 4096 ->
+// 2 x 11008 gated unless said): 32 rows each 151 / 163 / 189 us, 64: 193 / 203 / 239, 128: 301 / 275
+// / 367, 512: 793 / 701 / 705, 1024: 1567 / 1297 / 1349 (11008 -> 4096: 772 / 678 / 743), 2048 of
+// 4096 -> 4096: 615 / 470 / 449.  SQMP_EXPERT_ROWS overrides (A/B)
 template <class DT, int GB>
 static int by_shape(const GemvArgs& a, int E, int slots, int act, hipStream_t s) {
   const char* k = knob("SQMP_EXPERT_ROWS");
-  const int rows = k ? atoi(k) : slots / E <= 64 ? 64 : slots / E <= 192 ? 128 : 256;
+  const int rows = k && atoi(k) > 0 ? atoi(k) : slots / E <= 64 ? 64 : slots / E < 2048 ? 128 : 256;
   if (rows <= 64) return launch_tiles<DT, GB, Small>(a, E, slots, act, s);
   if (rows <= 128) return launch_tiles<DT, GB, Medium>(a, E, slots, act, s);
   return launch_tiles<DT, GB, Large>(a, E, slots, act, s);

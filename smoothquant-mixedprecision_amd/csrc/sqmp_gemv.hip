@@ -220,7 +220,10 @@ extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* row
   a.y = y, a.N = N, a.n_out = n_out, a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
   a.rows = rows, a.offsets = offsets, a.top_k = top_k;
   hipStream_t s = (hipStream_t)stream;
-  if (w4::expert_tiles_ok(a, dtype, E, x_rows) && slots >= 16 * E)
+  // tiles from 8 rows per expert on (few-row kernel / 64-row tiles: 64 experts of 6 rows 56 / 71 us,
+  // 8 of 16 rows 147 / 115 us); SQMP_EXPERT_ROWS = 0 / a tile height overrides (A/B)
+  const char* k = knob("SQMP_EXPERT_ROWS");
+  if (w4::expert_tiles_ok(a, dtype, E, x_rows) && (k ? atoi(k) > 0 : slots >= 8 * E))
     return w4::launch_expert_tiles(a, dtype, E, slots, act, s);
   const int est = cdiv(slots, E) * 2;  // rows of a busy expert (any count is right)
 #define SQMP_EX(DTT)                                                                  \

@@ -9,30 +9,176 @@
 //   sqmp_combine      y[t] = D( sum_j w[t][j] z[slots[t][j]] ), fp32 sums in the order of j
 //   sqmp_pack_rows    the activation operand of packed weights (columns gathered by a map)
 //
-// The order is a counting sort: a block of 256 tokens counts its pairs per expert, an exclusive
-// scan over the blocks places them, and inside a block the pairs are ranked 64 at a time by
-// ballots.  No atomics: slots depend on the ids alone.
+// What bounds it: launches and latency for a decoding batch (one launch up to 256 tokens), the
+// logits' bytes for prompts.  A token's logits are spread over 4 lanes, read once in 16-byte
+// pieces where they are aligned; each lane keeps its k largest in registers as keys that hold
+// the value's order and the index (so every compare-exchange is a max and a min, and ties go to
+// the lower index), and two merges over the lanes leave the k largest of all.  The order of the
+// pairs is a counting sort: a block of 256 tokens ranks its pairs 64 at a time by ballots, an
+// exclusive scan over the blocks places them.  No atomics: slots depend on the ids alone.
 #include "sqmp_common.h"
 
 namespace sqmp {
 namespace route {
 
-constexpr int TB = 256;          // tokens (and threads) per block
+constexpr int TB = 256;          // tokens per block
+constexpr int NT = 1024;         // threads per block: 4 lanes per token
+constexpr int NWAVE = NT / 64;
 constexpr int E_MAX = 256, K_MAX = 16;
-constexpr int NWAVE = TB / 64;
+constexpr int MAX_CHUNKS = TB * K_MAX / 64;       // 64-pair chunks of a block
+constexpr int PER_WAVE = MAX_CHUNKS / NWAVE;      // of a wave
 
-// descending order of floats as unsigned order: NaN highest, -0 equal to +0
-__device__ inline uint32_t order_key(float v) {
-  if (v != v) return 0xFFFFFFFFu;
-  uint32_t u = __float_as_uint(v);
-  if (u == 0x80000000u) u = 0u;
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+// Keys whose unsigned order is the order of (value, lower index first): NaN highest, -0 as +0.
+// 16-bit types: value and index in 32 bits; fp32: in 64.  (index 0xFFFF / ~0: none)
+template <class DT> struct Key;
+template <> struct Key<F32> {
+  typedef uint64_t K;
+  static constexpr K NEG_INF = (K)0x007FFFFFu << 32;  // of -inf, below every index
+  __device__ static inline K make(float v, int e) {
+    uint32_t u = __float_as_uint(v);
+    if (v != v) u = 0x7FFFFFFFu;
+    if (u == 0x80000000u) u = 0u;
+    u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return ((K)u << 32) | (uint32_t)~e;
+  }
+  __device__ static inline int index(K k) { return (int)~(uint32_t)k; }
+  __device__ static inline bool chosen(K k) { return (k >> 32) > 0x007FFFFFu; }
+  __device__ static inline float value(K k) {
+    const uint32_t u = (uint32_t)(k >> 32);
+    return __uint_as_float((u & 0x80000000u) ? (u & 0x7FFFFFFFu) : ~u);
+  }
+  __device__ static inline K shfl(K k, int x) {
+    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)k, x, 64);
+    const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(k >> 32), x, 64);
+    return ((K)hi << 32) | lo;
+  }
+};
+template <class DT, uint32_t INF> struct Key16 {
+  typedef uint32_t K;
+  static constexpr K NEG_INF = (K)(0x7FFFu - INF) << 16;  // ~(0x8000 | INF)
+  typedef typename DT::T T;
+  __device__ static inline K make(float v, int e) {
+    const T t = DT::from_f(v);  // (the value came from D: exact)
+    uint32_t u = (uint32_t)__builtin_bit_cast(uint16_t, t);
+    if (v != v) u = 0x7FFFu;
+    if (u == 0x8000u) u = 0u;
+    u = (u & 0x8000u) ? (~u & 0xFFFFu) : (u | 0x8000u);
+    return (u << 16) | (uint32_t)(0xFFFF - e);
+  }
+  __device__ static inline int index(K k) { return 0xFFFF - (int)(k & 0xFFFFu); }
+  __device__ static inline bool chosen(K k) { return (k >> 16) > (NEG_INF >> 16); }
+  __device__ static inline float value(K k) {
+    const uint32_t u = k >> 16;
+    const uint16_t b = (uint16_t)((u & 0x8000u) ? (u & 0x7FFFu) : ~u);
+    return DT::to_f(__builtin_bit_cast(T, b));
+  }
+  __device__ static inline K shfl(K k, int x) { return (K)__shfl_xor((int)k, x, 64); }
+};
+template <> struct Key<F16> : Key16<F16, 0x7C00u> {};
+template <> struct Key<BF16> : Key16<BF16, 0x7F80u> {};
+
+// list (descending) <- the KT largest of list and c
+template <class K, int KT>
+__device__ inline void insert(K (&list)[KT], K c) {
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    const K a = list[j];
+    list[j] = c > a ? c : a;
+    c = c > a ? a : c;
+  }
 }
-constexpr uint32_t KEY_NEG_INF = 0x007FFFFFu;  // order_key(-inf)
 
-__device__ inline float key_value(uint32_t k) {
-  if (k == 0xFFFFFFFFu) return __uint_as_float(0x7FC00000u);
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+// list <- the KT largest of the lanes lane and lane ^ x: the larger of a[j] and b[KT - 1 - j] are
+// those, in bitonic order; sorted by log2(KT) rounds of exchanges
+template <class DT, int KT>
+__device__ inline void merge(typename Key<DT>::K (&list)[KT], int x) {
+  typedef typename Key<DT>::K K;
+  K o[KT];
+#pragma unroll
+  for (int j = 0; j < KT; ++j) o[j] = Key<DT>::shfl(list[j], x);
+#pragma unroll
+  for (int j = 0; j < KT; ++j) list[j] = list[j] > o[KT - 1 - j] ? list[j] : o[KT - 1 - j];
+#pragma unroll
+  for (int d = KT / 2; d >= 1; d >>= 1)
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+      if ((j & d) == 0) {
+        const K a = list[j], b = list[j + d];
+        list[j] = a > b ? a : b;
+        list[j + d] = a > b ? b : a;
+      }
+}
+
+struct Args {
+  const void* logits;  // NULL: ids are given
+  long ldl;
+  int T, E, k, normalize;
+  float* weights;
+  int32_t* ids;
+  int32_t *offsets, *rows, *slots;
+  int32_t* hist;       // [E][blocks], then [E] totals
+  int blocks;
+};
+
+// lane c of a token's four visits its share of the logits: f(value, index)
+template <class DT, class F>
+__device__ inline void each_logit(const typename DT::T* row, int E, int c, bool vec, F f) {
+  typedef typename DT::T T;
+  constexpr int V = 16 / sizeof(T);
+  if (vec) {  // whole 16-byte pieces, piece p to lane p % 4
+    for (int p = c; p * V < E; p += 4) {
+      struct __attribute__((aligned(16))) P { T v[V]; };
+      const P x = *(const P*)(row + p * V);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f(DT::to_f(x.v[i]), p * V + i);
+    }
+  } else {
+    for (int e = c; e < E; e += 4) f(DT::to_f(row[e]), e);
+  }
+}
+
+// ids (and weights) of the block's tokens; lid: the ids again, in LDS
+template <class DT, int KT>
+__device__ inline void choose(const Args& a, int t0, int nt, uint16_t* lid) {
+  typedef typename DT::T T;
+  typedef Key<DT> KY;
+  typedef typename KY::K K;
+  const int tok = threadIdx.x >> 2, c = threadIdx.x & 3;
+  const int t = t0 + min(tok, nt - 1);  // (idle lanes repeat the last token)
+  const T* row = (const T*)a.logits + t * a.ldl;
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = a.E % V == 0 && a.ldl % V == 0 && (size_t)a.logits % 16 == 0;
+  K list[KT];
+#pragma unroll
+  for (int j = 0; j < KT; ++j) list[j] = 0;
+  each_logit<DT>(row, a.E, c, vec, [&](float v, int e) { insert<K, KT>(list, KY::make(v, e)); });
+  merge<DT, KT>(list, 1);
+  merge<DT, KT>(list, 2);
+  const float top = KY::value(list[0]);
+  float ex[KT], den = 0.f;
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    ex[j] = j < a.k && KY::chosen(list[j]) ? expf(KY::value(list[j]) - top) : 0.f;
+    den += ex[j];
+  }
+  if (!a.normalize) {
+    den = 0.f;
+    each_logit<DT>(row, a.E, c, vec, [&](float v, int) { den += expf(v - top); });
+    den += __shfl_xor(den, 1, 64);
+    den += __shfl_xor(den, 2, 64);
+  }
+  if (tok < nt) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+      if (j < a.k && (j & 3) == c) {
+        const bool sel = KY::chosen(list[j]);
+        const int id = sel ? KY::index(list[j]) : -1;
+        const long f = (long)t * a.k + j;
+        a.weights[f] = sel ? ex[j] / den : 0.f;
+        a.ids[f] = id;
+        lid[tok * a.k + j] = (uint16_t)(sel ? id : a.E);
+      }
+  }
 }
 
 // lanes of the wave whose expert equals this lane's (nbits bits of e are compared)
@@ -45,245 +191,153 @@ __device__ inline uint64_t same_expert(int e, int nbits) {
   return m;
 }
 
-// Ranks of a block's pairs.  cnt[chunk][e]: pairs of expert e in 64-pair chunk `chunk`.
-__device__ inline void count_chunks(const int32_t* ids, long f0, long f1, int E, int nbits,
-                                    uint16_t* cnt) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int chunks = (int)((f1 - f0 + 63) / 64);
-  for (int i = threadIdx.x; i < chunks * E; i += TB) cnt[i] = 0;
-  __syncthreads();
-  for (int c = wave; c < chunks; c += NWAVE) {
-    const long f = f0 + c * 64 + lane;
-    int e = f < f1 ? ids[f] : -1;
-    if (e < 0 || e >= E) e = E;  // nothing chosen
-    const uint64_t m = same_expert(e, nbits);
-    if (e < E && (m & ((1ull << lane) - 1)) == 0) cnt[c * E + e] = (uint16_t)__popcll(m);
-  }
-  __syncthreads();
-}
-
-// hist[blk][e] of one block's ids
-__device__ inline void block_hist(const uint16_t* cnt, int chunks, int E, int32_t* hist) {
-  for (int e = threadIdx.x; e < E; e += TB) {
-    int s = 0;
-    for (int c = 0; c < chunks; ++c) s += cnt[c * E + e];
-    hist[e] = s;
-  }
-}
-
-// start[e] = first slot of this block's pairs of expert e; writes the pairs' slots
-__device__ inline void scatter(const int32_t* ids, long f0, long f1, int E, int nbits,
-                               const uint16_t* cnt, int32_t* at /* LDS [E], consumed */,
-                               uint16_t* base /* LDS [chunks][E] */, int32_t* rows,
-                               int32_t* slots, int total) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int chunks = (int)((f1 - f0 + 63) / 64);
-  for (int e = threadIdx.x; e < E; e += TB) {
-    int s = 0;
-    for (int c = 0; c < chunks; ++c) {
-      base[c * E + e] = (uint16_t)s;
-      s += cnt[c * E + e];
-    }
-  }
-  __syncthreads();
-  for (int c = wave; c < chunks; c += NWAVE) {
-    const long f = f0 + c * 64 + lane;
-    int e = f < f1 ? ids[f] : -1;
-    if (e < 0 || e >= E) e = E;
-    const uint64_t m = same_expert(e, nbits);
-    if (f < f1) {
-      int slot = -1;
-      if (e < E) {
-        slot = at[e] + base[c * E + e] + (int)__popcll(m & ((1ull << lane) - 1));
-        rows[slot] = (int32_t)f;
-      }
-      slots[f] = slot;
-      if (f >= total) rows[f] = -1;  // behind the last pair
-    }
-  }
-}
-
-// at[e] (LDS) = exclusive prefix of tot[e] (+ base[e]); returns the total.  E <= 256 = TB
-__device__ inline int scan_experts(const int32_t* tot, const int32_t* base, int E, int32_t* at,
-                                   int32_t* tmp, int32_t* offsets) {
+// exclusive prefix over the E experts of v (thread e); *total: their sum.  tmp: LDS [E_MAX]
+__device__ inline int scan_experts(int v, int32_t* tmp, int* total) {
   const int e = threadIdx.x;
-  int v = e < E ? tot[e] : 0;
-  tmp[e] = v;
+  if (e < E_MAX) tmp[e] = v;
   __syncthreads();
-  for (int d = 1; d < TB; d <<= 1) {
-    const int add = e >= d ? tmp[e - d] : 0;
+  for (int d = 1; d < E_MAX; d <<= 1) {
+    const int add = e >= d && e < E_MAX ? tmp[e - d] : 0;
     __syncthreads();
-    tmp[e] += add;
+    if (e < E_MAX) tmp[e] += add;
     __syncthreads();
   }
-  const int total = tmp[TB - 1];
-  if (e < E) {
-    at[e] = tmp[e] - v + (base ? base[e] : 0);
-    if (offsets) offsets[e] = tmp[e] - v;
-  }
-  if (offsets && e == 0) offsets[E] = total;
-  __syncthreads();
-  return total;
+  *total = tmp[E_MAX - 1];
+  return e < E_MAX ? tmp[e] - v : 0;
 }
 
-// The k largest of a token's E logits, one thread per token; rows staged in LDS (coalesced).
-template <class DT, int KT>
-__device__ inline void top_k_rows(const typename DT::T* logits, long ldl, int t0, int nt, int E,
-                                  int k, int normalize, float* tile, float* weights,
-                                  int32_t* ids) {
-  const int pitch = E | 1;  // odd: a thread per row is conflict free
-  constexpr int ROWS = 64;  // tokens staged at once
-  for (int r0 = 0; r0 < nt; r0 += ROWS) {
-    const int nr = min(ROWS, nt - r0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < nr * E; i += TB) {
-      const int r = i / E, e = i - r * E;
-      tile[r * pitch + e] = DT::to_f(logits[(t0 + r0 + r) * ldl + e]);
-    }
-    __syncthreads();
-    if ((int)threadIdx.x < nr) {
-      const float* row = tile + threadIdx.x * pitch;
-      uint32_t key[KT];
-      int idx[KT];
-#pragma unroll
-      for (int j = 0; j < KT; ++j) key[j] = KEY_NEG_INF, idx[j] = -1;
-      for (int e = 0; e < E; ++e) {
-        const uint32_t ke = order_key(row[e]);
-        if (ke > key[KT - 1]) {  // strictly: equal logits keep the lower index
-          uint32_t ck = ke;
-          int ci = e;
-          bool up = false;  // inserted: the rest moves down one place, equal logits included
-#pragma unroll
-          for (int j = 0; j < KT; ++j) {
-            up = up || ck > key[j];
-            const uint32_t ok = key[j];
-            const int oi = idx[j];
-            key[j] = up ? ck : ok, idx[j] = up ? ci : oi;
-            ck = up ? ok : ck, ci = up ? oi : ci;
-          }
-        }
-      }
-      const float top = key_value(key[0]);
-      float ex[KT], den = 0.f;
-#pragma unroll
-      for (int j = 0; j < KT; ++j) {
-        ex[j] = idx[j] >= 0 && j < k ? expf(key_value(key[j]) - top) : 0.f;
-        den += ex[j];
-      }
-      if (!normalize && idx[0] >= 0) {
-        den = 0.f;
-        for (int e = 0; e < E; ++e) den += expf(row[e] - top);
-      }
-      const long f = (long)(t0 + r0 + threadIdx.x) * k;
-#pragma unroll
-      for (int j = 0; j < KT; ++j)
-        if (j < k) {
-          weights[f + j] = idx[j] >= 0 ? ex[j] / den : 0.f;
-          ids[f + j] = idx[j];
-        }
-    }
-  }
-  __syncthreads();
-}
-
-struct Args {
-  const void* logits;  // NULL: ids are given
-  long ldl;
-  int T, E, k, normalize;
-  float* weights;
-  int32_t* ids;
-  int32_t *offsets, *rows, *slots;
-  int32_t* hist;       // [blocks][E]
-};
-
-__host__ __device__ inline int bits_of(int E) {  // values 0 .. E
-  int b = 0;
-  while ((1 << b) <= E) ++b;
-  return b;
-}
-
-constexpr int TILE_F = 64 * (E_MAX | 1);           // floats of the logits tile
-constexpr int MAX_CHUNKS = TB * K_MAX / 64;        // 64
-// LDS: the tile, then (reused) two [chunks][E] tables of 16 bits
-constexpr int LDS_WORDS = TILE_F > MAX_CHUNKS * E_MAX ? TILE_F : MAX_CHUNKS * E_MAX;
-
-// one block of tokens: choose (or read) the ids and count them; ONE: the only block finishes
+// one block of tokens: its ids, and the rank of each of its pairs among the block's pairs of the
+// same expert.  ONE (the only block): the slots themselves; else the ranks, left in slots
 template <class DT, int KT, bool ONE>
-__global__ __launch_bounds__(TB) void route_kernel(const Args a) {
-  __shared__ float lds[LDS_WORDS];
-  __shared__ int32_t at[E_MAX], tmp[TB], tot[E_MAX];
+__global__ __launch_bounds__(NT) void route_kernel(const Args a) {
+  __shared__ uint16_t cnt[MAX_CHUNKS * E_MAX];
+  __shared__ uint16_t lid[TB * K_MAX];
+  __shared__ int32_t tmp[E_MAX], start[E_MAX];
   const int t0 = blockIdx.x * TB, nt = min(TB, a.T - t0);
-  if (a.logits)
-    top_k_rows<DT, KT>((const typename DT::T*)a.logits, a.ldl, t0, nt, a.E, a.k, a.normalize, lds,
-                       a.weights, a.ids);
-  __threadfence_block();
-  __syncthreads();
-  const long f0 = (long)t0 * a.k, f1 = f0 + (long)nt * a.k;
-  const int nbits = bits_of(a.E);
-  uint16_t* cnt = (uint16_t*)lds;
-  const int chunks = (int)((f1 - f0 + 63) / 64);
-  count_chunks(a.ids, f0, f1, a.E, nbits, cnt);
-  if constexpr (!ONE) {
-    block_hist(cnt, chunks, a.E, a.hist + (long)blockIdx.x * a.E);
+  const int np = nt * a.k, chunks = (np + 63) / 64;
+  const long f0 = (long)t0 * a.k;
+  if (a.logits) {
+    choose<DT, KT>(a, t0, nt, lid);
   } else {
-    block_hist(cnt, chunks, a.E, tot);
-    __syncthreads();
-    const int total = scan_experts(tot, nullptr, a.E, at, tmp, a.offsets);
-    scatter(a.ids, f0, f1, a.E, nbits, cnt, at, cnt + MAX_CHUNKS * E_MAX, a.rows, a.slots, total);
+    for (int i = threadIdx.x; i < np; i += NT) {
+      const int e = a.ids[f0 + i];
+      lid[i] = (uint16_t)(e < 0 || e >= a.E ? a.E : e);
+    }
   }
-}
-
-// hist[blk][e] -> exclusive scan over the blocks, hist[blocks][e] = the expert's total
-__global__ __launch_bounds__(TB) void scan_kernel(int32_t* hist, int blocks, int E) {
-  __shared__ int32_t part[TB];
-  const int e = blockIdx.x;
-  const int per = (blocks + TB - 1) / TB;
-  const int b0 = min((int)threadIdx.x * per, blocks), b1 = min(b0 + per, blocks);
-  int s = 0;
-  for (int b = b0; b < b1; ++b) s += hist[(long)b * E + e];
-  part[threadIdx.x] = s;
+  for (int i = threadIdx.x; i < chunks * a.E; i += NT) cnt[i] = 0;
   __syncthreads();
-  for (int d = 1; d < TB; d <<= 1) {
-    const int add = (int)threadIdx.x >= d ? part[threadIdx.x - d] : 0;
-    __syncthreads();
-    part[threadIdx.x] += add;
-    __syncthreads();
+  // pairs of each expert in every chunk, and a pair's rank inside its chunk
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int nbits = 32 - __clz(a.E);  // values 0 .. E
+  int my_e[PER_WAVE], my_r[PER_WAVE];
+#pragma unroll
+  for (int i = 0; i < PER_WAVE; ++i) {
+    const int c = wave + i * NWAVE, f = c * 64 + lane;
+    my_e[i] = a.E, my_r[i] = 0;
+    if (c < chunks) {
+      my_e[i] = f < np ? lid[f] : a.E;
+      const uint64_t m = same_expert(my_e[i], nbits);
+      my_r[i] = (int)__popcll(m & ((1ull << lane) - 1));
+      if (my_e[i] < a.E && my_r[i] == 0) cnt[c * a.E + my_e[i]] = (uint16_t)__popcll(m);
+    }
   }
-  int run = part[threadIdx.x] - s;
-  for (int b = b0; b < b1; ++b) {
-    const int v = hist[(long)b * E + e];
-    hist[(long)b * E + e] = run;
-    run += v;
+  __syncthreads();
+  // cnt -> pairs of the expert in earlier chunks; the block's count
+  int s = 0;
+  if ((int)threadIdx.x < a.E) {
+    for (int c = 0; c < chunks; ++c) {
+      const int v = cnt[c * a.E + threadIdx.x];
+      cnt[c * a.E + threadIdx.x] = (uint16_t)s;
+      s += v;
+    }
   }
-  if (threadIdx.x == TB - 1) hist[(long)blocks * E + e] = part[TB - 1];
+  int total = 0;
+  if constexpr (ONE) {
+    const int at = scan_experts(s, tmp, &total);
+    if ((int)threadIdx.x < a.E) start[threadIdx.x] = at, a.offsets[threadIdx.x] = at;
+    if (threadIdx.x == 0) a.offsets[a.E] = total;
+  } else {
+    if ((int)threadIdx.x < a.E) a.hist[(long)threadIdx.x * a.blocks + blockIdx.x] = s;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER_WAVE; ++i) {
+    const int c = wave + i * NWAVE, f = c * 64 + lane, e = my_e[i];
+    if (c < chunks && f < np) {
+      int slot = e < a.E ? cnt[c * a.E + e] + my_r[i] : -1;
+      if constexpr (ONE) {
+        if (e < a.E) {
+          slot += start[e];
+          a.rows[slot] = f;
+        }
+        if (f >= total) a.rows[f] = -1;  // behind the last pair
+      }
+      a.slots[f0 + f] = slot;
+    }
+  }
 }
 
-__global__ __launch_bounds__(TB) void scatter_kernel(const Args a, int blocks) {
-  __shared__ float lds[LDS_WORDS];
-  __shared__ int32_t at[E_MAX], tmp[TB];
-  const int t0 = blockIdx.x * TB, nt = min(TB, a.T - t0);
-  const long f0 = (long)t0 * a.k, f1 = f0 + (long)nt * a.k;
-  const int nbits = bits_of(a.E);
-  uint16_t* cnt = (uint16_t*)lds;
-  const int total = scan_experts(a.hist + (long)blocks * a.E, a.hist + (long)blockIdx.x * a.E, a.E,
-                                 at, tmp, blockIdx.x == 0 ? a.offsets : nullptr);
-  count_chunks(a.ids, f0, f1, a.E, nbits, cnt);
-  scatter(a.ids, f0, f1, a.E, nbits, cnt, at, cnt + MAX_CHUNKS * E_MAX, a.rows, a.slots, total);
+// hist[e][blk] -> exclusive scan over the blocks, the expert's total behind
+__global__ __launch_bounds__(256) void scan_kernel(int32_t* hist, int blocks, int E) {
+  __shared__ int32_t part[256];
+  const int e = blockIdx.x, tid = threadIdx.x;
+  int32_t* h = hist + (long)e * blocks;
+  int run = 0;
+  for (int b0 = 0; b0 < blocks; b0 += 256) {
+    const int v = b0 + tid < blocks ? h[b0 + tid] : 0;
+    part[tid] = v;
+    __syncthreads();
+    for (int d = 1; d < 256; d <<= 1) {
+      const int add = tid >= d ? part[tid - d] : 0;
+      __syncthreads();
+      part[tid] += add;
+      __syncthreads();
+    }
+    if (b0 + tid < blocks) h[b0 + tid] = run + part[tid] - v;
+    run += part[255];
+    __syncthreads();
+  }
+  if (tid == 0) hist[(long)E * blocks + e] = run;
+}
+
+// ranks in slots -> slots, and rows
+__global__ __launch_bounds__(NT) void place_kernel(const Args a) {
+  __shared__ int32_t tmp[E_MAX], start[E_MAX];
+  const int e = threadIdx.x;
+  int total = 0;
+  const int at = scan_experts(e < a.E ? a.hist[(long)a.E * a.blocks + e] : 0, tmp, &total);
+  if (e < a.E) {
+    start[e] = at + a.hist[(long)e * a.blocks + blockIdx.x];
+    if (blockIdx.x == 0) a.offsets[e] = at;
+  }
+  if (blockIdx.x == 0 && e == 0) a.offsets[a.E] = total;
+  __syncthreads();
+  const int t0 = blockIdx.x * TB, np = min(TB, a.T - t0) * a.k;
+  const long f0 = (long)t0 * a.k;
+  for (int i = threadIdx.x; i < np; i += NT) {
+    const long f = f0 + i;
+    const int r = a.slots[f];
+    if (r >= 0) {
+      const int slot = start[a.ids[f]] + r;
+      a.slots[f] = slot;
+      a.rows[slot] = (int32_t)f;
+    }
+    if (f >= total) a.rows[f] = -1;  // behind the last pair
+  }
 }
 
 template <class DT, int KT>
 static int launch(const Args& a, hipStream_t s) {
-  const int blocks = cdiv(a.T, TB);
-  if (blocks == 1) {
-    route_kernel<DT, KT, true><<<dim3(1), dim3(TB), 0, s>>>(a);
+  if (a.blocks == 1) {
+    route_kernel<DT, KT, true><<<dim3(1), dim3(NT), 0, s>>>(a);
     SQMP_LAUNCH_CHECK();
     return SQMP_OK;
   }
-  route_kernel<DT, KT, false><<<dim3(blocks), dim3(TB), 0, s>>>(a);
+  route_kernel<DT, KT, false><<<dim3(a.blocks), dim3(NT), 0, s>>>(a);
   SQMP_LAUNCH_CHECK();
-  scan_kernel<<<dim3(a.E), dim3(TB), 0, s>>>(a.hist, blocks, a.E);
+  scan_kernel<<<dim3(a.E), dim3(256), 0, s>>>(a.hist, a.blocks, a.E);
   SQMP_LAUNCH_CHECK();
-  scatter_kernel<<<dim3(blocks), dim3(TB), 0, s>>>(a, blocks);
+  place_kernel<<<dim3(a.blocks), dim3(NT), 0, s>>>(a);
   SQMP_LAUNCH_CHECK();
   return SQMP_OK;
 }
@@ -411,7 +465,7 @@ extern "C" int sqmp_route(const void* logits, long ldl, int dtype, int T, int E,
     return SQMP_OK;
   }
   const route::Args a{logits, ldl, T, E, top_k, normalize, weights, ids, offsets, rows, slots,
-                      (int32_t*)workspace};
+                      (int32_t*)workspace, cdiv(T, route::TB)};
   switch (dtype) {
     case SQMP_F32: return route::by_k<F32>(a, s);
     case SQMP_F16: return route::by_k<F16>(a, s);
@@ -433,7 +487,7 @@ extern "C" int sqmp_plan_routes(const int32_t* ids, int T, int E, int top_k, int
     return SQMP_OK;
   }
   const route::Args a{nullptr, 0, T, E, top_k, 0, nullptr, const_cast<int32_t*>(ids), offsets,
-                      rows, slots, (int32_t*)workspace};
+                      rows, slots, (int32_t*)workspace, cdiv(T, route::TB)};
   return route::launch<F32, 2>(a, s);
 }
 
