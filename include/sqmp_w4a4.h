@@ -420,9 +420,12 @@ int sqmp_gemm_h2d(const void* a2, int ldr, const int* aexp, const void* wt, cons
  * sqmp_quant_act_v2, or sqmp_pack_rows), row stride ldx elements, 16-B aligned rows; no row
  * beyond M is read.  codes_t / scale_t / sal_t: sqmp_pack_fq7 with J = 2.  Gw % 8 == 0. */
 #define SQMP_GEMV_MAX_ROWS 64
+/* workspace: in it the fp32 sums of tiles whose K is split meet (no need to clear it; NULL or a
+ * smaller one than asked for: no tile is split, the same values in another order of summation) */
+size_t sqmp_gemv_workspace_bytes(int dtype, int M, int N, int Kp);
 int sqmp_gemv_w4(const void* x, long ldx, const void* codes_t, const void* scale_t,
                  const void* sal_t, const void* bias, void* y, int dtype, int M, int N, int Kp,
-                 int S_pad, int Gw, int ngw, void* stream);
+                 int S_pad, int Gw, int ngw, void* workspace, size_t ws_bytes, void* stream);
 
 /* Routing (the MixtralSparseMoeBlock that fake_quant.py:564-668 quantizes).  logits D [T][E], row
  * stride ldl: per token the top_k largest (ties: the lowest index; NaN counts as the largest; -inf
@@ -446,10 +449,12 @@ int sqmp_plan_routes(const int32_t* ids, int T, int E, int top_k, int32_t* offse
  * and 16 up rows in turn, z = D( act(gate) * up ), n_out of the N / 2 columns are written.
  * slots = rows of z (an upper bound of offsets[E]); rows of z behind offsets[E] are left as they
  * were.  x_rows: rows of x. */
+size_t sqmp_expert_workspace_bytes(int dtype, int E, int slots, int N, int Kp);
 int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* rows, int top_k,
                           const int32_t* offsets, int E, const void* codes_t, const void* scale_t,
                           const void* sal_t, void* y, int dtype, int slots, int x_rows, int N,
-                          int n_out, int Kp, int S_pad, int Gw, int ngw, int act, void* stream);
+                          int n_out, int Kp, int S_pad, int Gw, int ngw, int act, void* workspace,
+                          size_t ws_bytes, void* stream);
 
 /* y[t] = D( sum_j weights[t][j] * z[slots[t][j]] ), fp32 sums in the order of j; slots < 0 are
  * skipped.  z D [slots][H], y D [T][H]. */

@@ -62,23 +62,36 @@ template <int IMAX_, int RING_, int DW_, int OCC_, bool SPLIT_>
 struct Shape {
   static constexpr int IMAX = IMAX_, RING = RING_, DW = DW_, OCC = OCC_, ROWS = 16 * IMAX_;
   static constexpr bool SPLIT = SPLIT_;
+  static constexpr int CAP = OCC_ == 4 ? 512 : 256;  // workgroups the 256 CUs hold at once
 };
 using Large = Shape<16, 4, 2, 1, true>;
 using Medium = Shape<8, 4, 2, 4, false>;
 using Small = Shape<4, 8, 4, 4, false>;
 
-// The tile of workgroup `bid`: expert e, slots [m0, m1), weight tile tn; false: no such tile.
-// Tiles are ordered by expert, groups of up to 4 row tiles, weight tile, row tile (the row tiles
-// of a group read the same weights), in contiguous runs per XCD.
+// What a workgroup computes: expert e, slots [m0, m1), weight tile tn, part `part` of `parts` of the
+// K stages (`split`: its place among the split tiles)
+struct Tile {
+  int e, m0, m1, tn, part, parts, split;
+};
+
+// The tiles of all experts are numbered by expert, groups of up to 4 row tiles, weight tile, row
+// tile (the row tiles of a group read the same weights).  Whole rounds of `cap` workgroups (those
+// the GPU holds at once) take a tile each, in contiguous runs per XCD; the tiles of the last,
+// partial round are split along K into as many parts as fit the round, at most smax, whose fp32
+// sums meet in the workspace (join_kernel).  join: workgroup bid is the bid-th split tile, whole.
+// dense_rows: the segment of a single weight, without offsets.  false: nothing to do
 template <int TILE_ROWS>
-__device__ inline bool find_tile(const int32_t* offsets, int E, int tiles_n, int bid, int& e,
-                                 int& m0, int& m1, int& tn) {
+__device__ inline bool find_tile(const int32_t* offsets, int dense_rows, int E, int tiles_n, int cap,
+                                 int smax, int bid, bool join, Tile& t) {
   const int lane = threadIdx.x & 63;
   const int per = (E + 63) >> 6;  // experts per lane (E <= 256: at most 4)
   const int e0 = lane * per;
   int off[5], cnt = 0;
 #pragma unroll
-  for (int i = 0; i < 5; ++i) off[i] = offsets[min(e0 + min(i, per), E)];
+  for (int i = 0; i < 5; ++i) {
+    const int x = min(e0 + min(i, per), E);
+    off[i] = offsets ? offsets[x] : x > 0 ? dense_rows : 0;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (i < per) cnt += (off[i + 1] - off[i] + TILE_ROWS - 1) / TILE_ROWS;
@@ -89,9 +102,23 @@ __device__ inline bool find_tile(const int32_t* offsets, int E, int tiles_n, int
     if (lane >= d) incl += v;
   }
   const int nwg = __builtin_amdgcn_readfirstlane(__shfl(incl, 63, 64)) * tiles_n;
-  if (bid >= nwg) return false;
-  const int xcd = bid & 7, q = nwg >> 3, r = nwg & 7;
-  const int wg = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
+  const int whole = smax > 1 ? nwg / cap * cap : nwg, left = nwg - whole;
+  const int parts = left > 0 ? max(1, min(smax, cap / left)) : 1;
+  int wg;
+  t.part = 0, t.parts = 1, t.split = 0;
+  if (join) {
+    if (bid >= left || parts == 1) return false;
+    wg = whole + bid;
+    t.parts = parts, t.split = bid;
+  } else if (bid < whole) {
+    const int xcd = bid & 7, q = whole >> 3, r = whole & 7;
+    wg = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
+  } else {
+    const int b = bid - whole;
+    if (b >= left * parts) return false;
+    t.split = b / parts, t.part = b - t.split * parts, t.parts = parts;
+    wg = whole + t.split;
+  }
   // the lane, then the expert within it, whose tiles hold wg
   const uint64_t mask = __ballot(incl * tiles_n > wg);
   const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)mask) - 1);
@@ -100,24 +127,26 @@ __device__ inline bool find_tile(const int32_t* offsets, int E, int tiles_n, int
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int a = __shfl(off[i], src, 64), b = __shfl(off[i + 1], src, 64);
-    const int t = i < per ? (b - a + TILE_ROWS - 1) / TILE_ROWS * tiles_n : 0;
-    if (!done && rem < t) found = src * per + i, lo = a, hi = b, done = 1;
-    if (!done) rem -= t;
+    const int n = i < per ? (b - a + TILE_ROWS - 1) / TILE_ROWS * tiles_n : 0;
+    if (!done && rem < n) found = src * per + i, lo = a, hi = b, done = 1;
+    if (!done) rem -= n;
   }
   const int tiles_m = (hi - lo + TILE_ROWS - 1) / TILE_ROWS;
   const int gid = rem / (4 * tiles_n), first = gid * 4, gsz = min(tiles_m - first, 4);
   const int in_g = rem - gid * 4 * tiles_n;
-  e = __builtin_amdgcn_readfirstlane(found);
-  m0 = __builtin_amdgcn_readfirstlane(lo + (first + in_g % gsz) * TILE_ROWS);
-  m1 = __builtin_amdgcn_readfirstlane(min(hi, lo + (first + in_g % gsz + 1) * TILE_ROWS));
-  tn = __builtin_amdgcn_readfirstlane(in_g / gsz);
+  t.e = __builtin_amdgcn_readfirstlane(found);
+  t.m0 = __builtin_amdgcn_readfirstlane(lo + (first + in_g % gsz) * TILE_ROWS);
+  t.m1 = __builtin_amdgcn_readfirstlane(min(hi, lo + (first + in_g % gsz + 1) * TILE_ROWS));
+  t.tn = __builtin_amdgcn_readfirstlane(in_g / gsz);
+  t.part = __builtin_amdgcn_readfirstlane(t.part), t.parts = __builtin_amdgcn_readfirstlane(t.parts);
+  t.split = __builtin_amdgcn_readfirstlane(t.split);
   return true;
 }
 
-// One tile of 16 I slots (I / 4 LDS-DMA pieces per wave and stage)
+// One tile (or one K part of it) of 16 I slots (I / 4 LDS-DMA pieces per wave and stage)
 template <class DT, int GB, bool GATED, class SH, int I>
-__device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int nm, int tn,
-                                unsigned char* lds) {
+__device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsigned char* lds,
+                                float* part_sums) {
   typedef typename DT::T T;
   constexpr int J = 2, NA = I / 4, PF = I == 16 || (I == 8 && SH::OCC == 4) ? 2 : 3;
   constexpr int SLOT = I * 16 * 128, RING = SH::RING, DW = SH::DW;
@@ -125,7 +154,13 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int r16 = lane & 15, q = lane >> 4;
-  const int nkm = a.Kp / 64, nks = a.S_pad / 64, nkt = nkm + nks;
+  const int e = t.e, m0 = t.m0, nm = t.m1 - t.m0, tn = t.tn;
+  const int nks_all = a.S_pad / 64, nkm_all = a.Kp / 64;
+  // this part's stages: codes [k0, nkm), then (last part) the salient ones up to nkt
+  const int k0 = (int)((long)nkm_all * t.part / t.parts) & ~3;
+  const bool last = t.part + 1 == t.parts;
+  const int nkm = last ? nkm_all : (int)((long)nkm_all * (t.part + 1) / t.parts) & ~3;
+  const int nks = last ? nks_all : 0, nkt = nkm + nks;
 
   // activation rows: piece i of a wave = rows 64 i + 8 wave + (lane >> 3); the lane brings the
   // chunk that belongs at physical place lane & 7 of its row (chunk c at brev3(c) ^ (row / 2))
@@ -162,7 +197,7 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
 
   // weights
   const long wb = (long)e * ((a.N + 255) / 256 * 8) + tn * 8 + wave;
-  const uint32_t* codes = a.codes + wb * nkm * 256 + lane * 4;
+  const uint32_t* codes = a.codes + wb * nkm_all * 256 + lane * 4;
   const T* scale = (const T*)a.scale + wb * a.ngw * 32 + r16 * 2;
   struct Codes {
     u32x4 w;
@@ -207,8 +242,8 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
   Codes cs[DW];
 #pragma unroll
   for (int p = 0; p < (RING - 1 > DW ? RING - 1 : DW); ++p) {
-    if (p < RING - 1 && p < nkt) issue_a(p);
-    if (p < DW && p < nkm) load_w(p, cs[p]);
+    if (p < RING - 1 && k0 + p < nkt) issue_a(k0 + p);
+    if (p < DW && k0 + p < nkm) load_w(k0 + p, cs[p]);
   }
   auto step = [&](int kt, Codes& c) {
     uint32_t sp[J];
@@ -226,14 +261,14 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
     if (kt + DW < nkm) load_w(kt + DW, c);
   };
   if (SH::SPLIT && wave >= 4) __builtin_amdgcn_s_setprio(1);
-  for (int kt = 0; kt < nkm; kt += DW)
+  for (int kt = k0; kt < nkm; kt += DW)
 #pragma unroll
     for (int u = 0; u < DW; ++u)
       if (u < 2 || kt + u < nkm) step(kt + u, cs[u]);  // (nkm is even)
   // the exact salient columns: fragments as they are
   for (int kd = 0; kd < nks; ++kd) {
     const int kt = nkm + kd;
-    const T* sal = (const T*)a.sal + (wb * nks + kd) * 2048 + lane * 32;
+    const T* sal = (const T*)a.sal + (wb * nks_all + kd) * 2048 + lane * 32;
     u32x4 d[2][J];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -247,20 +282,31 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
   }
   if (SH::SPLIT && wave >= 4) __builtin_amdgcn_s_setprio(0);
 
+  const int tid = threadIdx.x, er = r16, eq = q;
+  if (t.parts > 1) {  // fp32 sums in fragment order (16 bytes a lane, whole lines)
+    f32x4* ps = (f32x4*)part_sums + (long)(t.split * t.parts + t.part) * (SH::IMAX * J * 512) + tid;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < J; ++j) ps[(i * J + j) * 512] = acc[i][j];
+    return;
+  }
   // epilogue: the tile in LDS (16-B chunk c of row m at c ^ (m & 15)), then whole rows out
   constexpr int TNO = GATED ? TILE_N / 2 : TILE_N;
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   barrier();
 #pragma unroll
   for (int i = 0; i < I; ++i) {
-    const int m = 16 * i + r16;
+    const int m = 16 * i + er;
 #pragma unroll
     for (int j = 0; j < (GATED ? 1 : J); ++j) {
-      const int nl = GATED ? 16 * wave + 4 * q : 32 * wave + 16 * j + 4 * q;
+      const int nl = GATED ? 16 * wave + 4 * eq : 32 * wave + 16 * j + 4 * eq;
       T v[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float f = acc[i][j][r];
+        if constexpr (!GATED)
+          if (a.bias && tn * TILE_N + nl + r < a.N) f += DT::to_f(((const T*)a.bias)[tn * TILE_N + nl + r]);
         if constexpr (GATED)
           f = (act == ACT_SILU ? act_fn<ACT_SILU>(f) : act_fn<ACT_GELU>(f)) * acc[i][1][r];
         v[r] = DT::from_f(f);
@@ -274,7 +320,7 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
   const int n0 = tn * TNO;
   T* y = (T*)a.y + (long)m0 * a.n_out + n0;
   const bool vec = a.n_out % 8 == 0 && (size_t)a.y % 16 == 0;
-  for (int k = threadIdx.x; k < nm * CPR; k += 512) {
+  for (int k = tid; k < nm * CPR; k += 512) {
     const int m = k / CPR, c = k % CPR;
     const u32x4 val = *(const u32x4*)(lds + m * (TNO * 2) + ((c ^ (m & 15)) << 4));
     const int n = n0 + 8 * c;
@@ -291,48 +337,116 @@ __device__ inline void run_tile(const GemvArgs& a, int act, int e, int m0, int n
 
 template <class DT, int GB, bool GATED, class SH>
 __global__ __launch_bounds__(512, SH::OCC) void expert_tiles_kernel(const GemvArgs a, int E,
-                                                                    int tiles_n, int act) {
+                                                                    int tiles_n, int act, int smax,
+                                                                    float* part_sums) {
   constexpr int RB = SH::RING * SH::ROWS * 128;
   constexpr int EPI = SH::ROWS * (GATED ? TILE_N / 2 : TILE_N) * 2;
   __shared__ __attribute__((aligned(16))) unsigned char lds[RB > EPI ? RB : EPI];
-  int e, m0, m1, tn;
-  if (!find_tile<SH::ROWS>(a.offsets, E, tiles_n, blockIdx.x, e, m0, m1, tn)) return;
-  const int nm = m1 - m0;
+  Tile t;
+  if (!find_tile<SH::ROWS>(a.offsets, a.M, E, tiles_n, SH::CAP, smax, blockIdx.x, false, t)) return;
+  const int nm = t.m1 - t.m0;
   if constexpr (SH::IMAX >= 16) {
-    if (nm > 192) return run_tile<DT, GB, GATED, SH, 16>(a, act, e, m0, nm, tn, lds);
-    if (nm > 128) return run_tile<DT, GB, GATED, SH, 12>(a, act, e, m0, nm, tn, lds);
+    if (nm > 192) return run_tile<DT, GB, GATED, SH, 16>(a, act, t, lds, part_sums);
+    if (nm > 128) return run_tile<DT, GB, GATED, SH, 12>(a, act, t, lds, part_sums);
   }
   if constexpr (SH::IMAX >= 8) {
-    if (nm > 64) return run_tile<DT, GB, GATED, SH, 8>(a, act, e, m0, nm, tn, lds);
+    if (nm > 64) return run_tile<DT, GB, GATED, SH, 8>(a, act, t, lds, part_sums);
   }
-  run_tile<DT, GB, GATED, SH, 4>(a, act, e, m0, nm, tn, lds);
+  run_tile<DT, GB, GATED, SH, 4>(a, act, t, lds, part_sums);
 }
 
-template <class DT, int GB, class SH>
-static int launch_tiles(const GemvArgs& a, int E, int slots, int act, hipStream_t s) {
-  const int tiles_n = cdiv(a.N, TILE_N);
-  const long tiles_m = (long)slots / SH::ROWS + (slots < E ? slots : E);
-  const long grid = tiles_m * tiles_n;
-  if (grid > 0x7FFFFFFFL) return SQMP_EUNSUPPORTED;
-  if (act != ACT_NONE)
-    expert_tiles_kernel<DT, GB, true, SH><<<dim3((unsigned)grid), dim3(512), 0, s>>>(a, E, tiles_n, act);
-  else
-    expert_tiles_kernel<DT, GB, false, SH><<<dim3((unsigned)grid), dim3(512), 0, s>>>(a, E, tiles_n, act);
-  SQMP_LAUNCH_CHECK();
-  return SQMP_OK;
+// The split tiles: their parts' sums added in the order of K, activation, one rounding.
+// blockIdx.y: a 16-row slice of the tile
+template <class DT, bool GATED, class SH>
+__global__ __launch_bounds__(512) void join_kernel(const GemvArgs a, int E, int tiles_n, int act,
+                                                   int smax, const float* part_sums) {
+  typedef typename DT::T T;
+  Tile t;
+  if (!find_tile<SH::ROWS>(a.offsets, a.M, E, tiles_n, SH::CAP, smax, blockIdx.x, true, t)) return;
+  const int i = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m = 16 * i + (lane & 15), q = lane >> 4;
+  if (16 * i >= t.m1 - t.m0) return;
+  const f32x4* ps = (const f32x4*)part_sums + (long)t.split * t.parts * (SH::IMAX * 1024) + i * 1024 + threadIdx.x;
+  f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  for (int p = 0; p < t.parts; ++p) {
+    s[0] += ps[(long)p * (SH::IMAX * 1024)];
+    s[1] += ps[(long)p * (SH::IMAX * 1024) + 512];
+  }
+  if (m >= t.m1 - t.m0) return;
+  T* y = (T*)a.y + (long)(t.m0 + m) * a.n_out;
+#pragma unroll
+  for (int j = 0; j < (GATED ? 1 : 2); ++j) {
+    const int n0 = GATED ? t.tn * 128 + 16 * wave + 4 * q : t.tn * 256 + 32 * wave + 16 * j + 4 * q;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float f = s[j][r];
+      if constexpr (GATED) f = (act == ACT_SILU ? act_fn<ACT_SILU>(f) : act_fn<ACT_GELU>(f)) * s[1][r];
+      const int n = n0 + r;
+      if (n < a.n_out) y[n] = DT::from_f(a.bias ? f + DT::to_f(((const T*)a.bias)[n]) : f);
+    }
+  }
 }
 
 // The tile height, by the mean rows of an expert (64 / 128 / 256 rows, one box, 2 of 8 experts, 4096 ->
 // 2 x 11008 gated unless said): 32 rows each 151 / 163 / 189 us, 64: 193 / 203 / 239, 128: 301 / 275
 // / 367, 512: 793 / 701 / 705, 1024: 1567 / 1297 / 1349 (11008 -> 4096: 772 / 678 / 743), 2048 of
 // 4096 -> 4096: 615 / 470 / 449.  SQMP_EXPERT_ROWS overrides (A/B)
-template <class DT, int GB>
-static int by_shape(const GemvArgs& a, int E, int slots, int act, hipStream_t s) {
+static int tile_rows(int E, int slots) {
   const char* k = knob("SQMP_EXPERT_ROWS");
-  const int rows = k && atoi(k) > 0 ? atoi(k) : slots / E <= 64 ? 64 : slots / E < 2048 ? 128 : 256;
-  if (rows <= 64) return launch_tiles<DT, GB, Small>(a, E, slots, act, s);
-  if (rows <= 128) return launch_tiles<DT, GB, Medium>(a, E, slots, act, s);
-  return launch_tiles<DT, GB, Large>(a, E, slots, act, s);
+  const int mean = slots / E, r = k && atoi(k) > 0 ? atoi(k) : mean <= 64 ? 64 : mean < 2048 ? 128 : 256;
+  return r <= 64 ? 64 : r <= 128 ? 128 : 256;
+}
+
+// The parts a tile of the last round may be split into: at least 8 stages each, and only where
+// the last round is a good part of the whole (fewer than 4 full rounds at the least)
+static int max_parts(int E, int slots, int N, int Kp) {
+  const int rows = tile_rows(E, slots), cap = rows == 256 ? Large::CAP : Medium::CAP;
+  if ((long)cdiv(slots, rows) * cdiv(N, TILE_N) >= 4L * cap) return 1;
+  const int p = Kp / 64 / 8;
+  return p < 2 ? 1 : p > 16 ? 16 : p;
+}
+
+size_t expert_tiles_workspace(int E, int slots, int N, int Kp) {
+  if (slots <= 0 || max_parts(E, slots, N, Kp) == 1) return 0;
+  const int rows = tile_rows(E, slots), cap = rows == 256 ? Large::CAP : Medium::CAP;
+  // the parts of one round: no more than cap, and no more than every tile in max_parts
+  const long tiles = ((long)slots / rows + (slots < E ? slots : E)) * cdiv(N, TILE_N);
+  const long most = tiles * max_parts(E, slots, N, Kp);
+  return (size_t)(most < cap ? most : cap) * rows * TILE_N * sizeof(float);
+}
+
+template <class DT, int GB, bool GATED, class SH>
+static int launch_tiles(const GemvArgs& a, int E, int slots, int act, float* ws, hipStream_t s) {
+  const int tiles_n = cdiv(a.N, TILE_N);
+  const int smax = ws ? max_parts(E, slots, a.N, a.Kp) : 1;
+  const long tiles = ((long)slots / SH::ROWS + (slots < E ? slots : E)) * tiles_n;
+  const long extra = smax > 1 ? (tiles * smax < SH::CAP ? tiles * smax : SH::CAP) : 0;
+  const long grid = tiles + extra;
+  if (grid > 0x7FFFFFFFL) return SQMP_EUNSUPPORTED;
+  expert_tiles_kernel<DT, GB, GATED, SH><<<dim3((unsigned)grid), dim3(512), 0, s>>>(a, E, tiles_n, act, smax, ws);
+  SQMP_LAUNCH_CHECK();
+  if (smax > 1) {
+    const long nj = tiles < SH::CAP / 2 ? tiles : SH::CAP / 2;  // two parts or more: at most cap / 2
+    join_kernel<DT, GATED, SH><<<dim3((unsigned)nj, SH::IMAX), dim3(512), 0, s>>>(a, E, tiles_n, act, smax, ws);
+    SQMP_LAUNCH_CHECK();
+  }
+  return SQMP_OK;
+}
+
+template <class DT, int GB, bool GATED>
+static int by_shape(const GemvArgs& a, int E, int slots, int act, float* ws, hipStream_t s) {
+  switch (tile_rows(E, slots)) {
+    case 64: return launch_tiles<DT, GB, GATED, Small>(a, E, slots, act, ws, s);
+    case 128: return launch_tiles<DT, GB, GATED, Medium>(a, E, slots, act, ws, s);
+    default: return launch_tiles<DT, GB, GATED, Large>(a, E, slots, act, ws, s);
+  }
+}
+
+template <class DT>
+static int by_group_act(const GemvArgs& a, int E, int slots, int act, float* ws, hipStream_t s) {
+  if (a.Gw == 32)
+    return act != ACT_NONE ? by_shape<DT, 2, true>(a, E, slots, act, ws, s) : by_shape<DT, 2, false>(a, E, slots, act, ws, s);
+  return act != ACT_NONE ? by_shape<DT, 1, true>(a, E, slots, act, ws, s) : by_shape<DT, 1, false>(a, E, slots, act, ws, s);
 }
 
 bool expert_tiles_ok(const GemvArgs& a, int dtype, int E, long x_rows) {
@@ -341,10 +455,9 @@ bool expert_tiles_ok(const GemvArgs& a, int dtype, int E, long x_rows) {
          (a.rows ? x_rows : 256) * a.ldx * 2 < 0xFFFF0000L;
 }
 
-int launch_expert_tiles(const GemvArgs& a, int dtype, int E, int slots, int act, hipStream_t s) {
-  if (dtype == SQMP_F16)
-    return a.Gw == 32 ? by_shape<F16, 2>(a, E, slots, act, s) : by_shape<F16, 1>(a, E, slots, act, s);
-  return a.Gw == 32 ? by_shape<BF16, 2>(a, E, slots, act, s) : by_shape<BF16, 1>(a, E, slots, act, s);
+int launch_expert_tiles(const GemvArgs& a, int dtype, int E, int slots, int act, float* ws,
+                        hipStream_t s) {
+  return dtype == SQMP_F16 ? by_group_act<F16>(a, E, slots, act, ws, s) : by_group_act<BF16>(a, E, slots, act, ws, s);
 }
 
 }  // namespace w4

@@ -181,9 +181,21 @@ static int check_operand(const void* x, long ldx, int dtype, int N, int Kp, int 
 
 }  // namespace w4
 
+// (0 where the few-row kernel runs, which splits K inside a workgroup)
+extern "C" size_t sqmp_gemv_workspace_bytes(int dtype, int M, int N, int Kp) {
+  if (M <= 16 || N <= 0 || Kp <= 0 || dtype == SQMP_F32) return 0;
+  return w4::expert_tiles_workspace(1, M, N, Kp);
+}
+
+extern "C" size_t sqmp_expert_workspace_bytes(int dtype, int E, int slots, int N, int Kp) {
+  if (E <= 0 || slots < 8 * (long)E || N <= 0 || Kp <= 0 || dtype == SQMP_F32) return 0;
+  return w4::expert_tiles_workspace(E, slots, N, Kp);
+}
+
 extern "C" int sqmp_gemv_w4(const void* x, long ldx, const void* codes_t, const void* scale_t,
                             const void* sal_t, const void* bias, void* y, int dtype, int M, int N,
-                            int Kp, int S_pad, int Gw, int ngw, void* stream) {
+                            int Kp, int S_pad, int Gw, int ngw, void* workspace, size_t ws_bytes,
+                            void* stream) {
   SQMP_DEVICE_GUARD(stream);
   if (!x || !codes_t || !scale_t || !y || (S_pad > 0 && !sal_t)) return SQMP_EINVAL;
   if (M < 0 || M > SQMP_GEMV_MAX_ROWS) return SQMP_EINVAL;
@@ -195,6 +207,10 @@ extern "C" int sqmp_gemv_w4(const void* x, long ldx, const void* codes_t, const 
   a.bias = bias, a.y = y, a.M = M, a.N = N, a.n_out = N;
   a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
   hipStream_t s = (hipStream_t)stream;
+  if (M > 16 && w4::expert_tiles_ok(a, dtype, 1, M))
+    return w4::launch_expert_tiles(a, dtype, 1, M, w4::ACT_NONE,
+                                   workspace && ws_bytes >= w4::expert_tiles_workspace(1, M, N, Kp)
+                                       ? (float*)workspace : nullptr, s);
   if (dtype == SQMP_F32) return w4::by_group<F32, false, w4::ACT_NONE>(a, 1, M, s);
   if (dtype == SQMP_F16) return w4::by_group<F16, false, w4::ACT_NONE>(a, 1, M, s);
   return w4::by_group<BF16, false, w4::ACT_NONE>(a, 1, M, s);
@@ -204,7 +220,8 @@ extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* row
                                      const int32_t* offsets, int E, const void* codes_t,
                                      const void* scale_t, const void* sal_t, void* y, int dtype,
                                      int slots, int x_rows, int N, int n_out, int Kp, int S_pad, int Gw,
-                                     int ngw, int act, void* stream) {
+                                     int ngw, int act, void* workspace, size_t ws_bytes,
+                                     void* stream) {
   SQMP_DEVICE_GUARD(stream);
   if (!x || !offsets || !codes_t || !scale_t || !y || (S_pad > 0 && !sal_t)) return SQMP_EINVAL;
   if (slots < 0 || x_rows < 0 || E <= 0 || E > 65535 || top_k <= 0) return SQMP_EINVAL;
@@ -224,7 +241,9 @@ extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* row
   // 8 of 16 rows 147 / 115 us); SQMP_EXPERT_ROWS = 0 / a tile height overrides (A/B)
   const char* k = knob("SQMP_EXPERT_ROWS");
   if (w4::expert_tiles_ok(a, dtype, E, x_rows) && (k ? atoi(k) > 0 : slots >= 8 * E))
-    return w4::launch_expert_tiles(a, dtype, E, slots, act, s);
+    return w4::launch_expert_tiles(a, dtype, E, slots, act,
+                                   workspace && ws_bytes >= w4::expert_tiles_workspace(E, slots, N, Kp)
+                                       ? (float*)workspace : nullptr, s);
   const int est = cdiv(slots, E) * 2;  // rows of a busy expert (any count is right)
 #define SQMP_EX(DTT)                                                                  \
   switch (act) {                                                                      \

@@ -23,10 +23,13 @@ struct GemvArgs {
   int n_out;               // columns of y (gated: N / 2 rounded; else N)
 };
 
-// The tile kernel of many rows per expert: whether it takes the call (x_rows: rows of x), and the
-// launch.
+// The tile kernels (many rows per weight): whether they take the call (x_rows: rows of x); the
+// bytes of the workspace in which the K parts of split tiles meet (0: none); the launch (ws NULL: no
+// tile is split).  a.offsets NULL: one weight, slots = a.M rows.
 bool expert_tiles_ok(const GemvArgs& a, int dtype, int E, long x_rows);
-int launch_expert_tiles(const GemvArgs& a, int dtype, int E, int slots, int act, hipStream_t s);
+size_t expert_tiles_workspace(int E, int slots, int N, int Kp);
+int launch_expert_tiles(const GemvArgs& a, int dtype, int E, int slots, int act, float* ws,
+                        hipStream_t s);
 
 }  // namespace w4
 }  // namespace sqmp

@@ -49,10 +49,16 @@ class Routing:
 
 
 def _plan_buffers(T: int, k: int, E: int, dev):
+    """(offsets, rows, slots, workspace pointer and size), one allocation for the first three."""
     n = load().sqmp_route_workspace_bytes(T, E)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    i32 = dict(dtype=torch.int32, device=dev)
-    return (torch.empty(E + 1, **i32), torch.empty(T * k, **i32), torch.empty(T * k, **i32), ws, n)
+    rows, slots, offsets = torch.empty(2 * T * k + E + 1, dtype=torch.int32,
+                                       device=dev).split((T * k, T * k, E + 1))
+    return offsets, rows, slots, ws, n
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _check_sizes(what: str, E: int, k: int):
@@ -81,10 +87,10 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
     ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
     weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
     offsets, rows, slots, ws, n = _plan_buffers(T, top_k, E, dev)
-    p = ops._p
-    check(load().sqmp_route(p(logits), max(logits.stride(0), E), dt, T, E, top_k, int(normalize),
-                            p(weights), p(ids), p(offsets), p(rows), p(slots), p(ws), n,
-                            ops._stream(logits)), "route")
+    check(load().sqmp_route(logits.data_ptr(), max(logits.stride(0), E), dt, T, E, top_k,
+                            int(normalize), weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(),
+                            rows.data_ptr(), slots.data_ptr(), _ptr(ws), n,
+                            ops._raw_stream(dev.index)), "route")
     return Routing(ids, weights, offsets, rows, slots, E)
 
 
@@ -105,9 +111,9 @@ def plan_routes(ids: torch.Tensor, weights: torch.Tensor, num_experts: int) -> R
         ids = (ids.long().clamp(-1, num_experts)).to(torch.int32)  # (no id may wrap into range)
     ids = ids.contiguous()
     offsets, rows, slots, ws, n = _plan_buffers(T, k, num_experts, ids.device)
-    p = ops._p
-    check(load().sqmp_plan_routes(p(ids), T, num_experts, k, p(offsets), p(rows), p(slots), p(ws),
-                                  n, ops._stream(ids)), "plan_routes")
+    check(load().sqmp_plan_routes(ids.data_ptr(), T, num_experts, k, offsets.data_ptr(),
+                                  rows.data_ptr(), slots.data_ptr(), _ptr(ws), n,
+                                  ops._raw_stream(ids.device.index)), "plan_routes")
     return Routing(ids, weights.float().contiguous(), offsets, rows, slots, num_experts)
 
 
@@ -264,13 +270,15 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
     if S == 0:
         return out
     a, pairs = _operand(x, pe, routing, rows == "slot")
-    p = ops._p
-    check(load().sqmp_expert_linear_w4(p(a), a.stride(0) if a.shape[0] > 1 else pe.Kp + pe.S_pad,
-                                       p(pairs), routing.top_k, p(routing.offsets), pe.num_experts,
-                                       p(pe.codes_t), p(pe.scale_t), p(pe.sal_t), p(out),
-                                       ops._dtype_code(pe.dtype), S, a.shape[0], pe.N, pe.n_out, pe.Kp,
-                                       pe.S_pad, pe.Gw, pe.ngw, ACTS[act], ops._stream(x)),
-          "expert_linear")
+    lib, code = load(), ops._dtype_code(pe.dtype)
+    n = lib.sqmp_expert_workspace_bytes(code, pe.num_experts, S, pe.N, pe.Kp)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    check(lib.sqmp_expert_linear_w4(a.data_ptr(), a.stride(0) if a.shape[0] > 1 else pe.Kp + pe.S_pad,
+                                    _ptr(pairs), routing.top_k, routing.offsets.data_ptr(),
+                                    pe.num_experts, pe.codes_t.data_ptr(), pe.scale_t.data_ptr(),
+                                    _ptr(pe.sal_t), out.data_ptr(), code, S, a.shape[0], pe.N,
+                                    pe.n_out, pe.Kp, pe.S_pad, pe.Gw, pe.ngw, ACTS[act], _ptr(ws), n,
+                                    ops._raw_stream(x.device.index)), "expert_linear")
     return out
 
 
@@ -293,9 +301,9 @@ def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = Non
         raise ValueError(f"combine: out must be contiguous {z.dtype} [{T}, {H}] on {z.device}")
     if T == 0:
         return out
-    p = ops._p
-    check(load().sqmp_combine(p(z), dt, T, k, H, p(routing.slots), p(routing.weights), p(out),
-                              ops._stream(z)), "combine")
+    check(load().sqmp_combine(z.data_ptr(), dt, T, k, H, routing.slots.data_ptr(),
+                              routing.weights.data_ptr(), out.data_ptr(),
+                              ops._raw_stream(z.device.index)), "combine")
     return out
 
 

@@ -39,6 +39,12 @@ def _stream(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+# the current stream's handle as an int (torch.cuda.current_stream builds a Stream object: 1.8 us
+# against 0.1 us, a fifth of a few-row call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _require_gpu(t: torch.Tensor, what: str):
     if t.device.type != "cuda":
         raise RuntimeError(
@@ -97,6 +103,7 @@ class PackedWeight:
     sib_maps: Optional[tuple] = field(default=None)      # sibling position map (sqmp_permute_act)
     ident: Optional[bool] = field(default=None)          # packed order == column order (identity_layout)
     gemv: Optional[tuple] = field(default=None)          # (codes_t, scale_t, sal_t) of gemv
+    gemv_args: Optional[tuple] = field(default=None)     # what gemv passes for this weight
 
     @property
     def gemm_operand(self):
@@ -1055,15 +1062,14 @@ def gemv_operands(pw: PackedWeight):
     """(codes_t, scale_t, sal_t) of gemv: fq7_operands' copies where those are J = 2 (fp16 /
     bf16), else its own; built once per packed weight.  Inside a HIP-graph capture nothing is
     kept (the copy would be written at replay only): call gemv once before capturing."""
-    if pw.gemv is None and pw.fq7 is not None and pw.fq7[3] == 2:
-        pw.gemv = pw.fq7[:3]
     if pw.gemv is not None:
         return pw.gemv
-    ops_t = tile_major(pw.codes, pw.wscale, pw.wsal, pw.N, pw.Kp, pw.S_pad, pw.ngw, pw.dtype)
+    adopt = pw.fq7 is not None and pw.fq7[3] == 2
+    ops_t = pw.fq7[:3] if adopt else tile_major(pw.codes, pw.wscale, pw.wsal, pw.N, pw.Kp, pw.S_pad,
+                                                pw.ngw, pw.dtype)
     if torch.cuda.is_current_stream_capturing():
         return ops_t
-    # (built on this stream, read later from any other)
-    torch.cuda.current_stream(pw.codes.device).synchronize()
+    torch.cuda.synchronize(pw.codes.device)  # (built on one stream, read later from any)
     pw.gemv = ops_t
     if pw.fq7 is None and FQ7_J == 2 and pw.dtype != torch.float32:
         pw.fq7 = ops_t + (2,)
@@ -1098,37 +1104,77 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
     x: [M, K] in the columns' order -- a 4-bit weight with D activations -- or, with `packed`,
     the [M, Kp + S_pad] operand of quant_act_fp.  Any strides; rows that are not 16-B aligned,
     and packed weights in an order of their own, are copied first (sqmp_pack_rows)."""
-    _require_gpu(x, "gemv")
-    if x.dim() != 2:
-        raise ValueError(f"gemv: x must have 2 dimensions, got {tuple(x.shape)}")
-    M = x.shape[0]
-    L = pw.Kp + pw.S_pad
-    if x.shape[1] != (L if packed else pw.K):
-        raise ValueError(f"gemv: x has {x.shape[1]} columns, the weight {L if packed else pw.K}")
+    if not x.is_cuda:
+        _require_gpu(x, "gemv")
+    a = pw.gemv_args or _gemv_args(pw)
+    dtype, device, code, L, per, ident, codes_t, scale_t, sal_t, N, tail = a
+    shape = x.shape
+    if len(shape) != 2:
+        raise ValueError(f"gemv: x must have 2 dimensions, got {tuple(shape)}")
+    M = shape[0]
+    if shape[1] != (L if packed else pw.K):
+        raise ValueError(f"gemv: x has {shape[1]} columns, the weight {L if packed else pw.K}")
     if M > GEMV_MAX_ROWS:
         raise ValueError(f"gemv: {M} rows, at most {GEMV_MAX_ROWS}")
+    if x.dtype != dtype:
+        raise RuntimeError(f"expected input dtype {dtype}, got {x.dtype}")
+    if x.device != device:
+        raise RuntimeError(f"gemv: x on {x.device}, the weight on {device}")
+    bp = None
+    if bias is not None:
+        if bias.dtype != dtype or bias.device != device or bias.numel() != N:
+            raise RuntimeError(f"gemv: bias {bias.dtype} [{bias.numel()}] on {bias.device} does "
+                               f"not match {dtype} [{N}] on {device}")
+        bias = bias.reshape(-1).contiguous()
+        bp = bias.data_ptr()
+    y = x.new_empty((M, N))
+    if M == 0:
+        return y
+    ld, s1 = x.stride()
+    xp = x.data_ptr()
+    if not (packed or ident):
+        x = pack_rows(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
+        xp, ld = x.data_ptr(), L
+    elif M == 1 and s1 == 1 and xp % 16 == 0:
+        ld = L
+    elif s1 != 1 or xp % 16 or ld < L or ld % per:
+        x = x.clone(memory_format=torch.contiguous_format)
+        xp, ld = x.data_ptr(), L
+    lib = load()
+    ws, wn = None, 0
+    if M > 16:
+        wn = lib.sqmp_gemv_workspace_bytes(code, M, N, pw.Kp)
+        if wn:
+            ws = torch.empty(wn, dtype=torch.uint8, device=device)
+    status = lib.sqmp_gemv_w4(xp, ld, codes_t, scale_t, sal_t, bp, y.data_ptr(), code, M, N, *tail,
+                              None if ws is None else ws.data_ptr(), wn, _raw_stream(device.index))
+    if status:
+        check(status, "gemv")
+    return y
+
+
+def _gemv_args(pw: PackedWeight):
+    """gemv's arguments that depend on the weight alone; kept on it once its operands and order are
+    known for good (not inside a capture)."""
     if not gemv_eligible(pw):
         raise ValueError(f"gemv: needs 4-bit codes in groups of a multiple of 8 columns (n_bits "
                          f"{pw.n_bits}, group {pw.Gw})")
-    if x.dtype != pw.dtype:
-        raise RuntimeError(f"expected input dtype {pw.dtype}, got {x.dtype}")
-    if x.device != pw.codes.device:
-        raise RuntimeError(f"gemv: x on {x.device}, the weight on {pw.codes.device}")
-    if bias is not None:
-        if bias.dtype != pw.dtype or bias.device != x.device or bias.numel() != pw.N:
-            raise RuntimeError(f"gemv: bias {bias.dtype} [{bias.numel()}] on {bias.device} does "
-                               f"not match {pw.dtype} [{pw.N}] on {x.device}")
-        bias = bias.reshape(-1).contiguous()
-    y = torch.empty((M, pw.N), dtype=pw.dtype, device=x.device)
-    if M == 0:
-        return y
-    codes_t, scale_t, sal_t = gemv_operands(pw)
-    if not (packed or identity_layout(pw)):
-        x = pack_rows(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
-    elif not _operand_rows(x, L):
-        x = x.clone(memory_format=torch.contiguous_format)
-    check(load().sqmp_gemv_w4(_p(x), L if M == 1 else x.stride(0), _p(codes_t), _p(scale_t),
-                              _p(sal_t) if pw.S_pad else None, _p(bias), _p(y),
-                              _dtype_code(pw.dtype), M, pw.N, pw.Kp, pw.S_pad, pw.Gw, pw.ngw,
-                              _stream(x)), "gemv")
-    return y
+    t = gemv_operands(pw)
+    ident = identity_layout(pw)
+    dev = pw.codes.device
+    a = (pw.dtype, dev, _dtype_code(pw.dtype), pw.Kp + pw.S_pad,
+         4 if pw.dtype == torch.float32 else 8, ident, t[0].data_ptr(), t[1].data_ptr(),
+         t[2].data_ptr() if pw.S_pad else None, pw.N, (pw.Kp, pw.S_pad, pw.Gw, pw.ngw))
+    if pw.gemv is t and pw.ident is not None:
+        pw.gemv_args = a
+    else:
+        a = a[:6] + (_Keep(t, a[6]), _Keep(t, a[7]), None if a[8] is None else _Keep(t, a[8])) + a[9:]
+    return a
+
+
+class _Keep(int):
+    """A pointer that holds the tensors it points into (operands that nothing else keeps)."""
+    def __new__(cls, owner, ptr):
+        self = super().__new__(cls, ptr)
+        self.owner = owner
+        return self

@@ -18,7 +18,7 @@ def lib():
 def test_gemv_refusals(lib):
     def call(x=P, ldx=128, codes=P, scale=P, sal=None, bias=None, y=P, dtype=1, M=1, N=32, Kp=128, S_pad=0,
              Gw=64, ngw=2):
-        return lib.sqmp_gemv_w4(x, ldx, codes, scale, sal, bias, y, dtype, M, N, Kp, S_pad, Gw, ngw, None)
+        return lib.sqmp_gemv_w4(x, ldx, codes, scale, sal, bias, y, dtype, M, N, Kp, S_pad, Gw, ngw, None, 0, None)
     assert call(M=0) == 0                                   # nothing to do
     for bad in (dict(x=None), dict(codes=None), dict(scale=None), dict(y=None), dict(S_pad=64, ldx=192),
                 dict(M=-1), dict(M=65), dict(N=0), dict(Kp=64), dict(Kp=100), dict(S_pad=-64),
@@ -34,7 +34,7 @@ def test_expert_linear_refusals(lib):
     def call(x=P, ldx=128, rows=None, top_k=2, offsets=P, E=4, codes=P, scale=P, sal=None, y=P, dtype=1, slots=8,
              x_rows=4, N=32, n_out=32, Kp=128, S_pad=0, Gw=64, ngw=2, act=0):
         return lib.sqmp_expert_linear_w4(x, ldx, rows, top_k, offsets, E, codes, scale, sal, y, dtype, slots,
-                                         x_rows, N, n_out, Kp, S_pad, Gw, ngw, act, None)
+                                         x_rows, N, n_out, Kp, S_pad, Gw, ngw, act, None, 0, None)
     assert call(slots=0) == 0
     for bad in (dict(x=None), dict(offsets=None), dict(y=None), dict(E=0), dict(E=65536), dict(top_k=0),
                 dict(slots=-1), dict(x_rows=-1), dict(act=3), dict(act=-1), dict(n_out=31), dict(act=1),

@@ -171,7 +171,7 @@ def plain_experts(x, w, r, by_slot):
 SHAPES = [(1, 8, 2, 64, 128, 64), (9, 3, 1, 33, 100, 32), (130, 5, 3, 96, 256, 64),
           (300, 40, 6, 50, 192, 64), (40, 2, 2, 300, 1000, 8), (1100, 4, 2, 264, 384, 128),
           (500, 2, 1, 130, 256, 32), (256, 1, 1, 257, 128, 64), (777, 3, 3, 512, 640, 640),
-          (260, 256, 4, 16, 128, 128)]
+          (260, 256, 4, 16, 128, 128), (330, 3, 1, 512, 2048, 128), (64, 8, 2, 96, 4096, 64)]
 
 
 @pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
@@ -206,7 +206,7 @@ def test_tile_heights_agree(height, dt, monkeypatch):
     ids = torch.repeat_interleave(torch.arange(len(sizes), device="cuda"),
                                   torch.tensor(sizes, device="cuda"))
     ids = ids[torch.randperm(len(ids), generator=g, device="cuda")].view(-1, 1)
-    E, T, N, K, G = len(sizes), len(ids), 283, 640, 64
+    E, T, N, K, G = len(sizes), len(ids), 283, 1152, 64   # (18 stages: up to two parts)
     codes, scales = int_weight((E, N, K), G, D, g)
     pe = experts.pack_expert_codes(codes, scales, G)
     r = experts.plan_routes(ids, torch.ones(T, 1, device="cuda"), E)
