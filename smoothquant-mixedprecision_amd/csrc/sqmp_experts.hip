@@ -55,18 +55,21 @@ __device__ inline int brev3(int c) { return ((c & 1) << 2) | (c & 2) | ((c >> 2)
 
 constexpr int TILE_N = 256;      // weight rows per tile
 
-// A kernel of tiles of up to 16 IMAX slots: RING LDS stages of activations, DW stages of codes in
-// registers ahead, OCC waves per SIMD (two workgroups per CU at 4); SPLIT: waves 0-3 issue all
-// LDS-DMA and waves 4-7 run at a higher wave priority
-template <int IMAX_, int RING_, int DW_, int OCC_, bool SPLIT_>
+// A kernel of tiles of up to 16 IMAX slots: a ring of RB bytes of activations in LDS, OCC waves per
+// SIMD (two workgroups per CU at 4); SPLIT: waves 0-3 issue all LDS-DMA and waves 4-7 run at a
+// higher wave priority
+template <int IMAX_, int RB_, int OCC_, bool SPLIT_>
 struct Shape {
-  static constexpr int IMAX = IMAX_, RING = RING_, DW = DW_, OCC = OCC_, ROWS = 16 * IMAX_;
+  static constexpr int IMAX = IMAX_, RB = RB_, OCC = OCC_, ROWS = 16 * IMAX_;
   static constexpr bool SPLIT = SPLIT_;
   static constexpr int CAP = OCC_ == 4 ? 512 : 256;  // workgroups the 256 CUs hold at once
+  // of a tile of 16 I slots: ring stages, and stages of codes in registers ahead -- deeper for
+  // few rows, whose stages are shorter than a load
+  static constexpr int ring(int I) { return RB_ / (I * 2048) < 8 ? RB_ / (I * 2048) : 8; }
+  static constexpr int ahead(int I) { return I == 4 ? 4 : 2; }
 };
-using Large = Shape<16, 4, 2, 1, true>;
-using Medium = Shape<8, 4, 2, 4, false>;
-using Small = Shape<4, 8, 4, 4, false>;
+using Large = Shape<16, 131072, 1, true>;
+using Medium = Shape<8, 65536, 4, false>;
 
 // What a workgroup computes: expert e, slots [m0, m1), weight tile tn, part `part` of `parts` of the
 // K stages (`split`: its place among the split tiles)
@@ -149,7 +152,7 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
                                 float* part_sums) {
   typedef typename DT::T T;
   constexpr int J = 2, NA = I / 4, PF = I == 16 || (I == 8 && SH::OCC == 4) ? 2 : 3;
-  constexpr int SLOT = I * 16 * 128, RING = SH::RING, DW = SH::DW;
+  constexpr int SLOT = I * 16 * 128, RING = SH::ring(I), DW = SH::ahead(I);
   constexpr int NO = SH::SPLIT ? 2 : 1;  // waves whose pieces a loading wave issues
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -205,7 +208,7 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
   };
   auto load_w = [&](int kt, Codes& c) {
     c.w = *(const u32x4*)(codes + (long)kt * 256);
-    const int g = GB == 1 ? min((kt * 64) / a.Gw, a.ngw - 1) : min(2 * kt + (q & 1), a.ngw - 1);
+    const int g = GB == 1 ? group_of(kt, a) : min(2 * kt + (q & 1), a.ngw - 1);
     c.s = *(const uint32_t*)(scale + (long)g * 32);
   };
 
@@ -339,7 +342,7 @@ template <class DT, int GB, bool GATED, class SH>
 __global__ __launch_bounds__(512, SH::OCC) void expert_tiles_kernel(const GemvArgs a, int E,
                                                                     int tiles_n, int act, int smax,
                                                                     float* part_sums) {
-  constexpr int RB = SH::RING * SH::ROWS * 128;
+  constexpr int RB = SH::RB;
   constexpr int EPI = SH::ROWS * (GATED ? TILE_N / 2 : TILE_N) * 2;
   __shared__ __attribute__((aligned(16))) unsigned char lds[RB > EPI ? RB : EPI];
   Tile t;
@@ -387,14 +390,13 @@ __global__ __launch_bounds__(512) void join_kernel(const GemvArgs a, int E, int 
   }
 }
 
-// The tile height, by the mean rows of an expert (64 / 128 / 256 rows, one box, 2 of 8 experts, 4096 ->
-// 2 x 11008 gated unless said): 32 rows each 151 / 163 / 189 us, 64: 193 / 203 / 239, 128: 301 / 275
-// / 367, 512: 793 / 701 / 705, 1024: 1567 / 1297 / 1349 (11008 -> 4096: 772 / 678 / 743), 2048 of
-// 4096 -> 4096: 615 / 470 / 449.  SQMP_EXPERT_ROWS overrides (A/B)
+// The tile height, by the mean rows of an expert (128 / 256 rows, one box, 2 of 8 experts, 4096 ->
+// 2 x 11008 gated unless said): 128 rows each 275 / 367 us, 512: 701 / 705, 1024: 1297 / 1349 (11008
+// -> 4096: 678 / 743), 2048 of 4096 -> 4096: 470 / 449.  SQMP_EXPERT_ROWS overrides (A/B)
 static int tile_rows(int E, int slots) {
   const char* k = knob("SQMP_EXPERT_ROWS");
-  const int mean = slots / E, r = k && atoi(k) > 0 ? atoi(k) : mean <= 64 ? 64 : mean < 2048 ? 128 : 256;
-  return r <= 64 ? 64 : r <= 128 ? 128 : 256;
+  const int r = k && atoi(k) > 0 ? atoi(k) : slots / E < 2048 ? 128 : 256;
+  return r <= 128 ? 128 : 256;
 }
 
 // The parts a tile of the last round may be split into: at least 8 stages each, and only where
@@ -435,11 +437,8 @@ static int launch_tiles(const GemvArgs& a, int E, int slots, int act, float* ws,
 
 template <class DT, int GB, bool GATED>
 static int by_shape(const GemvArgs& a, int E, int slots, int act, float* ws, hipStream_t s) {
-  switch (tile_rows(E, slots)) {
-    case 64: return launch_tiles<DT, GB, GATED, Small>(a, E, slots, act, ws, s);
-    case 128: return launch_tiles<DT, GB, GATED, Medium>(a, E, slots, act, ws, s);
-    default: return launch_tiles<DT, GB, GATED, Large>(a, E, slots, act, ws, s);
-  }
+  if (tile_rows(E, slots) == 128) return launch_tiles<DT, GB, GATED, Medium>(a, E, slots, act, ws, s);
+  return launch_tiles<DT, GB, GATED, Large>(a, E, slots, act, ws, s);
 }
 
 template <class DT>

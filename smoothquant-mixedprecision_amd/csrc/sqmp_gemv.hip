@@ -73,7 +73,7 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
           st.s[2 * s + 1] = scale[(long)g * 32 + 1];
         }
       } else {
-        const int g = GB == 1 ? min((kt * 64) / a.Gw, a.ngw - 1) : min(2 * kt + (q & 1), a.ngw - 1);
+        const int g = GB == 1 ? group_of(kt, a) : min(2 * kt + (q & 1), a.ngw - 1);
         st.s[0] = scale[(long)g * 32];
         st.s[1] = scale[(long)g * 32 + 1];
       }
@@ -206,6 +206,7 @@ extern "C" int sqmp_gemv_w4(const void* x, long ldx, const void* codes_t, const 
   a.x = x, a.ldx = ldx, a.codes = (const uint32_t*)codes_t, a.scale = scale_t, a.sal = sal_t;
   a.bias = bias, a.y = y, a.M = M, a.N = N, a.n_out = N;
   a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
+  w4::set_groups(a);
   hipStream_t s = (hipStream_t)stream;
   if (M > 16 && w4::expert_tiles_ok(a, dtype, 1, M))
     return w4::launch_expert_tiles(a, dtype, 1, M, w4::ACT_NONE,
@@ -236,11 +237,12 @@ extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* row
   a.x = x, a.ldx = ldx, a.codes = (const uint32_t*)codes_t, a.scale = scale_t, a.sal = sal_t;
   a.y = y, a.N = N, a.n_out = n_out, a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
   a.rows = rows, a.offsets = offsets, a.top_k = top_k;
+  w4::set_groups(a);
   hipStream_t s = (hipStream_t)stream;
   // tiles from 8 rows per expert on (few-row kernel / 64-row tiles: 64 experts of 6 rows 56 / 71 us,
   // 8 of 16 rows 147 / 115 us); SQMP_EXPERT_ROWS = 0 / a tile height overrides (A/B)
   const char* k = knob("SQMP_EXPERT_ROWS");
-  if (w4::expert_tiles_ok(a, dtype, E, x_rows) && (k ? atoi(k) > 0 : slots >= 8 * E))
+  if (w4::expert_tiles_ok(a, dtype, E, x_rows) && (k ? atoi(k) > 0 : slots >= 8L * E))
     return w4::launch_expert_tiles(a, dtype, E, slots, act,
                                    workspace && ws_bytes >= w4::expert_tiles_workspace(E, slots, N, Kp)
                                        ? (float*)workspace : nullptr, s);

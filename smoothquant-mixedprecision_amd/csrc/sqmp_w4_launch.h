@@ -20,8 +20,20 @@ struct GemvArgs {
   const int32_t* rows;     // slot -> flat (token * top_k + j), or NULL: x row = slot
   const int32_t* offsets;  // [E + 1]
   int top_k;
+  uint32_t gmul;           // stage -> group (set_groups)
   int n_out;               // columns of y (gated: N / 2 rounded; else N)
 };
+
+// The group of stage kt is kt / d, d = Gw / 64 stages per group, without a division: kt m / 2^31
+// with m = ceil(2^31 / d) exceeds kt / d by kt (m d - 2^31) / (d 2^31) < 1 / d while kt d < 2^31
+// (d and kt are below 2^15 for rows of up to 2 million positions)
+inline void set_groups(GemvArgs& a) {
+  const uint32_t d = a.Gw >= 64 ? (uint32_t)a.Gw / 64 : 1;
+  a.gmul = (uint32_t)(((1ull << 31) + d - 1) / d);
+}
+__device__ inline int group_of(int kt, const GemvArgs& a) {
+  return min((int)__umulhi((uint32_t)kt * 2u, a.gmul), a.ngw - 1);
+}
 
 // The tile kernels (many rows per weight): whether they take the call (x_rows: rows of x); the
 // bytes of the workspace in which the K parts of split tiles meet (0: none); the launch (ws NULL: no
