@@ -200,16 +200,16 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
 
   // weights
   const long wb = (long)e * ((a.N + 255) / 256 * 8) + tn * 8 + wave;
-  const uint32_t* codes = a.codes + wb * nkm_all * 256 + lane * 4;
-  const T* scale = (const T*)a.scale + wb * a.ngw * 32 + r16 * 2;
+  const __amdgpu_buffer_rsrc_t rW = rsrc_of(a.codes + wb * nkm_all * 256);
+  const __amdgpu_buffer_rsrc_t rS = rsrc_of((const T*)a.scale + wb * a.ngw * 32);
   struct Codes {
     u32x4 w;
     uint32_t s;
   };
   auto load_w = [&](int kt, Codes& c) {
-    c.w = *(const u32x4*)(codes + (long)kt * 256);
-    const int g = GB == 1 ? group_of(kt, a) : min(2 * kt + (q & 1), a.ngw - 1);
-    c.s = *(const uint32_t*)(scale + (long)g * 32);
+    c.w = load16(rW, (uint32_t)lane * 16, (uint32_t)kt * 1024);
+    if constexpr (GB == 1) c.s = load4(rS, (uint32_t)r16 * 4, (uint32_t)group_of(kt, a) * 64);
+    else c.s = load4(rS, (uint32_t)min(2 * kt + (q & 1), a.ngw - 1) * 64 + (uint32_t)r16 * 4, 0);
   };
 
   f32x4 acc[I][J];
@@ -240,34 +240,39 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
     }
   };
 
-  // The decode of stage kt comes before the next activation loads are issued: the compiler waits
-  // for the codes by counting its own loads, and would otherwise wait for those as well.
+  // Codes are decoded between the MFMAs: sub-step 1 of this stage in its first blocks, sub-step 0 of
+  // the next one in the blocks that no longer use it, so vector and matrix pipes work side by side
+  // and a stage starts with its MFMAs.  (The compiler waits for codes by counting its own loads only,
+  // which makes it wait for LDS-DMA issued in between as well: codes are loaded far ahead.)
   Codes cs[DW];
 #pragma unroll
   for (int p = 0; p < (RING - 1 > DW ? RING - 1 : DW); ++p) {
     if (p < RING - 1 && k0 + p < nkt) issue_a(k0 + p);
-    if (p < DW && k0 + p < nkm) load_w(k0 + p, cs[p]);
+    if (p < DW) load_w(min(k0 + p, nkm - 1), cs[p]);
   }
-  auto step = [&](int kt, Codes& c) {
-    uint32_t sp[J];
-    sp[0] = Dec<DT>::prep(c.s & 0xFFFFu), sp[1] = Dec<DT>::prep(c.s >> 16);
-    u32x4 bf[2][J];
+  u32x4 bf[2][J];
+  auto dec = [&](const Codes& c, int s, int n) {  // half n & 1 of fragment [s][n / 2]
+    const int j = n >> 1;
+    DecHalf<DT>::run(bf[s][j], c.w[2 * j + s], Dec<DT>::prep(j ? c.s >> 16 : c.s & 0xFFFFu), dk, n & 1);
+  };
 #pragma unroll
-    for (int j = 0; j < J; ++j) bf[0][j] = Dec<DT>::run(c.w[2 * j], sp[j], dk);
+  for (int n = 0; n < 2 * J; ++n) dec(cs[0], 0, n);
+  auto step = [&](int kt, Codes& c, const Codes& next) {
     wait_a(kt);
     barrier();  // everyone's part of stage kt is in LDS, and nobody reads stage kt - 1 any more
     if (kt + RING - 1 < nkt) issue_a(kt + RING - 1);
     blocks(lds + (kt % RING) * SLOT, [&](int s, int j) -> const u32x4& { return bf[s][j]; },
            [&](int t) {
-             if (t < J) bf[1][t] = Dec<DT>::run(c.w[2 * t + 1], sp[t], dk);
+             if (t < 2 * J) dec(c, 1, t);
+             if (t == 2 * J) load_w(min(kt + DW, nkm - 1), c);
+             if (t >= I && t < I + 2 * J) dec(next, 0, t - I);
            });
-    if (kt + DW < nkm) load_w(kt + DW, c);
   };
   if (SH::SPLIT && wave >= 4) __builtin_amdgcn_s_setprio(1);
   for (int kt = k0; kt < nkm; kt += DW)
 #pragma unroll
     for (int u = 0; u < DW; ++u)
-      if (u < 2 || kt + u < nkm) step(kt + u, cs[u]);  // (nkm is even)
+      if (u < 2 || kt + u < nkm) step(kt + u, cs[u], cs[(u + 1) % DW]);  // (nkm is even)
   // the exact salient columns: fragments as they are
   for (int kd = 0; kd < nks; ++kd) {
     const int kt = nkm + kd;
