@@ -423,9 +423,14 @@ int sqmp_gemm_h2d(const void* a2, int ldr, const int* aexp, const void* wt, cons
 /* workspace: in it the fp32 sums of tiles whose K is split meet (no need to clear it; NULL or a
  * smaller one than asked for: no tile is split, the same values in another order of summation) */
 size_t sqmp_gemv_workspace_bytes(int dtype, int M, int N, int Kp);
-int sqmp_gemv_w4(const void* x, long ldx, const void* codes_t, const void* scale_t,
-                 const void* sal_t, const void* bias, void* y, int dtype, int M, int N, int Kp,
-                 int S_pad, int Gw, int ngw, void* workspace, size_t ws_bytes, void* stream);
+/* amap (int32 [Kp], with salient int32 [S]): x holds the columns in their own order, rows of any
+ * stride and alignment; operand position p is column amap[p] (zero where < 0) -- where
+ * sqmp_gemv_gathers says so (few rows; else SQMP_EUNSUPPORTED: sqmp_pack_rows first). */
+int sqmp_gemv_gathers(int dtype, int M, int Kp, int S_pad);
+int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const int32_t* salient, int S,
+                 const void* codes_t, const void* scale_t, const void* sal_t, const void* bias,
+                 void* y, int dtype, int M, int N, int Kp, int S_pad, int Gw, int ngw,
+                 void* workspace, size_t ws_bytes, void* stream);
 
 /* Routing (the MixtralSparseMoeBlock that fake_quant.py:564-668 quantizes).  logits D [T][E], row
  * stride ldl: per token the top_k largest (ties: the lowest index; NaN counts as the largest; -inf

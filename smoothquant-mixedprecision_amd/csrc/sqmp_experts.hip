@@ -363,19 +363,22 @@ __global__ __launch_bounds__(512, SH::OCC) void expert_tiles_kernel(const GemvAr
   run_tile<DT, GB, GATED, SH, 4>(a, act, t, lds, part_sums);
 }
 
-// The split tiles: their parts' sums added in the order of K, activation, one rounding.
-// blockIdx.y: a 16-row slice of the tile
+// The split tiles: their parts' sums added in the order of K, activation, one rounding.  blockIdx.y:
+// a 16-row slice of the tile and two of its waves' columns (small blocks: few tiles have to keep
+// every CU reading)
 template <class DT, bool GATED, class SH>
-__global__ __launch_bounds__(512) void join_kernel(const GemvArgs a, int E, int tiles_n, int act,
+__global__ __launch_bounds__(128) void join_kernel(const GemvArgs a, int E, int tiles_n, int act,
                                                    int smax, const float* part_sums) {
   typedef typename DT::T T;
   Tile t;
   if (!find_tile<SH::ROWS>(a.offsets, a.M, E, tiles_n, SH::CAP, smax, blockIdx.x, true, t)) return;
-  const int i = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i = blockIdx.y >> 2, lane = threadIdx.x & 63;
+  const int wave = (blockIdx.y & 3) * 2 + (threadIdx.x >> 6);
   const int m = 16 * i + (lane & 15), q = lane >> 4;
   if (16 * i >= t.m1 - t.m0) return;
-  const f32x4* ps = (const f32x4*)part_sums + (long)t.split * t.parts * (SH::IMAX * 1024) + i * 1024 + threadIdx.x;
+  const f32x4* ps = (const f32x4*)part_sums + (long)t.split * t.parts * (SH::IMAX * 1024) + i * 1024 + 64 * wave + lane;
   f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 4
   for (int p = 0; p < t.parts; ++p) {
     s[0] += ps[(long)p * (SH::IMAX * 1024)];
     s[1] += ps[(long)p * (SH::IMAX * 1024) + 512];
@@ -434,7 +437,7 @@ static int launch_tiles(const GemvArgs& a, int E, int slots, int act, float* ws,
   SQMP_LAUNCH_CHECK();
   if (smax > 1) {
     const long nj = tiles < SH::CAP / 2 ? tiles : SH::CAP / 2;  // two parts or more: at most cap / 2
-    join_kernel<DT, GATED, SH><<<dim3((unsigned)nj, SH::IMAX), dim3(512), 0, s>>>(a, E, tiles_n, act, smax, ws);
+    join_kernel<DT, GATED, SH><<<dim3((unsigned)nj, SH::IMAX * 4), dim3(128), 0, s>>>(a, E, tiles_n, act, smax, ws);
     SQMP_LAUNCH_CHECK();
   }
   return SQMP_OK;

@@ -15,16 +15,25 @@ namespace sqmp {
 namespace w4 {
 
 // GB: 1 = groups of whole 64-position stages, 2 = groups of 32, 0 = any multiple of 8
-// MT: 16-row token tiles per pass; NW waves; U stages in flight; ACT / EXP: the expert forms
-template <class DT, int GB, int MT, int NW, int U, bool EXP, int ACT>
+// MT: 16-row token tiles per pass; J: 16-row halves of the block per workgroup (1: two workgroups,
+// neighbours on one XCD, share the block's lines); NW waves; U stages in flight; STAGE: the rows of
+// x gathered into LDS first; ACT / EXP: the expert forms
+template <class DT, int GB, int MT, int J, int NW, int U, bool STAGE, bool EXP, int ACT>
 __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
   typedef typename DT::T T;
-  constexpr int RS = 36;  // floats per token row of a partial (32 + 4: spreads the LDS banks)
+  constexpr int SZ = sizeof(T);
+  constexpr int RS = 16 * J + 4;  // floats per token row of a partial (+ 4: spreads the LDS banks)
+  static_assert(ACT == ACT_NONE || J == 2, "gate and up rows meet in one workgroup");
   __shared__ __attribute__((aligned(16))) float red[NW * MT * 16 * RS];
+  extern __shared__ __attribute__((aligned(16))) unsigned char xs[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int r16 = lane & 15, q = lane >> 4;
-  const int nb = blockIdx.x;
+  int nb = blockIdx.x, half = 0;
+  if constexpr (J == 1) {
+    nb = ((int)blockIdx.x >> 4) * 8 + (blockIdx.x & 7), half = (blockIdx.x >> 3) & 1;
+    if (nb * 32 + half * 16 >= a.N) return;
+  }
   const int nblk = (a.N + 255) / 256 * 8;  // 32-row blocks of one weight's operands
   const int nkm = a.Kp / 64, nks = a.S_pad / 64;
   int lo = 0, hi = a.M;
@@ -34,11 +43,51 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
     hi = a.offsets[blockIdx.y + 1];
     wb += (long)blockIdx.y * nblk;
   }
-  const uint32_t* codes = a.codes + wb * nkm * 256 + lane * 4;
-  const T* scale = (const T*)a.scale + wb * a.ngw * 32 + r16 * 2;
-  const T* sal = (const T*)a.sal + wb * (nks > 0 ? nks : 1) * 2048 + lane * 32;
+  const __amdgpu_buffer_rsrc_t rW = rsrc_of(a.codes + wb * nkm * 256);
+  const __amdgpu_buffer_rsrc_t rS = rsrc_of((const T*)a.scale + wb * a.ngw * 32);
+  const T* sal = (const T*)a.sal + wb * nks * 2048 + lane * 32 + half * 16;
+  const uint32_t vw = (uint32_t)lane * 16 + half * 8, vs = (uint32_t)(r16 * 2 + half) * SZ;
   const DecK dk = make_deck();
   const int c0 = 4 * (q & 1) + (q >> 1);  // chunk of s = 0; s = 1: + 2
+
+  struct Codes {
+    uint32_t w[2 * J];               // [j][s]
+    T s[GB == 0 ? 2 * J : J];        // scales of the row halves (GB 0: for either s)
+  };
+  auto scale_at = [&](uint32_t voff, uint32_t soff, T* d) {
+    if constexpr (SZ == 2 && J == 2) {
+      const uint32_t v = load4(rS, voff, soff);
+      d[0] = __builtin_bit_cast(T, (uint16_t)v), d[1] = __builtin_bit_cast(T, (uint16_t)(v >> 16));
+    } else if constexpr (SZ == 2) {
+      d[0] = __builtin_bit_cast(T, (uint16_t)load2(rS, voff, soff));
+    } else if constexpr (J == 2) {
+      const uint64_t v = load8(rS, voff, soff);
+      d[0] = __uint_as_float((uint32_t)v), d[1] = __uint_as_float((uint32_t)(v >> 32));
+    } else {
+      d[0] = __uint_as_float(load4(rS, voff, soff));
+    }
+  };
+  auto load_w = [&](int kt, Codes& c) {
+    if constexpr (J == 2) {
+      const u32x4 v = load16(rW, vw, (uint32_t)kt * 1024);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c.w[i] = v[i];
+    } else {
+      const uint64_t v = load8(rW, vw, (uint32_t)kt * 1024);
+      c.w[0] = (uint32_t)v, c.w[1] = (uint32_t)(v >> 32);
+    }
+    if constexpr (GB == 0) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int g = min((kt * 64 + 8 * (c0 + 2 * s)) / a.Gw, a.ngw - 1);
+        scale_at(vs + (uint32_t)g * 32 * SZ, 0, c.s + J * s);
+      }
+    } else if constexpr (GB == 1) {
+      scale_at(vs, (uint32_t)group_of(kt, a) * 32 * SZ, c.s);
+    } else {
+      scale_at(vs + (uint32_t)min(2 * kt + (q & 1), a.ngw - 1) * 32 * SZ, 0, c.s);
+    }
+  };
 
   for (int m0 = lo; m0 < hi; m0 += 16 * MT) {
     // this lane's tokens (rows past the end repeat the last one; their columns of C are dropped)
@@ -50,60 +99,72 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
       if constexpr (EXP) {
         if (a.rows) xr = a.rows[m] / a.top_k;
       }
-      xp[i] = (const T*)a.x + xr * a.ldx + 8 * c0;
+      xp[i] = STAGE ? (const T*)xs + (long)(m - lo) * ((a.Kp + a.S_pad) + 16 / SZ) + 8 * c0
+                    : (const T*)a.x + xr * a.ldx + 8 * c0;
     }
-    f32x4 acc[MT][2];
+    f32x4 acc[MT][J];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < J; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     struct Stage {
-      u32x4 w;
-      T s[GB == 0 ? 4 : 2];  // scales of the two row halves (GB 0: for either s)
+      Codes c;
       Frag<DT> x[MT][2];
     };
-    auto load = [&](int kt, Stage& st) {
-      st.w = *(const u32x4*)(codes + (long)kt * 256);
-      if constexpr (GB == 0) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int g = min((kt * 64 + 8 * (c0 + 2 * s)) / a.Gw, a.ngw - 1);
-          st.s[2 * s] = scale[(long)g * 32];
-          st.s[2 * s + 1] = scale[(long)g * 32 + 1];
-        }
-      } else {
-        const int g = GB == 1 ? group_of(kt, a) : min(2 * kt + (q & 1), a.ngw - 1);
-        st.s[0] = scale[(long)g * 32];
-        st.s[1] = scale[(long)g * 32 + 1];
-      }
+    auto load_x = [&](int kt, Frag<DT> (&x)[MT][2]) {
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) st.x[i][s] = load_frag<DT>(xp[i] + (long)kt * 64 + 16 * s);
+        for (int s = 0; s < 2; ++s) x[i][s] = load_frag<DT>(xp[i] + (long)kt * 64 + 16 * s);
     };
     auto compute = [&](const Stage& st) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const Frag<DT> w = decode<DT>(st.w[2 * j + s], st.s[GB == 0 ? 2 * s + j : j], dk);
+        for (int j = 0; j < J; ++j) {
+          const Frag<DT> w = decode<DT>(st.c.w[2 * j + s], st.c.s[GB == 0 ? J * s + j : j], dk);
 #pragma unroll
           for (int i = 0; i < MT; ++i) mfma<DT>(acc[i][j], w, st.x[i][s]);
         }
     };
     int kt = wave;
-    for (; kt + (U - 1) * NW < nkm; kt += U * NW) {
-      Stage st[U];
+    Stage st[U];
+    if constexpr (STAGE) {
+      // the first codes are on their way while the rows are gathered
 #pragma unroll
-      for (int u = 0; u < U; ++u) load(kt + u * NW, st[u]);
+      for (int u = 0; u < U; ++u) load_w(min(kt + u * NW, nkm - 1), st[u].c);
+      const int L = a.Kp + a.S_pad, LP = L + 16 / SZ, M = hi - lo;
+      const T* x = (const T*)a.x;
+      for (int p = threadIdx.x; p < L; p += NW * 64) {
+        int k = -1;
+        if (p < a.Kp) k = a.amap[p];
+        else if (p - a.Kp < a.S) k = a.salient[p - a.Kp];
+        T v[16];
+#pragma unroll
+        for (int m = 0; m < 16; ++m)
+          if (m < M) v[m] = k >= 0 ? x[(long)m * a.ldx + k] : (T)0.f;
+#pragma unroll
+        for (int m = 0; m < 16; ++m)
+          if (m < M) ((T*)xs)[(long)m * LP + p] = v[m];
+      }
+      __syncthreads();
+    }
+    bool first = STAGE;
+    for (; kt + (U - 1) * NW < nkm; kt += U * NW) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!first) load_w(kt + u * NW, st[u].c);
+        load_x(kt + u * NW, st[u].x);
+      }
+      first = false;
 #pragma unroll
       for (int u = 0; u < U; ++u) compute(st[u]);
     }
     for (; kt < nkm; kt += NW) {
-      Stage st;
-      load(kt, st);
-      compute(st);
+      load_w(kt, st[0].c);
+      load_x(kt, st[0].x);
+      compute(st[0]);
     }
     // the exact salient columns: operand fragments as they are
     for (int kd = wave; kd < nks; kd += NW) {
@@ -113,7 +174,7 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) x[i] = load_frag<DT>(xp[i] + (long)(nkm + kd) * 64 + 16 * s);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < J; ++j) {
           const Frag<DT> w = load_frag<DT>(sal + (long)kd * 2048 + j * 16 + s * 8);
 #pragma unroll
           for (int i = 0; i < MT; ++i) mfma<DT>(acc[i][j], w, x[i]);
@@ -124,14 +185,14 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < J; ++j)
         *(f32x4*)(red + ((wave * MT + i) * 16 + r16) * RS + 16 * j + 4 * q) = acc[i][j];
     __syncthreads();
     const int nm = min(16 * MT, hi - m0);
-    constexpr int NO = ACT == ACT_NONE ? 32 : 16;  // outputs per token of this block
+    constexpr int NO = ACT == ACT_NONE ? 16 * J : 16;  // outputs per token of this workgroup
     for (int t = threadIdx.x; t < nm * NO; t += NW * 64) {
       const int m = t / NO, r = t % NO;
-      const int n = nb * NO + r;
+      const int n = (ACT == ACT_NONE ? nb * 32 + half * 16 : nb * 16) + r;
       float v = 0.f, u = 0.f;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
@@ -147,15 +208,43 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
   }
 }
 
+// LDS a call may use for gathered rows (with the partial sums, up to 36 KiB at 16 waves and 32 rows,
+// below 64 KiB)
+constexpr long STAGE_BYTES = 27 * 1024;
+static long stage_bytes(int dtype, int M, int Kp, int S_pad) {
+  return (long)M * ((Kp + S_pad) * (dtype == SQMP_F32 ? 4 : 2) + 16);
+}
+
 template <class DT, int GB, bool EXP, int ACT>
 static int launch(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
   const int nb = cdiv(a.N, 32);
-  const dim3 grid(nb, EXP ? E : 1);
-#define SQMP_GV(MT, NW, U) \
-  gemv_kernel<DT, GB, MT, NW, U, EXP, ACT><<<grid, dim3(NW * 64), 0, s>>>(a)
-  if (max_rows <= 16) SQMP_GV(1, 8, 4);
-  else if (max_rows <= 32) SQMP_GV(2, 8, 2);
-  else SQMP_GV(4, 8, 1);
+  const size_t xb = a.amap ? (size_t)stage_bytes(DT::id, a.M, a.Kp, a.S_pad) : 0;
+#define SQMP_GV(MT, J, NW, U, ST)                                                                  \
+  gemv_kernel<DT, GB, MT, J, NW, U, ST, EXP, ACT>                                                  \
+      <<<dim3((J) == 1 ? cdiv(nb, 8) * 16 : nb, EXP ? E : 1), dim3((NW) * 64), xb, s>>>(a)
+  if (max_rows <= 16) {
+    // Waves per workgroup, and whether a block's halves go to two workgroups, by how many blocks
+    // there are for the 256 CUs.  8 waves / 16 waves / 16 waves and halves, one row, one box: 32
+    // blocks of K 4096 5.3 / 4.7 / 4.3 us, 128 of K 4096 5.8 / 5.1 / 4.6, of K 11008 11.6 / 10.4 / 9.5,
+    // 256 of K 2048 (fp32) 9.0 / 8.2 / 10.2, 344 of K 4096 9.3 / 9.4 / 11.7, 1000 16.9 / 19.4 / 32.0
+    if constexpr (EXP) {
+      // (many experts' blocks: 4 waves, 8 experts x 688 blocks of K 4096 61 us against 74 with 8)
+      if ((long)nb * E >= 2048) SQMP_GV(1, 2, 4, 4, false);
+      else SQMP_GV(1, 2, 8, 4, false);
+    } else {
+      if (nb <= 192) {
+        if (a.amap) SQMP_GV(1, 1, 16, 4, true); else SQMP_GV(1, 1, 16, 4, false);
+      } else if (nb <= 320) {
+        if (a.amap) SQMP_GV(1, 2, 16, 4, true); else SQMP_GV(1, 2, 16, 4, false);
+      } else {
+        if (a.amap) SQMP_GV(1, 2, 8, 4, true); else SQMP_GV(1, 2, 8, 4, false);
+      }
+    }
+  } else if (max_rows <= 32) {
+    SQMP_GV(2, 2, 8, 2, false);
+  } else {
+    SQMP_GV(4, 2, 8, 1, false);
+  }
 #undef SQMP_GV
   SQMP_LAUNCH_CHECK();
   return SQMP_OK;
@@ -170,10 +259,11 @@ static int by_group(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
 }
 
 static int check_operand(const void* x, long ldx, int dtype, int N, int Kp, int S_pad, int Gw,
-                         int ngw) {
+                         int ngw, bool gathered = false) {
   if (N <= 0 || Kp <= 0 || Kp % 128 || S_pad < 0 || S_pad % 64 || Gw <= 0 || ngw <= 0)
     return SQMP_EINVAL;
   if (dtype != SQMP_F32 && dtype != SQMP_F16 && dtype != SQMP_BF16) return SQMP_EUNSUPPORTED;
+  if (gathered) return ldx > 0 ? SQMP_OK : SQMP_EINVAL;
   const long per16 = dtype == SQMP_F32 ? 4 : 8;  // whole 16-byte loads of x
   if (ldx < (long)Kp + S_pad || ldx % per16 || (size_t)x % 16) return SQMP_EINVAL;
   return SQMP_OK;
@@ -192,19 +282,28 @@ extern "C" size_t sqmp_expert_workspace_bytes(int dtype, int E, int slots, int N
   return w4::expert_tiles_workspace(E, slots, N, Kp);
 }
 
-extern "C" int sqmp_gemv_w4(const void* x, long ldx, const void* codes_t, const void* scale_t,
+// whether sqmp_gemv_w4 gathers these rows itself (amap)
+extern "C" int sqmp_gemv_gathers(int dtype, int M, int Kp, int S_pad) {
+  return M <= 16 && w4::stage_bytes(dtype, M, Kp, S_pad) <= w4::STAGE_BYTES;
+}
+
+extern "C" int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const int32_t* salient,
+                            int S, const void* codes_t, const void* scale_t,
                             const void* sal_t, const void* bias, void* y, int dtype, int M, int N,
                             int Kp, int S_pad, int Gw, int ngw, void* workspace, size_t ws_bytes,
                             void* stream) {
   SQMP_DEVICE_GUARD(stream);
   if (!x || !codes_t || !scale_t || !y || (S_pad > 0 && !sal_t)) return SQMP_EINVAL;
   if (M < 0 || M > SQMP_GEMV_MAX_ROWS) return SQMP_EINVAL;
-  const int st = w4::check_operand(x, ldx, dtype, N, Kp, S_pad, Gw, ngw);
+  if (S < 0 || S > S_pad || (S > 0 && amap && !salient)) return SQMP_EINVAL;
+  const int st = w4::check_operand(x, ldx, dtype, N, Kp, S_pad, Gw, ngw, amap != nullptr);
   if (st != SQMP_OK) return st;
+  if (amap && !sqmp_gemv_gathers(dtype, M, Kp, S_pad)) return SQMP_EUNSUPPORTED;
   if (M == 0) return SQMP_OK;
   w4::GemvArgs a{};
   a.x = x, a.ldx = ldx, a.codes = (const uint32_t*)codes_t, a.scale = scale_t, a.sal = sal_t;
   a.bias = bias, a.y = y, a.M = M, a.N = N, a.n_out = N;
+  a.amap = amap, a.salient = salient, a.S = S;
   a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
   w4::set_groups(a);
   hipStream_t s = (hipStream_t)stream;

@@ -300,14 +300,38 @@ __global__ __launch_bounds__(256) void scan_kernel(int32_t* hist, int blocks, in
   if (tid == 0) hist[(long)E * blocks + e] = run;
 }
 
-// ranks in slots -> slots, and rows
+// ranks in slots -> slots, and rows.  SCANNED: hist holds the scan of scan_kernel; else (few
+// blocks) every block adds up the counts of the blocks before it by itself
+constexpr int SELF_SCAN_BLOCKS = 512;
+template <bool SCANNED>
 __global__ __launch_bounds__(NT) void place_kernel(const Args a) {
-  __shared__ int32_t tmp[E_MAX], start[E_MAX];
+  __shared__ int32_t tmp[E_MAX], start[E_MAX], count[E_MAX];
   const int e = threadIdx.x;
+  if constexpr (!SCANNED) {
+    int g = 64;  // threads per expert: a power of two within a wave
+    while (g * a.E > NT) g >>= 1;
+    const int ex = threadIdx.x / g, c = threadIdx.x % g;
+    int before = 0, all = 0;
+    if (ex < a.E)
+      for (int b = c; b < a.blocks; b += g) {
+        const int v = a.hist[(long)ex * a.blocks + b];
+        all += v;
+        before += b < (int)blockIdx.x ? v : 0;
+      }
+    for (int d = 1; d < g; d <<= 1) {
+      all += __shfl_xor(all, d, 64);
+      before += __shfl_xor(before, d, 64);
+    }
+    if (ex < a.E && c == 0) count[ex] = all, start[ex] = before;
+    __syncthreads();
+  } else if (e < a.E) {
+    count[e] = a.hist[(long)a.E * a.blocks + e];
+    start[e] = a.hist[(long)e * a.blocks + blockIdx.x];
+  }
   int total = 0;
-  const int at = scan_experts(e < a.E ? a.hist[(long)a.E * a.blocks + e] : 0, tmp, &total);
+  const int at = scan_experts(e < a.E ? count[e] : 0, tmp, &total);
   if (e < a.E) {
-    start[e] = at + a.hist[(long)e * a.blocks + blockIdx.x];
+    start[e] += at;
     if (blockIdx.x == 0) a.offsets[e] = at;
   }
   if (blockIdx.x == 0 && e == 0) a.offsets[a.E] = total;
@@ -335,9 +359,14 @@ static int launch(const Args& a, hipStream_t s) {
   }
   route_kernel<DT, KT, false><<<dim3(a.blocks), dim3(NT), 0, s>>>(a);
   SQMP_LAUNCH_CHECK();
+  if (a.blocks <= SELF_SCAN_BLOCKS) {
+    place_kernel<false><<<dim3(a.blocks), dim3(NT), 0, s>>>(a);
+    SQMP_LAUNCH_CHECK();
+    return SQMP_OK;
+  }
   scan_kernel<<<dim3(a.E), dim3(256), 0, s>>>(a.hist, a.blocks, a.E);
   SQMP_LAUNCH_CHECK();
-  place_kernel<<<dim3(a.blocks), dim3(NT), 0, s>>>(a);
+  place_kernel<true><<<dim3(a.blocks), dim3(NT), 0, s>>>(a);
   SQMP_LAUNCH_CHECK();
   return SQMP_OK;
 }

@@ -16,6 +16,10 @@ struct GemvArgs {
   void* y;                // D [M][N_out]
   int M, N;               // rows (dense form); weight rows (gated: gate and up rows together)
   int Kp, S_pad, Gw, ngw;
+  // x in an order of its own (STAGE): operand position p is column amap[p] (< 0: zero), position
+  // Kp + j the column salient[j], j < S
+  const int32_t *amap, *salient;
+  int S;
   // expert form
   const int32_t* rows;     // slot -> flat (token * top_k + j), or NULL: x row = slot
   const int32_t* offsets;  // [E + 1]

@@ -96,8 +96,9 @@ SIGNATURES = {
     "sqmp_pack_h2d": (_i, [_vp, _i, _i, _vp, _vp]),
     "sqmp_gemm_h2d": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp]),
     "sqmp_gemv_workspace_bytes": (_sz, [_i, _i, _i, _i]),
-    "sqmp_gemv_w4": (_i, [_vp, _l, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _sz,
-                          _vp]),
+    "sqmp_gemv_gathers": (_i, [_i, _i, _i, _i]),
+    "sqmp_gemv_w4": (_i, [_vp, _l, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
+                          _i, _vp, _sz, _vp]),
     "sqmp_expert_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "sqmp_route_workspace_bytes": (_sz, [_i, _i]),
     "sqmp_route": (_i, [_vp, _l, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

@@ -220,7 +220,7 @@ def _operand(x: torch.Tensor, pe: PackedExperts, r: Routing, by_slot: bool):
     rows = None if by_slot else r.rows
     if pe.identity and ops._operand_rows(x, pe.Kp):
         return x, rows
-    if x.stride(1) != 1:
+    if x.stride(1) != 1 or x.stride(0) == 0:  # (0: rows of an expanded tensor)
         x = x.contiguous()
     L = pe.Kp + pe.S_pad
     own = pe.amap.dim() == 2

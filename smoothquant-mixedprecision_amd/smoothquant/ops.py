@@ -1087,7 +1087,7 @@ def pack_rows(x2: torch.Tensor, amap: torch.Tensor, Kp: int, salient: Optional[t
               S: int, S_pad: int) -> torch.Tensor:
     """x [M, K] -> [M, Kp + S_pad]: the unquantized activation operand (columns gathered by amap,
     then the salient columns)."""
-    if x2.stride(1) != 1:
+    if x2.stride(1) != 1 or x2.stride(0) == 0:  # (0: rows of an expanded tensor)
         x2 = x2.contiguous()
     out = torch.empty((x2.shape[0], Kp + S_pad), dtype=x2.dtype, device=x2.device)
     check(load().sqmp_pack_rows(_p(x2), max(x2.stride(0), 1), _dtype_code(x2.dtype), x2.shape[0],
@@ -1103,7 +1103,8 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
 
     x: [M, K] in the columns' order -- a 4-bit weight with D activations -- or, with `packed`,
     the [M, Kp + S_pad] operand of quant_act_fp.  Any strides; rows that are not 16-B aligned,
-    and packed weights in an order of their own, are copied first (sqmp_pack_rows)."""
+    and those of weights packed in an order of their own, are gathered by the kernel where they
+    are few, else copied first (sqmp_pack_rows)."""
     if not x.is_cuda:
         _require_gpu(x, "gemv")
     a = pw.gemv_args or _gemv_args(pw)
@@ -1130,23 +1131,27 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
     y = x.new_empty((M, N))
     if M == 0:
         return y
+    lib = load()
     ld, s1 = x.stride()
     xp = x.data_ptr()
-    if not (packed or ident):
-        x = pack_rows(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
-        xp, ld = x.data_ptr(), L
-    elif M == 1 and s1 == 1 and xp % 16 == 0:
-        ld = L
-    elif s1 != 1 or xp % 16 or ld < L or ld % per:
+    amap = sal = None
+    if (packed or ident) and s1 == 1 and xp % 16 == 0 and (M == 1 or (ld >= L and ld % per == 0)):
+        if M == 1:
+            ld = L
+    elif packed:
         x = x.clone(memory_format=torch.contiguous_format)
         xp, ld = x.data_ptr(), L
-    lib = load()
+    elif s1 == 1 and ld > 0 and lib.sqmp_gemv_gathers(code, M, pw.Kp, pw.S_pad):
+        amap, sal = pw.amap.data_ptr(), None if pw.salient is None else pw.salient.data_ptr()
+    else:
+        x = pack_rows(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
+        xp, ld = x.data_ptr(), L
     ws, wn = None, 0
     if M > 16:
         wn = lib.sqmp_gemv_workspace_bytes(code, M, N, pw.Kp)
         if wn:
             ws = torch.empty(wn, dtype=torch.uint8, device=device)
-    status = lib.sqmp_gemv_w4(xp, ld, codes_t, scale_t, sal_t, bp, y.data_ptr(), code, M, N, *tail,
+    status = lib.sqmp_gemv_w4(xp, ld, amap, sal, pw.S, codes_t, scale_t, sal_t, bp, y.data_ptr(), code, M, N, *tail,
                               None if ws is None else ws.data_ptr(), wn, _raw_stream(device.index))
     if status:
         check(status, "gemv")

@@ -16,9 +16,9 @@ def lib():
 
 
 def test_gemv_refusals(lib):
-    def call(x=P, ldx=128, codes=P, scale=P, sal=None, bias=None, y=P, dtype=1, M=1, N=32, Kp=128, S_pad=0,
-             Gw=64, ngw=2):
-        return lib.sqmp_gemv_w4(x, ldx, codes, scale, sal, bias, y, dtype, M, N, Kp, S_pad, Gw, ngw, None, 0, None)
+    def call(x=P, ldx=128, amap=None, salient=None, S=0, codes=P, scale=P, sal=None, bias=None, y=P, dtype=1,
+             M=1, N=32, Kp=128, S_pad=0, Gw=64, ngw=2):
+        return lib.sqmp_gemv_w4(x, ldx, amap, salient, S, codes, scale, sal, bias, y, dtype, M, N, Kp, S_pad, Gw, ngw, None, 0, None)
     assert call(M=0) == 0                                   # nothing to do
     for bad in (dict(x=None), dict(codes=None), dict(scale=None), dict(y=None), dict(S_pad=64, ldx=192),
                 dict(M=-1), dict(M=65), dict(N=0), dict(Kp=64), dict(Kp=100), dict(S_pad=-64),
@@ -28,6 +28,12 @@ def test_gemv_refusals(lib):
     assert call(dtype=3) == -2
     assert call(Gw=12) == -2                                # groups of whole 8 positions only
     assert call(dtype=0, ldx=130) == -1
+    assert call(S=1, amap=P, S_pad=64, sal=P) == -1 and call(S=65, S_pad=64, sal=P, ldx=192) == -1
+    assert call(amap=P, ldx=0) == -1
+    # rows gathered by the kernel: few enough for its LDS
+    assert lib.sqmp_gemv_gathers(1, 1, 12800, 0) == 1 and lib.sqmp_gemv_gathers(1, 1, 16384, 0) == 0
+    assert lib.sqmp_gemv_gathers(1, 17, 128, 0) == 0
+    assert lib.sqmp_gemv_gathers(1, 16, 4096, 0) == 0 and call(amap=P, M=16, Kp=4096, ngw=64) == -2
 
 
 def test_expert_linear_refusals(lib):

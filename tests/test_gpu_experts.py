@@ -87,11 +87,10 @@ def test_route_special_values():
     check_routing(r, r.ids.cpu(), 4)
 
 
-@pytest.mark.parametrize("T", [70001])
-def test_route_many_blocks(T):
-    """More blocks than a scan has threads would need 65536 tokens: the scan's second level."""
+@pytest.mark.parametrize("T,E,k", [(70001, 17, 4), (131072 + 300, 64, 2), (5000, 1, 1), (3000, 256, 3)])
+def test_route_many_blocks(T, E, k):
+    """Up to 512 blocks of 256 tokens add up the counts before them themselves, more take a scan."""
     g = gen(3)
-    E, k = 17, 4
     logits = torch.randn(T, E, generator=g, device="cuda").to(torch.bfloat16)
     logits[torch.rand(T, generator=g, device="cuda") < 0.3] = -INF
     r = experts.route(logits, k)
@@ -296,6 +295,8 @@ def test_products_strides_empty_and_refusals():
     odd[:, 1:] = x
     assert torch.equal(experts.expert_linear(odd[:, 1:], pe, r), want)
     assert torch.equal(experts.expert_linear(x.t().contiguous().t(), pe, r), want)
+    one = x[2:3].expand(6, 128)
+    assert torch.equal(experts.expert_linear(one, pe, r), experts.expert_linear(one.contiguous(), pe, r))
     nothing = experts.plan_routes(torch.full((6, 2), -1, device="cuda"), torch.ones(6, 2, device="cuda"), 3)
     out = torch.full((12, 48), 3.0, device="cuda", dtype=D)
     assert (experts.expert_linear(x, pe, nothing, out=out) == 3.0).all()
