@@ -15,7 +15,7 @@
 // the value's order and the index (so every compare-exchange is a max and a min, and ties go to
 // the lower index), and two merges over the lanes leave the k largest of all.  The order of the
 // pairs is a counting sort: a block of 256 tokens ranks its pairs 64 at a time by ballots, an
-// exclusive scan over the blocks places them.  No atomics: slots depend on the ids alone.
+// exclusive scan over the blocks places them: slots depend on the ids alone.
 #include "sqmp_common.h"
 
 namespace sqmp {
@@ -27,6 +27,7 @@ constexpr int NWAVE = NT / 64;
 constexpr int E_MAX = 256, K_MAX = 16;
 constexpr int MAX_CHUNKS = TB * K_MAX / 64;       // 64-pair chunks of a block
 constexpr int PER_WAVE = MAX_CHUNKS / NWAVE;      // of a wave
+constexpr int PITCH = MAX_CHUNKS + 4;             // of an expert's chunk counts (8-byte rows)
 
 // Keys whose unsigned order is the order of (value, lower index first): NaN highest, -0 as +0.
 // 16-bit types: value and index in 32 bits; fp32: in 64.  (index 0xFFFF / ~0: none)
@@ -55,12 +56,11 @@ template <> struct Key<F32> {
 };
 template <class DT, uint32_t INF> struct Key16 {
   typedef uint32_t K;
-  static constexpr K NEG_INF = (K)(0x7FFFu - INF) << 16;  // ~(0x8000 | INF)
   typedef typename DT::T T;
-  __device__ static inline K make(float v, int e) {
-    const T t = DT::from_f(v);  // (the value came from D: exact)
-    uint32_t u = (uint32_t)__builtin_bit_cast(uint16_t, t);
-    if (v != v) u = 0x7FFFu;
+  static constexpr K NEG_INF = (K)(0x7FFFu - INF) << 16;  // ~(0x8000 | INF)
+  __device__ static inline K make(T v, int e) {
+    uint32_t u = (uint32_t)__builtin_bit_cast(uint16_t, v);
+    if ((u & 0x7FFFu) > INF) u = 0x7FFFu;
     if (u == 0x8000u) u = 0u;
     u = (u & 0x8000u) ? (~u & 0xFFFFu) : (u | 0x8000u);
     return (u << 16) | (uint32_t)(0xFFFF - e);
@@ -116,7 +116,7 @@ struct Args {
   float* weights;
   int32_t* ids;
   int32_t *offsets, *rows, *slots;
-  int32_t* hist;       // [E][blocks], then [E] totals
+  int32_t* hist;       // [blocks][E], then [E] totals
   int blocks;
 };
 
@@ -130,10 +130,10 @@ __device__ inline void each_logit(const typename DT::T* row, int E, int c, bool 
       struct __attribute__((aligned(16))) P { T v[V]; };
       const P x = *(const P*)(row + p * V);
 #pragma unroll
-      for (int i = 0; i < V; ++i) f(DT::to_f(x.v[i]), p * V + i);
+      for (int i = 0; i < V; ++i) f(x.v[i], p * V + i);
     }
   } else {
-    for (int e = c; e < E; e += 4) f(DT::to_f(row[e]), e);
+    for (int e = c; e < E; e += 4) f(row[e], e);
   }
 }
 
@@ -151,33 +151,47 @@ __device__ inline void choose(const Args& a, int t0, int nt, uint16_t* lid) {
   K list[KT];
 #pragma unroll
   for (int j = 0; j < KT; ++j) list[j] = 0;
-  each_logit<DT>(row, a.E, c, vec, [&](float v, int e) { insert<K, KT>(list, KY::make(v, e)); });
+  each_logit<DT>(row, a.E, c, vec, [&](T v, int e) { insert<K, KT>(list, KY::make(v, e)); });
   merge<DT, KT>(list, 1);
   merge<DT, KT>(list, 2);
+  // lane c finishes the choices j = c, c + 4, ...
+  constexpr int PER = (KT + 3) / 4;
   const float top = KY::value(list[0]);
-  float ex[KT], den = 0.f;
+  K own[PER];
+  float ex[PER], den = 0.f;
 #pragma unroll
-  for (int j = 0; j < KT; ++j) {
-    ex[j] = j < a.k && KY::chosen(list[j]) ? expf(KY::value(list[j]) - top) : 0.f;
-    den += ex[j];
+  for (int i = 0; i < PER; ++i) {
+    own[i] = list[4 * i];
+#pragma unroll
+    for (int x = 1; x < 4; ++x)
+      if (4 * i + x < KT && c == x) own[i] = list[4 * i + x];
+    const bool sel = 4 * i + c < a.k && 4 * i + c < KT && KY::chosen(own[i]);
+    ex[i] = sel ? expf(KY::value(own[i]) - top) : 0.f;
+    den += ex[i];
   }
   if (!a.normalize) {
+    // (exp2 of a rounded product: off by |d| 2^-24 of a term exp(d), d <= 0, at most 0.4 steps of
+    // the sum, which is at least 1)
     den = 0.f;
-    each_logit<DT>(row, a.E, c, vec, [&](float v, int) { den += expf(v - top); });
-    den += __shfl_xor(den, 1, 64);
-    den += __shfl_xor(den, 2, 64);
+    each_logit<DT>(row, a.E, c, vec, [&](T v, int) {
+      den += __builtin_amdgcn_exp2f((DT::to_f(v) - top) * 1.44269504f);
+    });
   }
+  den += __shfl_xor(den, 1, 64);
+  den += __shfl_xor(den, 2, 64);
   if (tok < nt) {
 #pragma unroll
-    for (int j = 0; j < KT; ++j)
-      if (j < a.k && (j & 3) == c) {
-        const bool sel = KY::chosen(list[j]);
-        const int id = sel ? KY::index(list[j]) : -1;
+    for (int i = 0; i < PER; ++i) {
+      const int j = 4 * i + c;
+      if (j < a.k) {
+        const bool sel = KY::chosen(own[i]);
+        const int id = sel ? KY::index(own[i]) : -1;
         const long f = (long)t * a.k + j;
-        a.weights[f] = sel ? ex[j] / den : 0.f;
+        a.weights[f] = sel ? ex[i] / den : 0.f;
         a.ids[f] = id;
         lid[tok * a.k + j] = (uint16_t)(sel ? id : a.E);
       }
+    }
   }
 }
 
@@ -210,7 +224,7 @@ __device__ inline int scan_experts(int v, int32_t* tmp, int* total) {
 // same expert.  ONE (the only block): the slots themselves; else the ranks, left in slots
 template <class DT, int KT, bool ONE>
 __global__ __launch_bounds__(NT) void route_kernel(const Args a) {
-  __shared__ uint16_t cnt[MAX_CHUNKS * E_MAX];
+  __shared__ __attribute__((aligned(8))) uint16_t cnt[PITCH * E_MAX];  // [expert][chunk]
   __shared__ uint16_t lid[TB * K_MAX];
   __shared__ int32_t tmp[E_MAX], start[E_MAX];
   const int t0 = blockIdx.x * TB, nt = min(TB, a.T - t0);
@@ -224,7 +238,9 @@ __global__ __launch_bounds__(NT) void route_kernel(const Args a) {
       lid[i] = (uint16_t)(e < 0 || e >= a.E ? a.E : e);
     }
   }
-  for (int i = threadIdx.x; i < chunks * a.E; i += NT) cnt[i] = 0;
+  const int quads = (chunks + 3) / 4;
+  for (int i = threadIdx.x; i < quads * a.E; i += NT)
+    *(uint64_t*)(cnt + (i / quads) * PITCH + (i % quads) * 4) = 0;
   __syncthreads();
   // pairs of each expert in every chunk, and a pair's rank inside its chunk
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -238,17 +254,23 @@ __global__ __launch_bounds__(NT) void route_kernel(const Args a) {
       my_e[i] = f < np ? lid[f] : a.E;
       const uint64_t m = same_expert(my_e[i], nbits);
       my_r[i] = (int)__popcll(m & ((1ull << lane) - 1));
-      if (my_e[i] < a.E && my_r[i] == 0) cnt[c * a.E + my_e[i]] = (uint16_t)__popcll(m);
+      if (my_e[i] < a.E && my_r[i] == 0) cnt[my_e[i] * PITCH + c] = (uint16_t)__popcll(m);
     }
   }
   __syncthreads();
-  // cnt -> pairs of the expert in earlier chunks; the block's count
+  // cnt -> pairs of the expert in earlier chunks, four chunks at a time; the block's count
   int s = 0;
   if ((int)threadIdx.x < a.E) {
-    for (int c = 0; c < chunks; ++c) {
-      const int v = cnt[c * a.E + threadIdx.x];
-      cnt[c * a.E + threadIdx.x] = (uint16_t)s;
-      s += v;
+    uint64_t* row = (uint64_t*)(cnt + threadIdx.x * PITCH);
+    for (int c = 0; c < quads; ++c) {
+      const uint64_t v = row[c];
+      uint64_t o = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o |= (uint64_t)(uint16_t)s << (16 * i);
+        s += (int)((v >> (16 * i)) & 0xFFFFu);
+      }
+      row[c] = o;
     }
   }
   int total = 0;
@@ -257,14 +279,14 @@ __global__ __launch_bounds__(NT) void route_kernel(const Args a) {
     if ((int)threadIdx.x < a.E) start[threadIdx.x] = at, a.offsets[threadIdx.x] = at;
     if (threadIdx.x == 0) a.offsets[a.E] = total;
   } else {
-    if ((int)threadIdx.x < a.E) a.hist[(long)threadIdx.x * a.blocks + blockIdx.x] = s;
+    if ((int)threadIdx.x < a.E) a.hist[(long)blockIdx.x * a.E + threadIdx.x] = s;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < PER_WAVE; ++i) {
     const int c = wave + i * NWAVE, f = c * 64 + lane, e = my_e[i];
     if (c < chunks && f < np) {
-      int slot = e < a.E ? cnt[c * a.E + e] + my_r[i] : -1;
+      int slot = e < a.E ? cnt[e * PITCH + c] + my_r[i] : -1;
       if constexpr (ONE) {
         if (e < a.E) {
           slot += start[e];
@@ -277,14 +299,14 @@ __global__ __launch_bounds__(NT) void route_kernel(const Args a) {
   }
 }
 
-// hist[e][blk] -> exclusive scan over the blocks, the expert's total behind
+// hist[blk][e] -> exclusive scan over the blocks, the expert's total behind
 __global__ __launch_bounds__(256) void scan_kernel(int32_t* hist, int blocks, int E) {
   __shared__ int32_t part[256];
   const int e = blockIdx.x, tid = threadIdx.x;
-  int32_t* h = hist + (long)e * blocks;
+  int32_t* h = hist + e;
   int run = 0;
   for (int b0 = 0; b0 < blocks; b0 += 256) {
-    const int v = b0 + tid < blocks ? h[b0 + tid] : 0;
+    const int v = b0 + tid < blocks ? h[(long)(b0 + tid) * E] : 0;
     part[tid] = v;
     __syncthreads();
     for (int d = 1; d < 256; d <<= 1) {
@@ -293,7 +315,7 @@ __global__ __launch_bounds__(256) void scan_kernel(int32_t* hist, int blocks, in
       part[tid] += add;
       __syncthreads();
     }
-    if (b0 + tid < blocks) h[b0 + tid] = run + part[tid] - v;
+    if (b0 + tid < blocks) h[(long)(b0 + tid) * E] = run + part[tid] - v;
     run += part[255];
     __syncthreads();
   }
@@ -308,25 +330,32 @@ __global__ __launch_bounds__(NT) void place_kernel(const Args a) {
   __shared__ int32_t tmp[E_MAX], start[E_MAX], count[E_MAX];
   const int e = threadIdx.x;
   if constexpr (!SCANNED) {
-    int g = 64;  // threads per expert: a power of two within a wave
-    while (g * a.E > NT) g >>= 1;
-    const int ex = threadIdx.x / g, c = threadIdx.x % g;
+    // thread (group c, expert ex): every groups-th block, 8 loads in flight; summed in LDS
+    const int groups = NT / a.E, ex = e % a.E, c = e / a.E;
+    if (e < a.E) count[e] = start[e] = 0;
+    __syncthreads();
     int before = 0, all = 0;
-    if (ex < a.E)
-      for (int b = c; b < a.blocks; b += g) {
-        const int v = a.hist[(long)ex * a.blocks + b];
-        all += v;
-        before += b < (int)blockIdx.x ? v : 0;
+    if (c < groups) {
+      for (int b0 = c; b0 < a.blocks; b0 += 8 * groups) {
+        int v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int b = b0 + i * groups;
+          v[i] = b < a.blocks ? a.hist[(long)b * a.E + ex] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          all += v[i];
+          before += b0 + i * groups < (int)blockIdx.x ? v[i] : 0;
+        }
       }
-    for (int d = 1; d < g; d <<= 1) {
-      all += __shfl_xor(all, d, 64);
-      before += __shfl_xor(before, d, 64);
+      atomicAdd(&count[ex], all);   // (LDS; whole numbers: the order does not matter)
+      atomicAdd(&start[ex], before);
     }
-    if (ex < a.E && c == 0) count[ex] = all, start[ex] = before;
     __syncthreads();
   } else if (e < a.E) {
     count[e] = a.hist[(long)a.E * a.blocks + e];
-    start[e] = a.hist[(long)e * a.blocks + blockIdx.x];
+    start[e] = a.hist[(long)blockIdx.x * a.E + e];
   }
   int total = 0;
   const int at = scan_experts(e < a.E ? count[e] : 0, tmp, &total);
