@@ -191,11 +191,20 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
       for (int i = 0; i < NA; ++i)
         dma16(rA, a_off[o][i], (uint32_t)kt * 128, slot + o * 4096 + i * 8192);
   };
-  // stage kt's activations of this wave are in LDS: at most the RING - 2 later stages' LDS-DMA
-  // (the youngest operations; codes loads among them only make it wait for more) are in flight
-  auto wait_a = [&](int kt) {
-    if (!loads) return;
-    if (nkt - 1 - kt >= RING - 2) vmwait<(RING - 2) * NO * NA>(); else vmwait<0>();
+  // One barrier per BPS stages (short stages: two).  Before it this wave's part of those stages has
+  // to be in LDS -- at most the LDS-DMA of the stages behind them (the youngest operations; codes
+  // loads among them only make it wait for more) is in flight; after it everyone's part is, and
+  // nobody reads the BPS stages before any more, whose ring places the next loads take.
+  constexpr int BPS = I == 4 && SH::OCC == 4 ? 2 : 1, FLY = RING - 2 * BPS;
+  auto enter = [&](int kt) {
+    if (BPS == 2 && ((kt - k0) & 1)) return;
+    if (loads) {
+      if (nkt - BPS - kt >= FLY) vmwait<FLY * NO * NA>(); else vmwait<0>();
+    }
+    barrier();
+#pragma unroll
+    for (int b = 0; b < BPS; ++b)
+      if (kt + RING - BPS + b < nkt) issue_a(kt + RING - BPS + b);
   };
 
   // weights
@@ -246,8 +255,8 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
   // which makes it wait for LDS-DMA issued in between as well: codes are loaded far ahead.)
   Codes cs[DW];
 #pragma unroll
-  for (int p = 0; p < (RING - 1 > DW ? RING - 1 : DW); ++p) {
-    if (p < RING - 1 && k0 + p < nkt) issue_a(k0 + p);
+  for (int p = 0; p < (RING - BPS > DW ? RING - BPS : DW); ++p) {
+    if (p < RING - BPS && k0 + p < nkt) issue_a(k0 + p);
     if (p < DW) load_w(min(k0 + p, nkm - 1), cs[p]);
   }
   u32x4 bf[2][J];
@@ -258,9 +267,7 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
 #pragma unroll
   for (int n = 0; n < 2 * J; ++n) dec(cs[0], 0, n);
   auto step = [&](int kt, Codes& c, const Codes& next) {
-    wait_a(kt);
-    barrier();  // everyone's part of stage kt is in LDS, and nobody reads stage kt - 1 any more
-    if (kt + RING - 1 < nkt) issue_a(kt + RING - 1);
+    enter(kt);
     blocks(lds + (kt % RING) * SLOT, [&](int s, int j) -> const u32x4& { return bf[s][j]; },
            [&](int t) {
              if (t < 2 * J) dec(c, 1, t);
@@ -282,9 +289,7 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int j = 0; j < J; ++j) d[s][j] = *(const u32x4*)(sal + j * 16 + s * 8);
-    wait_a(kt);
-    barrier();
-    if (kt + RING - 1 < nkt) issue_a(kt + RING - 1);
+    enter(kt);
     blocks(lds + (kt % RING) * SLOT, [&](int s, int j) -> const u32x4& { return d[s][j]; },
            [](int) {});
   }
