@@ -48,13 +48,13 @@ class Routing:
         return self.ids.shape[1]
 
 
-def _plan_buffers(T: int, k: int, E: int, dev):
-    """(offsets, rows, slots, workspace pointer and size), one allocation for the first three."""
-    n = load().sqmp_route_workspace_bytes(T, E)
+def _plan_buffers(T: int, k: int, E: int, dev, n_ids: int):
+    """(ids, rows, slots, offsets, workspace, its size): the first four, int32, from one
+    allocation in this order."""
+    n = load().sqmp_route_workspace_bytes(T, E) if T > 256 else 0
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    rows, slots, offsets = torch.empty(2 * T * k + E + 1, dtype=torch.int32,
-                                       device=dev).split((T * k, T * k, E + 1))
-    return offsets, rows, slots, ws, n
+    buf = torch.empty(n_ids + 2 * T * k + E + 1, dtype=torch.int32, device=dev)
+    return (*buf.split_with_sizes((n_ids, T * k, T * k, E + 1)), ws, n)
 
 
 def _ptr(t):
@@ -73,7 +73,8 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
     largest, -inf is never chosen) with their softmax weights -- over the chosen ones, or
     over all E with normalize=False -- and the plan of plan_routes.  A token whose logits are all
     -inf (padding) goes to no expert."""
-    ops._require_gpu(logits, "route")
+    if not logits.is_cuda:
+        ops._require_gpu(logits, "route")
     if logits.dim() != 2:
         raise ValueError(f"route: logits must be [tokens, experts], got {tuple(logits.shape)}")
     T, E = logits.shape
@@ -81,17 +82,21 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
     if top_k > E:
         raise ValueError(f"route: top_k {top_k} of {E} experts")
     dt = ops._dtype_code(logits.dtype)
-    if logits.stride(1) != 1 or logits.stride(0) < E:
+    ld, s1 = logits.stride()
+    if s1 != 1 or ld < E:
         logits = logits.contiguous()
+        ld = E
     dev = logits.device
-    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
     weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-    offsets, rows, slots, ws, n = _plan_buffers(T, top_k, E, dev)
-    check(load().sqmp_route(logits.data_ptr(), max(logits.stride(0), E), dt, T, E, top_k,
-                            int(normalize), weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(),
-                            rows.data_ptr(), slots.data_ptr(), _ptr(ws), n,
-                            ops._raw_stream(dev.index)), "route")
-    return Routing(ids, weights, offsets, rows, slots, E)
+    ids, rows, slots, offsets, wp, n = _plan_buffers(T, top_k, E, dev, T * top_k)
+    op = offsets.data_ptr()
+    tk = 4 * T * top_k  # bytes of each of the three lists before it
+    status = load().sqmp_route(logits.data_ptr(), ld, dt, T, E, top_k, int(normalize),
+                               weights.data_ptr(), op - 3 * tk, op, op - 2 * tk, op - tk,
+                               _ptr(wp), n, ops._raw_stream(dev.index))
+    if status:
+        check(status, "route")
+    return Routing(ids.view(T, top_k), weights, offsets, rows, slots, E)
 
 
 def plan_routes(ids: torch.Tensor, weights: torch.Tensor, num_experts: int) -> Routing:
@@ -110,7 +115,7 @@ def plan_routes(ids: torch.Tensor, weights: torch.Tensor, num_experts: int) -> R
     if ids.dtype != torch.int32:
         ids = (ids.long().clamp(-1, num_experts)).to(torch.int32)  # (no id may wrap into range)
     ids = ids.contiguous()
-    offsets, rows, slots, ws, n = _plan_buffers(T, k, num_experts, ids.device)
+    _, rows, slots, offsets, ws, n = _plan_buffers(T, k, num_experts, ids.device, 0)
     check(load().sqmp_plan_routes(ids.data_ptr(), T, num_experts, k, offsets.data_ptr(),
                                   rows.data_ptr(), slots.data_ptr(), _ptr(ws), n,
                                   ops._raw_stream(ids.device.index)), "plan_routes")
@@ -141,12 +146,13 @@ class PackedExperts:
 
 
 def _interleave(t: torch.Tensor) -> torch.Tensor:
-    """[2 I, ...] (gate rows, then up rows) -> 16 gate and 16 up rows in turn, I padded to 16."""
-    inter = t.shape[0] // 2
-    pad = (inter + 15) // 16 * 16
-    full = t.new_zeros((2, pad) + t.shape[1:])
-    full[0, :inter], full[1, :inter] = t[:inter], t[inter:]
-    return full.view((2, pad // 16, 16) + t.shape[1:]).transpose(0, 1).reshape((2 * pad,) + t.shape[1:])
+    """[E, 2 I, X] (gate rows, then up rows) -> 16 gate and 16 up rows in turn, I padded to 16."""
+    E, rows, X = t.shape
+    inter, pad = rows // 2, (rows // 2 + 15) // 16 * 16
+    halves = t.reshape(E, 2, inter, X)
+    if pad != inter:
+        halves = torch.nn.functional.pad(halves, (0, 0, 0, pad - inter))
+    return halves.view(E, 2, pad // 16, 16, X).transpose(1, 2).reshape(E, 2 * pad, X)
 
 
 def _pack_all(weights, E: int, rows: int, gated: bool) -> PackedExperts:
@@ -195,7 +201,8 @@ def pack_experts(w: torch.Tensor, weight_quant: str = "per_channel", group_size:
     _check_stack("pack_experts", w, gated)
     if weight_quant == "none":
         raise ValueError("pack_experts: needs a quantized weight")
-    it = (ops.pack_weight(_interleave(w[e]) if gated else w[e], weight_quant, 4, group_size, salient)
+    it = (ops.pack_weight(_interleave(w[e:e + 1])[0] if gated else w[e], weight_quant, 4, group_size,
+                          salient)
           for e in range(w.shape[0]))
     return _pack_all(it, w.shape[0], w.shape[1], gated)
 
@@ -207,10 +214,23 @@ def pack_expert_codes(codes: torch.Tensor, scales: torch.Tensor, group_size: int
     if scales.dim() != 3 or scales.shape[:2] != codes.shape[:2]:
         raise ValueError(f"pack_expert_codes: scales {tuple(scales.shape)} do not match codes "
                          f"{tuple(codes.shape)}")
-    pick = _interleave if gated else (lambda t: t)
-    it = (ops.pack_codes(pick(codes[e]), pick(scales[e]), group_size)
-          for e in range(codes.shape[0]))
-    return _pack_all(it, codes.shape[0], codes.shape[1], gated)
+    n_rows = codes.shape[1]
+    if gated:
+        codes, scales = _interleave(codes), _interleave(scales)
+    # one weight whose rows are the experts', each padded to the operands' 256
+    E, N, K = codes.shape
+    pad = (N + 255) // 256 * 256
+    if pad != N:
+        codes = torch.nn.functional.pad(codes, (0, 0, 0, pad - N))
+        scales = torch.nn.functional.pad(scales, (0, 0, 0, pad - N))
+    pw = ops.pack_codes(codes.reshape(E * pad, K), scales.reshape(E * pad, -1), group_size)
+    if not ops.gemv_eligible(pw):
+        raise ValueError("pack_expert_codes: needs groups of a multiple of 8 columns, got "
+                         f"{group_size}")
+    one = ops.tile_major(pw.codes, pw.wscale, pw.wsal, E * pad, pw.Kp, 0, pw.ngw, pw.dtype)
+    return PackedExperts(one[0].view(E, -1), one[1].view(E, -1), None, pw.amap, None, E,
+                         n_rows // 2 if gated else n_rows, N, K, pw.Kp, 0, 0, pw.Gw, pw.ngw,
+                         pw.dtype, gated, pw.Kp == K)
 
 
 # ------------------------------------------------------------------ products
@@ -285,25 +305,32 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
 def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y [tokens, H]: y[t] = D(sum_j weights[t, j] * z[slot of pair (t, j)]), fp32 sums in the
     order of j; a token that goes nowhere gets zeros."""
-    ops._require_gpu(z, "combine")
-    T, k = routing.tokens, routing.top_k
+    if not z.is_cuda:
+        ops._require_gpu(z, "combine")
+    T, k = routing.ids.shape
     if z.dim() != 2 or z.shape[0] != T * k or z.shape[1] == 0:
         raise ValueError(f"combine: z must be [{T * k}, H], got {tuple(z.shape)}")
-    dt = ops._dtype_code(z.dtype)
-    if routing.slots.device != z.device:
-        raise RuntimeError(f"combine: z on {z.device}, routing on {routing.slots.device}")
-    z = z.contiguous()
+    dt = ops.DTYPE_CODE.get(z.dtype)
+    if dt is None:
+        ops._dtype_code(z.dtype)
+    dev = z.device
+    if routing.slots.device != dev:
+        raise RuntimeError(f"combine: z on {dev}, routing on {routing.slots.device}")
+    if not z.is_contiguous():
+        z = z.contiguous()
     H = z.shape[1]
     if out is None:
-        out = torch.empty((T, H), dtype=z.dtype, device=z.device)
-    elif (tuple(out.shape) != (T, H) or out.dtype != z.dtype or out.device != z.device
+        out = z.new_empty((T, H))
+    elif (tuple(out.shape) != (T, H) or out.dtype != z.dtype or out.device != dev
           or not out.is_contiguous()):
-        raise ValueError(f"combine: out must be contiguous {z.dtype} [{T}, {H}] on {z.device}")
+        raise ValueError(f"combine: out must be contiguous {z.dtype} [{T}, {H}] on {dev}")
     if T == 0:
         return out
-    check(load().sqmp_combine(z.data_ptr(), dt, T, k, H, routing.slots.data_ptr(),
-                              routing.weights.data_ptr(), out.data_ptr(),
-                              ops._raw_stream(z.device.index)), "combine")
+    status = load().sqmp_combine(z.data_ptr(), dt, T, k, H, routing.slots.data_ptr(),
+                                 routing.weights.data_ptr(), out.data_ptr(),
+                                 ops._raw_stream(dev.index))
+    if status:
+        check(status, "combine")
     return out
 
 

@@ -1107,26 +1107,22 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
     are few, else copied first (sqmp_pack_rows)."""
     if not x.is_cuda:
         _require_gpu(x, "gemv")
-    a = pw.gemv_args or _gemv_args(pw)
-    dtype, device, code, L, per, ident, codes_t, scale_t, sal_t, N, tail = a
-    shape = x.shape
-    if len(shape) != 2:
-        raise ValueError(f"gemv: x must have 2 dimensions, got {tuple(shape)}")
-    M = shape[0]
-    if shape[1] != (L if packed else pw.K):
-        raise ValueError(f"gemv: x has {shape[1]} columns, the weight {L if packed else pw.K}")
+    dtype, device, code, L, K, per, ident, codes_t, scale_t, sal_t, N, tail = (
+        pw.gemv_args or _gemv_args(pw))
+    if x.dim() != 2 or x.dtype is not dtype or x.device != device:
+        _gemv_refuse(x, dtype, device)
+    M, C = x.shape
+    if C != (L if packed else K):
+        raise ValueError(f"gemv: x has {C} columns, the weight {L if packed else K}")
     if M > GEMV_MAX_ROWS:
         raise ValueError(f"gemv: {M} rows, at most {GEMV_MAX_ROWS}")
-    if x.dtype != dtype:
-        raise RuntimeError(f"expected input dtype {dtype}, got {x.dtype}")
-    if x.device != device:
-        raise RuntimeError(f"gemv: x on {x.device}, the weight on {device}")
     bp = None
     if bias is not None:
-        if bias.dtype != dtype or bias.device != device or bias.numel() != N:
+        if bias.dtype is not dtype or bias.device != device or bias.numel() != N:
             raise RuntimeError(f"gemv: bias {bias.dtype} [{bias.numel()}] on {bias.device} does "
                                f"not match {dtype} [{N}] on {device}")
-        bias = bias.reshape(-1).contiguous()
+        if bias.dim() != 1 or not bias.is_contiguous():
+            bias = bias.reshape(-1).contiguous()
         bp = bias.data_ptr()
     y = x.new_empty((M, N))
     if M == 0:
@@ -1146,16 +1142,25 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
     else:
         x = pack_rows(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
         xp, ld = x.data_ptr(), L
-    ws, wn = None, 0
+    wp, wn = None, 0
     if M > 16:
         wn = lib.sqmp_gemv_workspace_bytes(code, M, N, pw.Kp)
         if wn:
             ws = torch.empty(wn, dtype=torch.uint8, device=device)
-    status = lib.sqmp_gemv_w4(xp, ld, amap, sal, pw.S, codes_t, scale_t, sal_t, bp, y.data_ptr(), code, M, N, *tail,
-                              None if ws is None else ws.data_ptr(), wn, _raw_stream(device.index))
+            wp = ws.data_ptr()
+    status = lib.sqmp_gemv_w4(xp, ld, amap, sal, pw.S, codes_t, scale_t, sal_t, bp, y.data_ptr(),
+                              code, M, N, *tail, wp, wn, _raw_stream(device.index))
     if status:
         check(status, "gemv")
     return y
+
+
+def _gemv_refuse(x: torch.Tensor, dtype: torch.dtype, device: torch.device):
+    if x.dim() != 2:
+        raise ValueError(f"gemv: x must have 2 dimensions, got {tuple(x.shape)}")
+    if x.dtype is not dtype:
+        raise RuntimeError(f"expected input dtype {dtype}, got {x.dtype}")
+    raise RuntimeError(f"gemv: x on {x.device}, the weight on {device}")
 
 
 def _gemv_args(pw: PackedWeight):
@@ -1167,13 +1172,13 @@ def _gemv_args(pw: PackedWeight):
     t = gemv_operands(pw)
     ident = identity_layout(pw)
     dev = pw.codes.device
-    a = (pw.dtype, dev, _dtype_code(pw.dtype), pw.Kp + pw.S_pad,
+    a = (pw.dtype, dev, _dtype_code(pw.dtype), pw.Kp + pw.S_pad, pw.K,
          4 if pw.dtype == torch.float32 else 8, ident, t[0].data_ptr(), t[1].data_ptr(),
          t[2].data_ptr() if pw.S_pad else None, pw.N, (pw.Kp, pw.S_pad, pw.Gw, pw.ngw))
     if pw.gemv is t and pw.ident is not None:
         pw.gemv_args = a
     else:
-        a = a[:6] + (_Keep(t, a[6]), _Keep(t, a[7]), None if a[8] is None else _Keep(t, a[8])) + a[9:]
+        a = a[:7] + (_Keep(t, a[7]), _Keep(t, a[8]), None if a[9] is None else _Keep(t, a[9])) + a[10:]
     return a
 
 

@@ -94,7 +94,7 @@ def test_bpack_layout():
 
 
 def test_interleaved_halves():
-    t = torch.arange(40).view(40, 1)
+    t = torch.arange(40).view(1, 40, 1)
     rows = experts._interleave(t).view(2, 2, 16)             # 20 + 20 rows, padded to 32 + 32
     assert rows[0, 0].tolist() == list(range(16)) and rows[0, 1].tolist() == list(range(20, 36))
     assert rows[1, 0, :4].tolist() == [16, 17, 18, 19] and rows[1, 1, :4].tolist() == [36, 37, 38, 39]
