@@ -68,6 +68,7 @@ def _check_sizes(what: str, E: int, k: int):
         raise ValueError(f"{what}: top_k {k}, supported are 1 .. {MAX_TOP_K}")
 
 
+@ops.on_tensor_device
 def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
     """The top_k largest logits of every token [T, E] (ties: the lowest index; NaN counts as the
     largest, -inf is never chosen) with their softmax weights -- over the chosen ones, or
@@ -99,6 +100,7 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
     return Routing(ids.view(T, top_k), weights, offsets, rows, slots, E)
 
 
+@ops.on_tensor_device
 def plan_routes(ids: torch.Tensor, weights: torch.Tensor, num_experts: int) -> Routing:
     """The plan for a routing chosen elsewhere: ids [T, top_k] (any integer type; a value outside
     0 .. num_experts - 1 means that nothing was chosen), weights [T, top_k].  The pairs of an expert
@@ -193,6 +195,7 @@ def _check_stack(what: str, w: torch.Tensor, gated: bool):
         raise ValueError(f"{what}: a gated weight has an even number of rows, got {w.shape[1]}")
 
 
+@ops.on_tensor_device
 def pack_experts(w: torch.Tensor, weight_quant: str = "per_channel", group_size: int = 128,
                  salient: Optional[torch.Tensor] = None, gated: bool = False) -> PackedExperts:
     """Quantize w D [E, N, K] to 4 bits expert by expert (ops.pack_weight).  gated: the rows are
@@ -207,6 +210,7 @@ def pack_experts(w: torch.Tensor, weight_quant: str = "per_channel", group_size:
     return _pack_all(it, w.shape[0], w.shape[1], gated)
 
 
+@ops.on_tensor_device
 def pack_expert_codes(codes: torch.Tensor, scales: torch.Tensor, group_size: int,
                       gated: bool = False) -> PackedExperts:
     """As ops.pack_codes for codes int8 [E, N, K] and scales D [E, N, ceil(K / group_size)]."""
@@ -254,6 +258,7 @@ def _operand(x: torch.Tensor, pe: PackedExperts, r: Routing, by_slot: bool):
     return out, None if own else rows
 
 
+@ops.on_tensor_device
 def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Optional[str] = None,
                   rows: str = "token", out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """z [tokens * top_k, n_out], rows in expert order: D(W_e x) for every (token, expert) pair, or
@@ -302,6 +307,7 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
     return out
 
 
+@ops.on_tensor_device
 def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y [tokens, H]: y[t] = D(sum_j weights[t, j] * z[slot of pair (t, j)]), fp32 sums in the
     order of j; a token that goes nowhere gets zeros."""

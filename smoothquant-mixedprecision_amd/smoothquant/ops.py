@@ -6,6 +6,7 @@ raises if a tensor is not on a ROCm device: the W4A4 operator has no CPU path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import weakref
 from dataclasses import dataclass, field
@@ -43,6 +44,20 @@ def _stream(t: torch.Tensor):
 # against 0.1 us, a fifth of a few-row call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+# A device's default stream has the null handle, which names no device: the few-row and expert
+# calls make their tensors' device current first where it is not
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def on_tensor_device(fn):
+    """fn(tensor, ...) with the tensor's device current."""
+    @functools.wraps(fn)
+    def call(t, *args, **kw):
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != _current_device():
+            with torch.cuda.device(t.device):
+                return fn(t, *args, **kw)
+        return fn(t, *args, **kw)
+    return call
 
 
 def _require_gpu(t: torch.Tensor, what: str):
@@ -998,6 +1013,7 @@ def bpack_codes(codes: torch.Tensor) -> torch.Tensor:
     return w.view(R, Kp // 8).view(torch.uint8)
 
 
+@on_tensor_device
 def pack_codes(codes: torch.Tensor, scales: torch.Tensor, group_size: int) -> PackedWeight:
     """A PackedWeight from 4-bit codes that exist already (a checkpoint quantized elsewhere):
     codes int8 [N, K] in -8 .. 7, scales D [N, ceil(K / group_size)], W = D(code * scale) with
@@ -1033,6 +1049,7 @@ def pack_codes(codes: torch.Tensor, scales: torch.Tensor, group_size: int) -> Pa
     return pw
 
 
+@on_tensor_device
 def tile_major(codes: torch.Tensor, wscale: torch.Tensor, wsal: torch.Tensor, N: int, Kp: int,
                S_pad: int, ngw: int, dtype: torch.dtype, out=None):
     """sqmp_pack_fq7 (J = 2) of a packed 4-bit weight: (codes_t, scale_t, sal_t), into `out`
@@ -1083,6 +1100,7 @@ def _operand_rows(x2: torch.Tensor, width: int):
             and (x2.shape[0] == 1 or (x2.stride(0) >= width and x2.stride(0) % per == 0)))
 
 
+@on_tensor_device
 def pack_rows(x2: torch.Tensor, amap: torch.Tensor, Kp: int, salient: Optional[torch.Tensor],
               S: int, S_pad: int) -> torch.Tensor:
     """x [M, K] -> [M, Kp + S_pad]: the unquantized activation operand (columns gathered by amap,
@@ -1096,6 +1114,7 @@ def pack_rows(x2: torch.Tensor, amap: torch.Tensor, Kp: int, salient: Optional[t
     return out
 
 
+@on_tensor_device
 def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
          packed: bool = False) -> torch.Tensor:
     """y [M, N] = D(x . W_hat^T + bias) for M <= GEMV_MAX_ROWS rows (the decoding form of

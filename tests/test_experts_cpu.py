@@ -143,3 +143,34 @@ def test_module_state_roundtrip(tmp_path):
             assert torch.equal(fresh.state_dict()[k], v)
     with pytest.raises(RuntimeError, match="cast"):
         fresh.float()
+
+
+def test_calls_make_their_tensors_device_current(monkeypatch):
+    """A device's default stream is the null handle: the calls enter their tensor's device when it is
+    not the current one (shown with a stand-in for a tensor on the second device)."""
+    class OnDevice1(torch.Tensor):
+        is_cuda = True
+        device = torch.device("cuda", 1)
+
+    entered = []
+
+    class Ctx:
+        def __init__(self, dev):
+            entered.append(dev)
+
+        def __enter__(self):
+            monkeypatch.setattr(ops, "_current_device", lambda: 1)
+
+        def __exit__(self, *exc):
+            monkeypatch.setattr(ops, "_current_device", lambda: 0)
+            return False
+
+    monkeypatch.setattr(ops, "_current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Ctx)
+    t = torch.zeros(2, 8).as_subclass(OnDevice1)
+    seen = ops.on_tensor_device(lambda x, y: (ops._current_device(), y))(t, 5)
+    assert seen == (1, 5) and entered == [torch.device("cuda", 1)] and ops._current_device() == 0
+    assert ops.on_tensor_device(lambda x: ops._current_device())(torch.zeros(1)) == 0
+    for fn in (ops.pack_codes, ops.tile_major, ops.pack_rows, ops.gemv, experts.route, experts.plan_routes,
+               experts.pack_experts, experts.pack_expert_codes, experts.expert_linear, experts.combine):
+        assert fn.__wrapped__ is not None
