@@ -2,19 +2,26 @@
 // segments offsets[e] .. offsets[e + 1], W_e = D(code * scale) (+ exact salient columns), or
 // D( act(gate) * up ) for weights whose rows are 16 gate and 16 up rows in turn.
 //
-// What bounds it: the MFMA (2 slots N K flops), with the LDS reads of the activation tile close
-// behind.  A workgroup of 8 waves computes up to 256 slots of one expert by 256 weight rows:
+// What bounds it: the MFMA (2 slots N K flops) from some 100 rows per expert on, the decoding of the
+// codes (13 VALU per 8 in fp16, 20 in bf16) and their bytes below.  A workgroup of 8 waves computes
+// up to 128 or 256 slots of one expert by 256 weight rows:
 //   * each wave owns 32 weight rows; their codes and scales go straight from the tile-major
-//     operands to registers, two stages ahead, and are decoded there -- a decoded fragment feeds
-//     all the tile's tokens, and no weight passes through LDS;
-//   * the activation rows go to a three-slot LDS ring by LDS-DMA, gathered by the slot -> row
-//     list as they are loaded, so the tokens are never copied into expert order;
-//   * the last tile of an expert runs 64, 128 or 192 rows (TM), so a ragged segment wastes less
-//     than 64 rows of MFMA;
+//     operands to registers, stages ahead, and are decoded there between the MFMAs -- a decoded
+//     fragment feeds all the tile's tokens, and no weight passes through LDS;
+//   * the activation rows go to an LDS ring by LDS-DMA, gathered by the slot -> row list as they
+//     are loaded, so the tokens are never copied into expert order;
+//   * the last tile of an expert runs 64 rows (of 256: 64, 128 or 192), so a ragged segment wastes
+//     less than 64 rows of MFMA;
 //   * gate and up rows of one output are the two accumulators of one lane: the activation and the
-//     product happen in registers, half the output bytes, no second launch.
+//     product happen in registers, half the output bytes, no second launch;
+//   * the tiles of the last, partial round of workgroups are split along K (join_kernel).
 // The grid holds every tile that any split of `slots` over the experts can need; the tiles that
 // exist are found from the offsets on the GPU (no host synchronisation), the rest return.
+// Measured: 16384 x 4096 x 4096 as one expert 423 us (1300 TFLOP/s, 256-row tiles; a library product of
+// 8192^3 reaches 1200 on that card), 2 of 8 experts x 2048 tokens, 4096 -> 2 x 11008 gated 675 us
+// (1094 TFLOP/s; 616 us at the library's rate), 11008 -> 4096 355 us (1040; 308 us); 509 tokens x 6 of
+// 64, 2048 -> 1408 gated bf16 95 + 13 us of join (40 us of bytes at the rate of a large copy): there the
+// vector pipe decodes for 41 % and the MFMA runs for 27 % of the time.
 #include "sqmp_w4_launch.h"
 
 namespace sqmp {
@@ -403,7 +410,7 @@ __global__ __launch_bounds__(128) void join_kernel(const GemvArgs a, int E, int 
   }
 }
 
-// The tile height, by the mean rows of an expert (128 / 256 rows, one box, 2 of 8 experts, 4096 ->
+// The tile height, by the mean rows of an expert (128 / 256 rows, one card, 2 of 8 experts, 4096 ->
 // 2 x 11008 gated unless said): 128 rows each 275 / 367 us, 512: 701 / 705, 1024: 1297 / 1349 (11008
 // -> 4096: 678 / 743), 2048 of 4096 -> 4096: 470 / 449.  SQMP_EXPERT_ROWS overrides (A/B)
 static int tile_rows(int E, int slots) {

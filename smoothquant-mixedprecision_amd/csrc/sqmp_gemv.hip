@@ -3,12 +3,20 @@
 // of a mixture (ragged rows).  W = D(code * scale) at the Kp coded positions, then the S_pad
 // exact salient columns.
 //
-// What bounds it: the weight bytes (N Kp / 2 codes + scales), read once.  So a wave streams
-// whole 1-KiB stages of the tile-major codes straight into registers, decodes them there and
-// feeds the MFMA with the tokens in the B slot -- up to 16 tokens cost what one does.  A
-// workgroup owns one block of 32 weight rows and its NW waves take the K stages round robin
-// (consecutive stages are consecutive memory), each with U stages of loads in flight; the NW
-// partial sums meet in LDS and are added in a fixed order, so results do not depend on timing.
+// What bounds it: the weight bytes (N Kp / 2 codes + scales), read once; for single weights of a few
+// MB the latency of one trip to HBM.  So a wave streams whole 1-KiB stages of the tile-major codes
+// straight into registers, decodes them there and feeds the MFMA with the tokens in the B slot: the
+// matrix work of 16 tokens is that of one.  A workgroup owns one block of 32 weight rows (or, where
+// blocks are few, its halves go to two workgroups on one XCD, which share the lines) and its NW
+// waves take the K stages round robin (consecutive stages are consecutive memory), U stages of loads
+// in flight each; the NW partial sums meet in LDS and are added in a fixed order, so results do not
+// depend on timing.  x comes as 16-byte fragments from L2, or, where its rows are unaligned or the
+// weight has an order of its own, gathered into LDS while the first codes are on their way.
+// Measured in a captured graph: 1 x 4096 x 4096 fp16 4.5 us (8.7 MB: 1.9 TB/s, 1.7 us at the rate of a
+// large copy; latency), 8 x 11008 x 4096 bf16 10.3 us (2.3 TB/s; decoding, and 344 blocks on 256
+// CUs), 1 x 32000 x 4096 16.8 us (4.0 TB/s), 8 experts of 2 rows, 22016 x 4096: 63 us (5.3 TB/s).
+// From 17 rows on (fp16 / bf16, groups of 32 or of whole stages) the product runs on the expert
+// tiles, K split over workgroups: 64 x 4096 x 11008 43 us here, 23 us there.
 #include "sqmp_w4_launch.h"
 
 namespace sqmp {
@@ -17,14 +25,19 @@ namespace w4 {
 // GB: 1 = groups of whole 64-position stages, 2 = groups of 32, 0 = any multiple of 8
 // MT: 16-row token tiles per pass; J: 16-row halves of the block per workgroup (1: two workgroups,
 // neighbours on one XCD, share the block's lines); NW waves; U stages in flight; STAGE: the rows of
-// x gathered into LDS first; ACT / EXP: the expert forms
-template <class DT, int GB, int MT, int J, int NW, int U, bool STAGE, bool EXP, int ACT>
+// x gathered into LDS first; NX > 0 (16-bit types, MT 1): a stage's rows come as 8 NX whole 128-byte
+// lines and are turned into fragments in a wave's own corner of LDS (fragments straight from L2
+// touch every line four times); ACT / EXP: the expert forms
+template <class DT, int GB, int MT, int J, int NW, int U, bool STAGE, int NX, bool EXP, int ACT>
 __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
   typedef typename DT::T T;
   constexpr int SZ = sizeof(T);
   constexpr int RS = 16 * J + 4;  // floats per token row of a partial (+ 4: spreads the LDS banks)
   static_assert(ACT == ACT_NONE || J == 2, "gate and up rows meet in one workgroup");
   __shared__ __attribute__((aligned(16))) float red[NW * MT * 16 * RS];
+  static_assert(NX == 0 || (MT == 1 && SZ == 2 && !STAGE && !EXP), "whole lines: 16-bit rows of one weight");
+  constexpr int XP = 144;         // bytes of a row of the corner (128 + 16: spreads the banks)
+  __shared__ __attribute__((aligned(16))) unsigned char turn[NX > 0 ? NW * 2 * 16 * XP : 16];
   extern __shared__ __attribute__((aligned(16))) unsigned char xs[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -111,14 +124,38 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
     struct Stage {
       Codes c;
       Frag<DT> x[MT][2];
+      u32x4 line[NX > 0 ? NX : 1];
     };
-    auto load_x = [&](int kt, Frag<DT> (&x)[MT][2]) {
+    const T* lp[NX > 0 ? NX : 1];  // this lane's pieces of the lines: row 8 i + lane / 8
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < NX; ++i)
+      lp[i] = (const T*)a.x + (long)min(m0 + 8 * i + (lane >> 3), hi - 1) * a.ldx + 8 * (lane & 7);
+    auto load_x = [&](int kt, Stage& st) {
+      if constexpr (NX > 0) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) x[i][s] = load_frag<DT>(xp[i] + (long)kt * 64 + 16 * s);
+        for (int i = 0; i < NX; ++i) st.line[i] = *(const u32x4*)(lp[i] + (long)kt * 64);
+      } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) st.x[i][s] = load_frag<DT>(xp[i] + (long)kt * 64 + 16 * s);
+      }
     };
-    auto compute = [&](const Stage& st) {
+    auto compute = [&](Stage& st, int u) {
+      if constexpr (NX > 0) {
+        // (the LDS operations of one wave run in order: the reads see the writes, and the next
+        // writes to this half come after these reads)
+        unsigned char* t = turn + (wave * 2 + (u & 1)) * 16 * XP;
+#pragma unroll
+        for (int i = 0; i < NX; ++i)
+          *(u32x4*)(t + (8 * i + (lane >> 3)) * XP + (lane & 7) * 16) = st.line[i];
+        asm volatile("" ::: "memory");
+        const int r = NX == 1 ? r16 & 7 : r16;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          st.x[0][s] = load_frag<DT>((const T*)(t + r * XP + (c0 + 2 * s) * 16));
+        asm volatile("" ::: "memory");
+      }
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -155,16 +192,16 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (!first) load_w(kt + u * NW, st[u].c);
-        load_x(kt + u * NW, st[u].x);
+        load_x(kt + u * NW, st[u]);
       }
       first = false;
 #pragma unroll
-      for (int u = 0; u < U; ++u) compute(st[u]);
+      for (int u = 0; u < U; ++u) compute(st[u], u);
     }
     for (; kt < nkm; kt += NW) {
       load_w(kt, st[0].c);
-      load_x(kt, st[0].x);
-      compute(st[0]);
+      load_x(kt, st[0]);
+      compute(st[0], 0);
     }
     // the exact salient columns: operand fragments as they are
     for (int kd = wave; kd < nks; kd += NW) {
@@ -219,31 +256,33 @@ template <class DT, int GB, bool EXP, int ACT>
 static int launch(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
   const int nb = cdiv(a.N, 32);
   const size_t xb = a.amap ? (size_t)stage_bytes(DT::id, a.M, a.Kp, a.S_pad) : 0;
-#define SQMP_GV(MT, J, NW, U, ST)                                                                  \
-  gemv_kernel<DT, GB, MT, J, NW, U, ST, EXP, ACT>                                                  \
+#define SQMP_GV(MT, J, NW, U, ST, NX)                                                                  \
+  gemv_kernel<DT, GB, MT, J, NW, U, ST, NX, EXP, ACT>                                                  \
       <<<dim3((J) == 1 ? cdiv(nb, 8) * 16 : nb, EXP ? E : 1), dim3((NW) * 64), xb, s>>>(a)
   if (max_rows <= 16) {
     // Waves per workgroup, and whether a block's halves go to two workgroups, by how many blocks
-    // there are for the 256 CUs.  8 waves / 16 waves / 16 waves and halves, one row, one box: 32
+    // there are for the 256 CUs.  8 waves / 16 waves / 16 waves and halves, one row, one card: 32
     // blocks of K 4096 5.3 / 4.7 / 4.3 us, 128 of K 4096 5.8 / 5.1 / 4.6, of K 11008 11.6 / 10.4 / 9.5,
     // 256 of K 2048 (fp32) 9.0 / 8.2 / 10.2, 344 of K 4096 9.3 / 9.4 / 11.7, 1000 16.9 / 19.4 / 32.0
     if constexpr (EXP) {
       // (many experts' blocks: 4 waves, 8 experts x 688 blocks of K 4096 61 us against 74 with 8)
-      if ((long)nb * E >= 2048) SQMP_GV(1, 2, 4, 4, false);
-      else SQMP_GV(1, 2, 8, 4, false);
+      if ((long)nb * E >= 2048) SQMP_GV(1, 2, 4, 4, false, 0);
+      else SQMP_GV(1, 2, 8, 4, false, 0);
     } else {
-      if (nb <= 192) {
-        if (a.amap) SQMP_GV(1, 1, 16, 4, true); else SQMP_GV(1, 1, 16, 4, false);
-      } else if (nb <= 320) {
-        if (a.amap) SQMP_GV(1, 2, 16, 4, true); else SQMP_GV(1, 2, 16, 4, false);
-      } else {
-        if (a.amap) SQMP_GV(1, 2, 8, 4, true); else SQMP_GV(1, 2, 8, 4, false);
-      }
+#define SQMP_GVX(J, NW)                                                                            \
+  if (a.amap) SQMP_GV(1, J, NW, 4, true, 0);                                                       \
+  else if (DT::id == SQMP_F32 || a.M <= 4) SQMP_GV(1, J, NW, 4, false, 0);                         \
+  else if (a.M <= 8) SQMP_GV(1, J, NW, 4, false, (DT::id == SQMP_F32 ? 0 : 1));                    \
+  else SQMP_GV(1, J, NW, 4, false, (DT::id == SQMP_F32 ? 0 : 2))
+      if (nb <= 192) { SQMP_GVX(1, 16); }
+      else if (nb <= 320) { SQMP_GVX(2, 16); }
+      else { SQMP_GVX(2, 8); }
+#undef SQMP_GVX
     }
   } else if (max_rows <= 32) {
-    SQMP_GV(2, 2, 8, 2, false);
+    SQMP_GV(2, 2, 8, 2, false, 0);
   } else {
-    SQMP_GV(4, 2, 8, 1, false);
+    SQMP_GV(4, 2, 8, 1, false, 0);
   }
 #undef SQMP_GV
   SQMP_LAUNCH_CHECK();
