@@ -35,7 +35,8 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
   constexpr int RS = 16 * J + 4;  // floats per token row of a partial (+ 4: spreads the LDS banks)
   static_assert(ACT == ACT_NONE || J == 2, "gate and up rows meet in one workgroup");
   __shared__ __attribute__((aligned(16))) float red[NW * MT * 16 * RS];
-  static_assert(NX == 0 || (MT == 1 && SZ == 2 && !STAGE && !EXP), "whole lines: 16-bit rows of one weight");
+  static_assert(NX == 0 || (MT == 1 && SZ == 2 && !STAGE), "whole lines: 16-bit rows");
+  constexpr int PASS = NX == 1 ? 8 : 16 * MT;  // tokens per pass over the weights
   constexpr int XP = 144;         // bytes of a row of the corner (128 + 16: spreads the banks)
   __shared__ __attribute__((aligned(16))) unsigned char turn[NX > 0 ? NW * 2 * 16 * XP : 16];
   extern __shared__ __attribute__((aligned(16))) unsigned char xs[];
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
     }
   };
 
-  for (int m0 = lo; m0 < hi; m0 += 16 * MT) {
+  for (int m0 = lo; m0 < hi; m0 += PASS) {
     // this lane's tokens (rows past the end repeat the last one; their columns of C are dropped)
     const T* xp[MT];
 #pragma unroll
@@ -126,10 +127,18 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
       Frag<DT> x[MT][2];
       u32x4 line[NX > 0 ? NX : 1];
     };
-    const T* lp[NX > 0 ? NX : 1];  // this lane's pieces of the lines: row 8 i + lane / 8
+    // this lane's pieces of the lines: row 8 i + lane / 8 (loads of rows past the end left out by
+    // predicates cost more than they save: 4.8 us instead of 4.4 at 1 x 4096 x 4096)
+    const T* lp[NX > 0 ? NX : 1];
 #pragma unroll
-    for (int i = 0; i < NX; ++i)
-      lp[i] = (const T*)a.x + (long)min(m0 + 8 * i + (lane >> 3), hi - 1) * a.ldx + 8 * (lane & 7);
+    for (int i = 0; i < NX; ++i) {
+      const int m = min(m0 + 8 * i + (lane >> 3), hi - 1);
+      long xr = m;
+      if constexpr (EXP) {
+        if (a.rows) xr = a.rows[m] / a.top_k;
+      }
+      lp[i] = (const T*)a.x + xr * a.ldx + 8 * (lane & 7);
+    }
     auto load_x = [&](int kt, Stage& st) {
       if constexpr (NX > 0) {
 #pragma unroll
@@ -225,7 +234,7 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
       for (int j = 0; j < J; ++j)
         *(f32x4*)(red + ((wave * MT + i) * 16 + r16) * RS + 16 * j + 4 * q) = acc[i][j];
     __syncthreads();
-    const int nm = min(16 * MT, hi - m0);
+    const int nm = min(PASS, hi - m0);
     constexpr int NO = ACT == ACT_NONE ? 16 * J : 16;  // outputs per token of this workgroup
     for (int t = threadIdx.x; t < nm * NO; t += NW * 64) {
       const int m = t / NO, r = t % NO;
@@ -261,20 +270,24 @@ static int launch(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
       <<<dim3((J) == 1 ? cdiv(nb, 8) * 16 : nb, EXP ? E : 1), dim3((NW) * 64), xb, s>>>(a)
   if (max_rows <= 16) {
     // Waves per workgroup, and whether a block's halves go to two workgroups, by how many blocks
-    // there are for the 256 CUs.  8 waves / 16 waves / 16 waves and halves, one row, one card: 32
-    // blocks of K 4096 5.3 / 4.7 / 4.3 us, 128 of K 4096 5.8 / 5.1 / 4.6, of K 11008 11.6 / 10.4 / 9.5,
-    // 256 of K 2048 (fp32) 9.0 / 8.2 / 10.2, 344 of K 4096 9.3 / 9.4 / 11.7, 1000 16.9 / 19.4 / 32.0
+    // there are for the 256 CUs.  8 waves / 16 waves / 8 waves and halves / 16 and halves, one row, one
+    // card: 32 blocks of K 4096 4.9 / 4.7 / 4.1 / 4.1 us, 128 of K 4096 5.2 / 4.9 / 4.4 / 4.4, of K 11008
+    // 10.1 / 9.4 / 7.9 / 8.4, 256 of K 2048 (fp32) 8.5 / 8.1 / 8.6 / 10.1, 344 of K 4096 8.1 / 9.2 / 8.8
+    // / 10.6, 1000 of K 4096 19.7 / 21.6 / 20.8 / 28.8
+    constexpr int N1 = DT::id == SQMP_F32 ? 0 : 1, N2 = DT::id == SQMP_F32 ? 0 : 2;
     if constexpr (EXP) {
       // (many experts' blocks: 4 waves, 8 experts x 688 blocks of K 4096 61 us against 74 with 8)
-      if ((long)nb * E >= 2048) SQMP_GV(1, 2, 4, 4, false, 0);
-      else SQMP_GV(1, 2, 8, 4, false, 0);
+      if ((long)nb * E >= 2048) {
+        if (max_rows <= 8) SQMP_GV(1, 2, 4, 4, false, N1); else SQMP_GV(1, 2, 4, 4, false, N2);
+      } else {
+        if (max_rows <= 8) SQMP_GV(1, 2, 8, 4, false, N1); else SQMP_GV(1, 2, 8, 4, false, N2);
+      }
     } else {
 #define SQMP_GVX(J, NW)                                                                            \
   if (a.amap) SQMP_GV(1, J, NW, 4, true, 0);                                                       \
-  else if (DT::id == SQMP_F32 || a.M <= 4) SQMP_GV(1, J, NW, 4, false, 0);                         \
-  else if (a.M <= 8) SQMP_GV(1, J, NW, 4, false, (DT::id == SQMP_F32 ? 0 : 1));                    \
-  else SQMP_GV(1, J, NW, 4, false, (DT::id == SQMP_F32 ? 0 : 2))
-      if (nb <= 192) { SQMP_GVX(1, 16); }
+  else if (a.M <= 8) SQMP_GV(1, J, NW, 4, false, N1);                                              \
+  else SQMP_GV(1, J, NW, 4, false, N2)
+      if (nb <= 192) { SQMP_GVX(1, 8); }
       else if (nb <= 320) { SQMP_GVX(2, 16); }
       else { SQMP_GVX(2, 8); }
 #undef SQMP_GVX
@@ -384,7 +397,10 @@ extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* row
     return w4::launch_expert_tiles(a, dtype, E, slots, act,
                                    workspace && ws_bytes >= w4::expert_tiles_workspace(E, slots, N, Kp)
                                        ? (float*)workspace : nullptr, s);
-  const int est = cdiv(slots, E) * 2;  // rows of a busy expert (any count is right)
+  // the most rows an expert can have where a token picks it once (any count is right: more take
+  // more passes), or twice the mean where that is less
+  const int most = rows ? x_rows : cdiv(slots, top_k), twice = cdiv(slots, E) * 2;
+  const int est = most <= 8 || most < twice ? most : twice;
 #define SQMP_EX(DTT)                                                                  \
   switch (act) {                                                                      \
     case w4::ACT_SILU: return w4::by_group<DTT, true, w4::ACT_SILU>(a, E, est, s);    \
