@@ -266,7 +266,38 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
 
     x: [tokens, K] (rows="token") or [tokens * top_k, K] already in expert order (rows="slot").
     Rows of z behind routing.offsets[-1] (tokens that go nowhere) are left as they were."""
-    ops._require_gpu(x, "expert_linear")
+    if not x.is_cuda:
+        ops._require_gpu(x, "expert_linear")
+    code = ACTS.get(act, -1)
+    by_slot = rows == "slot"
+    S, dev = routing.rows.shape[0], x.device
+    if (code < 0 or (code > 0) != pe.gated or not (by_slot or rows == "token")
+            or routing.num_experts != pe.num_experts or x.dim() != 2
+            or x.shape[0] != (S if by_slot else routing.ids.shape[0]) or x.shape[1] != pe.K
+            or x.dtype is not pe.dtype or dev != pe.codes_t.device or routing.rows.device != dev):
+        _expert_refuse(x, pe, routing, act, rows)
+    if out is None:
+        out = x.new_empty((S, pe.n_out))
+    elif (tuple(out.shape) != (S, pe.n_out) or out.dtype != pe.dtype or out.device != dev
+          or not out.is_contiguous()):
+        raise ValueError(f"expert_linear: out must be contiguous {pe.dtype} [{S}, {pe.n_out}] on {dev}")
+    if S == 0:
+        return out
+    a, pairs = _operand(x, pe, routing, by_slot)
+    lib, dt = load(), ops.DTYPE_CODE[pe.dtype]
+    n = ops.workspace_bytes("expert", dt, pe.num_experts, S, pe.N, pe.Kp)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    status = lib.sqmp_expert_linear_w4(
+        a.data_ptr(), a.stride(0) if a.shape[0] > 1 else pe.Kp + pe.S_pad, _ptr(pairs),
+        routing.ids.shape[1], routing.offsets.data_ptr(), pe.num_experts, pe.codes_t.data_ptr(),
+        pe.scale_t.data_ptr(), _ptr(pe.sal_t), out.data_ptr(), dt, S, a.shape[0], pe.N, pe.n_out,
+        pe.Kp, pe.S_pad, pe.Gw, pe.ngw, code, _ptr(ws), n, ops._raw_stream(dev.index))
+    if status:
+        check(status, "expert_linear")
+    return out
+
+
+def _expert_refuse(x, pe, routing, act, rows):
     if act not in ACTS:
         raise ValueError(f"expert_linear: act must be one of {sorted(map(str, ACTS))}, got {act!r}")
     if (act is not None) != pe.gated:
@@ -277,34 +308,13 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
     if routing.num_experts != pe.num_experts:
         raise ValueError(f"expert_linear: routing over {routing.num_experts} experts, weight of "
                          f"{pe.num_experts}")
-    S = routing.rows.shape[0]
-    want = (S if rows == "slot" else routing.tokens, pe.K)
+    want = (routing.rows.shape[0] if rows == "slot" else routing.tokens, pe.K)
     if tuple(x.shape) != want:
         raise ValueError(f"expert_linear: x must be {list(want)}, got {list(x.shape)}")
     if x.dtype != pe.dtype:
         raise RuntimeError(f"expected input dtype {pe.dtype}, got {x.dtype}")
-    if x.device != pe.codes_t.device or routing.rows.device != x.device:
-        raise RuntimeError(f"expert_linear: x on {x.device}, weight on {pe.codes_t.device}, routing "
-                           f"on {routing.rows.device}")
-    if out is None:
-        out = torch.empty((S, pe.n_out), dtype=pe.dtype, device=x.device)
-    elif (tuple(out.shape) != (S, pe.n_out) or out.dtype != pe.dtype or out.device != x.device
-          or not out.is_contiguous()):
-        raise ValueError(f"expert_linear: out must be contiguous {pe.dtype} [{S}, {pe.n_out}] on "
-                         f"{x.device}")
-    if S == 0:
-        return out
-    a, pairs = _operand(x, pe, routing, rows == "slot")
-    lib, code = load(), ops._dtype_code(pe.dtype)
-    n = lib.sqmp_expert_workspace_bytes(code, pe.num_experts, S, pe.N, pe.Kp)
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    check(lib.sqmp_expert_linear_w4(a.data_ptr(), a.stride(0) if a.shape[0] > 1 else pe.Kp + pe.S_pad,
-                                    _ptr(pairs), routing.top_k, routing.offsets.data_ptr(),
-                                    pe.num_experts, pe.codes_t.data_ptr(), pe.scale_t.data_ptr(),
-                                    _ptr(pe.sal_t), out.data_ptr(), code, S, a.shape[0], pe.N,
-                                    pe.n_out, pe.Kp, pe.S_pad, pe.Gw, pe.ngw, ACTS[act], _ptr(ws), n,
-                                    ops._raw_stream(x.device.index)), "expert_linear")
-    return out
+    raise RuntimeError(f"expert_linear: x on {x.device}, weight on {pe.codes_t.device}, routing on "
+                       f"{routing.rows.device}")
 
 
 @ops.on_tensor_device
@@ -431,9 +441,14 @@ class W4A4Experts(nn.Module):
             kw.update({n: self._meta[f"{part}_{n}"] for n in _INTS})
             pes.append(PackedExperts(dtype=self._meta["dtype"], **kw))
         dev = pes[0].codes_t.device
-        maps = [ops.build_maps(pe.K, pe.salient, dev)[2:] for pe in pes]
-        self.__dict__["_packed"] = (b, (pes[0], pes[1], maps))
-        return self.__dict__["_packed"][1]
+        with torch.cuda.device(dev):
+            maps = [ops.build_maps(pe.K, pe.salient, dev)[2:] for pe in pes]
+            if not torch.cuda.is_current_stream_capturing():
+                # kept: built on one stream, read later from any (a capture's maps belong to its
+                # replays and are built again)
+                torch.cuda.synchronize(dev)
+                self.__dict__["_packed"] = (b, (pes[0], pes[1], maps))
+        return pes[0], pes[1], maps
 
     # -------------------------------------------------------------- forward
     def _quant(self, t2: torch.Tensor, pe: PackedExperts, maps) -> torch.Tensor:

@@ -1070,6 +1070,20 @@ def tile_major(codes: torch.Tensor, wscale: torch.Tensor, wsal: torch.Tensor, N:
     return out
 
 
+_SPLIT_WS = {}
+_lib.on_reload(_SPLIT_WS.clear)  # (the tile height is a knob)
+
+
+def workspace_bytes(kind: str, *sizes: int) -> int:
+    """sqmp_<kind>_workspace_bytes(*sizes), memoized (saves a ctypes call per product)."""
+    n = _SPLIT_WS.get((kind, sizes))
+    if n is None:
+        n = _SPLIT_WS[(kind, sizes)] = getattr(load(), f"sqmp_{kind}_workspace_bytes")(*sizes)
+        if len(_SPLIT_WS) > 65536:
+            _SPLIT_WS.clear()
+    return n
+
+
 def gemv_eligible(pw: PackedWeight) -> bool:
     """Whether gemv computes this weight: 4-bit codes in groups of whole 8 positions."""
     return pw.n_bits == 4 and pw.dense is None and pw.Gw % 8 == 0
@@ -1163,7 +1177,7 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
         xp, ld = x.data_ptr(), L
     wp, wn = None, 0
     if M > 16:
-        wn = lib.sqmp_gemv_workspace_bytes(code, M, N, pw.Kp)
+        wn = workspace_bytes("gemv", code, M, N, pw.Kp)
         if wn:
             ws = torch.empty(wn, dtype=torch.uint8, device=device)
             wp = ws.data_ptr()

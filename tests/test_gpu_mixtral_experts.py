@@ -82,6 +82,33 @@ def test_module(wq, aq, p, T, dt):
         mod.to(torch.float64)
 
 
+@pytest.mark.parametrize("T", [3, 90])
+@pytest.mark.parametrize("aq", ["per_token", None])
+def test_module_captured(T, aq):
+    """The module captured before and after its first eager call: replays equal the eager bits, and
+    nothing that a capture built is used outside of it."""
+    g = gen(T)
+    base = copy.deepcopy(_model(3).model.layers[0].mlp.experts).to("cuda", torch.float16)
+    x = torch.randn(T, base.hidden_dim, generator=g, device="cuda").half()
+    ids = torch.rand(T, base.num_experts, generator=g, device="cuda").topk(2, dim=1).indices
+    w = torch.rand(T, 2, generator=g, device="cuda")
+    warm = experts.W4A4Experts.from_float(base, "per_channel", aq, None, 0, 4, 32)
+    want = warm(x, ids, w)
+    fresh = experts.W4A4Experts.from_float(base, "per_channel", aq, None, 0, 4, 32)
+    for mod in (warm, fresh):
+        xs = x.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = mod(xs, ids, w)
+        assert torch.equal(mod(x, ids, w), want)          # eager between capture and replay
+        for i in range(3):
+            xs.copy_(x.roll(i, 0))
+            graph.replay()
+            eager = mod(x.roll(i, 0), ids, w)
+            torch.cuda.synchronize()
+            assert torch.equal(y, eager)
+
+
 @pytest.mark.parametrize("aq,p", [("per_token", 0.0), ("per_token", 0.1)])
 def test_quantize_mixtral_experts(tmp_path, aq, p):
     from smoothquant.calibration import get_calib_feat
