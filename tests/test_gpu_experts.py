@@ -385,3 +385,38 @@ def test_block_captured_and_replayed(T):
         torch.cuda.synchronize()
         assert torch.equal(y, eager)
     assert torch.equal(block(x, logits)[0], y0)                 # the same bits again
+
+
+def test_offsets_beyond_32_bits():
+    """Operands and outputs of more than 4 GiB: rows and weights on either side of the border."""
+    D, g = torch.float16, gen(8)
+    # a weight whose codes take 4.3 GB
+    N, K = 1_050_000, 8192
+    codes = torch.randint(-8, 8, (N, K), generator=g, device="cuda", dtype=torch.int8)
+    scales = torch.ones(N, K // 256, device="cuda", dtype=D)
+    scales[::2] = 0.5
+    pw = ops.pack_codes(codes, scales, 256)
+    for M in (1, 20):
+        x = int_rows(M, K, D, g)
+        y = ops.gemv(x, pw)
+        pick = torch.cat([torch.arange(64), torch.arange(N // 2, N // 2 + 64), torch.arange(N - 64, N)]).cuda()
+        want = x.double() @ values(codes[pick], scales[pick], 256).T
+        assert torch.equal(y[:, pick], want.float().to(D))
+    del codes, scales, pw
+    # rows in expert order, 4.9 GB of them; then the same rows picked by token
+    T, K, N = 600_000, 4096, 40
+    codes, scales = int_weight((3, N, K), 128, D, g)
+    pe = experts.pack_expert_codes(codes, scales, 128)
+    x = torch.randint(-4, 5, (T, K), generator=g, device="cuda", dtype=torch.int8).to(D)
+    ids = torch.randint(0, 3, (T, 1), generator=g, device="cuda")
+    r = experts.plan_routes(ids, torch.ones(T, 1, device="cuda"), 3)
+    pick = torch.cat([torch.arange(50), torch.arange(T // 2, T // 2 + 50), torch.arange(T - 50, T)]).cuda()
+    e_of = ids.view(-1)[r.rows.long()]
+    w = values(codes, scales, 128)
+    for by_slot in (True, False):
+        z = experts.expert_linear(x, pe, r, rows="slot" if by_slot else "token")
+        src = pick if by_slot else r.rows.long()[pick]
+        want = torch.einsum("sk,snk->sn", x[src].double(), w[e_of[pick]])
+        assert torch.equal(z[pick], want.float().to(D))
+    y = experts.combine(z, r)
+    assert torch.equal(y[r.rows.long()[pick]], z[pick])
