@@ -50,7 +50,8 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
   }
   const int nblk = (a.N + 255) / 256 * 8;  // 32-row blocks of one weight's operands
   const int nkm = a.Kp / 64, nks = a.S_pad / 64;
-  int lo = 0, hi = a.M;
+  // one weight: every pass of tokens has workgroups of its own (blockIdx.y)
+  int lo = (int)blockIdx.y * PASS, hi = min(a.M, lo + PASS);
   long wb = nb;
   if constexpr (EXP) {
     lo = a.offsets[blockIdx.y];
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
         T v[16];
 #pragma unroll
         for (int m = 0; m < 16; ++m)
-          if (m < M) v[m] = k >= 0 ? x[(long)m * a.ldx + k] : (T)0.f;
+          if (m < M) v[m] = k >= 0 ? x[(long)(lo + m) * a.ldx + k] : (T)0.f;
 #pragma unroll
         for (int m = 0; m < 16; ++m)
           if (m < M) ((T*)xs)[(long)m * LP + p] = v[m];
@@ -258,44 +259,46 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
 // below 64 KiB)
 constexpr long STAGE_BYTES = 27 * 1024;
 static long stage_bytes(int dtype, int M, int Kp, int S_pad) {
-  return (long)M * ((Kp + S_pad) * (dtype == SQMP_F32 ? 4 : 2) + 16);
+  return (long)(M < 16 ? M : 16) * ((Kp + S_pad) * (dtype == SQMP_F32 ? 4L : 2L) + 16);
 }
 
 template <class DT, int GB, bool EXP, int ACT>
 static int launch(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
   const int nb = cdiv(a.N, 32);
   const size_t xb = a.amap ? (size_t)stage_bytes(DT::id, a.M, a.Kp, a.S_pad) : 0;
+  const int groups = a.M <= 16 ? 1 : cdiv(a.M, 16);  // of 16 tokens (one weight)
 #define SQMP_GV(MT, J, NW, U, ST, NX)                                                                  \
   gemv_kernel<DT, GB, MT, J, NW, U, ST, NX, EXP, ACT>                                                  \
-      <<<dim3((J) == 1 ? cdiv(nb, 8) * 16 : nb, EXP ? E : 1), dim3((NW) * 64), xb, s>>>(a)
-  if (max_rows <= 16) {
-    // Waves per workgroup, and whether a block's halves go to two workgroups, by how many blocks
-    // there are for the 256 CUs.  8 waves / 16 waves / 8 waves and halves / 16 and halves, one row, one
-    // card: 32 blocks of K 4096 4.9 / 4.7 / 4.1 / 4.1 us, 128 of K 4096 5.2 / 4.9 / 4.4 / 4.4, of K 11008
-    // 10.1 / 9.4 / 7.9 / 8.4, 256 of K 2048 (fp32) 8.5 / 8.1 / 8.6 / 10.1, 344 of K 4096 8.1 / 9.2 / 8.8
-    // / 10.6, 1000 of K 4096 19.7 / 21.6 / 20.8 / 28.8
-    constexpr int N1 = DT::id == SQMP_F32 ? 0 : 1, N2 = DT::id == SQMP_F32 ? 0 : 2;
-    if constexpr (EXP) {
-      // (many experts' blocks: 4 waves, 8 experts x 688 blocks of K 4096 61 us against 74 with 8)
+      <<<dim3((J) == 1 ? cdiv(nb, 8) * 16 : nb, EXP ? E : groups), dim3((NW) * 64), xb, s>>>(a)
+  // Waves per workgroup, and whether a block's halves go to two workgroups, by how many blocks
+  // there are for the 256 CUs.  8 waves / 16 waves / 8 waves and halves / 16 and halves, one row, one
+  // card: 32 blocks of K 4096 4.9 / 4.7 / 4.1 / 4.1 us, 128 of K 4096 5.2 / 4.9 / 4.4 / 4.4, of K 11008
+  // 10.1 / 9.4 / 7.9 / 8.4, 256 of K 2048 (fp32) 8.5 / 8.1 / 8.6 / 10.1, 344 of K 4096 8.1 / 9.2 / 8.8
+  // / 10.6, 1000 of K 4096 19.7 / 21.6 / 20.8 / 28.8
+  constexpr int N1 = DT::id == SQMP_F32 ? 0 : 1, N2 = DT::id == SQMP_F32 ? 0 : 2;
+  if constexpr (EXP) {
+    // (many experts' blocks: 4 waves, 8 experts x 688 blocks of K 4096 61 us against 74 with 8)
+    if (max_rows <= 16) {
       if ((long)nb * E >= 2048) {
         if (max_rows <= 8) SQMP_GV(1, 2, 4, 4, false, N1); else SQMP_GV(1, 2, 4, 4, false, N2);
       } else {
         if (max_rows <= 8) SQMP_GV(1, 2, 8, 4, false, N1); else SQMP_GV(1, 2, 8, 4, false, N2);
       }
+    } else if (max_rows <= 32) {
+      SQMP_GV(2, 2, 8, 2, false, 0);
     } else {
+      SQMP_GV(4, 2, 8, 1, false, 0);
+    }
+  } else {
 #define SQMP_GVX(J, NW)                                                                            \
   if (a.amap) SQMP_GV(1, J, NW, 4, true, 0);                                                       \
   else if (a.M <= 8) SQMP_GV(1, J, NW, 4, false, N1);                                              \
   else SQMP_GV(1, J, NW, 4, false, N2)
-      if (nb <= 192) { SQMP_GVX(1, 8); }
-      else if (nb <= 320) { SQMP_GVX(2, 16); }
-      else { SQMP_GVX(2, 8); }
+    const int blocks = nb * groups;
+    if (blocks <= 192) { SQMP_GVX(1, 8); }
+    else if (blocks <= 320) { SQMP_GVX(2, 16); }
+    else { SQMP_GVX(2, 8); }
 #undef SQMP_GVX
-    }
-  } else if (max_rows <= 32) {
-    SQMP_GV(2, 2, 8, 2, false, 0);
-  } else {
-    SQMP_GV(4, 2, 8, 1, false, 0);
   }
 #undef SQMP_GV
   SQMP_LAUNCH_CHECK();
@@ -336,7 +339,8 @@ extern "C" size_t sqmp_expert_workspace_bytes(int dtype, int E, int slots, int N
 
 // whether sqmp_gemv_w4 gathers these rows itself (amap)
 extern "C" int sqmp_gemv_gathers(int dtype, int M, int Kp, int S_pad) {
-  return M <= 16 && w4::stage_bytes(dtype, M, Kp, S_pad) <= w4::STAGE_BYTES;
+  return M <= (dtype == SQMP_F32 ? SQMP_GEMV_MAX_ROWS : 16) &&
+         w4::stage_bytes(dtype, M, Kp, S_pad) <= w4::STAGE_BYTES;
 }
 
 extern "C" int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const int32_t* salient,
@@ -359,7 +363,8 @@ extern "C" int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const 
   a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
   w4::set_groups(a);
   hipStream_t s = (hipStream_t)stream;
-  if (M > 16 && w4::expert_tiles_ok(a, dtype, 1, M))
+  const char* k = knob("SQMP_EXPERT_ROWS");
+  if (M > 16 && !(k && atoi(k) == 0) && w4::expert_tiles_ok(a, dtype, 1, M))
     return w4::launch_expert_tiles(a, dtype, 1, M, w4::ACT_NONE,
                                    workspace && ws_bytes >= w4::expert_tiles_workspace(1, M, N, Kp)
                                        ? (float*)workspace : nullptr, s);
