@@ -12,11 +12,10 @@
 // in flight each; the NW partial sums meet in LDS and are added in a fixed order, so results do not
 // depend on timing.  x comes as 16-byte fragments from L2, or, where its rows are unaligned or the
 // weight has an order of its own, gathered into LDS while the first codes are on their way.
-// Measured in a captured graph: 1 x 4096 x 4096 fp16 4.5 us (8.7 MB: 1.9 TB/s, 1.7 us at the rate of a
-// large copy; latency), 8 x 11008 x 4096 bf16 10.3 us (2.3 TB/s; decoding, and 344 blocks on 256
-// CUs), 1 x 32000 x 4096 16.8 us (4.0 TB/s), 8 experts of 2 rows, 22016 x 4096: 63 us (5.3 TB/s).
-// From 17 rows on (fp16 / bf16, groups of 32 or of whole stages) the product runs on the expert
-// tiles, K split over workgroups: 64 x 4096 x 11008 43 us here, 23 us there.
+// Measured in a captured graph: 1 x 4096 x 4096 fp16 4.4 us (8.7 MB: 2.0 TB/s, 1.7 us at the rate of a
+// large copy; latency), 8 x 11008 x 4096 bf16 9.5 us (2.5 TB/s; decoding, and 344 blocks on 256
+// CUs), 1 x 32000 x 4096 15.1 us (4.5 TB/s), 64 x 4096 x 11008 16.1 us (1.6 TB/s; two groups of tokens
+// decode everything twice), 8 experts of 2 rows, 22016 x 4096: 62 us (5.4 TB/s).
 #include "sqmp_w4_launch.h"
 
 namespace sqmp {
@@ -25,7 +24,7 @@ namespace w4 {
 // GB: 1 = groups of whole 64-position stages, 2 = groups of 32, 0 = any multiple of 8
 // MT: 16-row token tiles per pass; J: 16-row halves of the block per workgroup (1: two workgroups,
 // neighbours on one XCD, share the block's lines); NW waves; U stages in flight; STAGE: the rows of
-// x gathered into LDS first; NX > 0 (16-bit types, MT 1): a stage's rows come as 8 NX whole 128-byte
+// x gathered into LDS first; NX > 0 (16-bit types): a stage's rows come as 8 NX whole 128-byte
 // lines and are turned into fragments in a wave's own corner of LDS (fragments straight from L2
 // touch every line four times); ACT / EXP: the expert forms
 template <class DT, int GB, int MT, int J, int NW, int U, bool STAGE, int NX, bool EXP, int ACT>
@@ -35,10 +34,11 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
   constexpr int RS = 16 * J + 4;  // floats per token row of a partial (+ 4: spreads the LDS banks)
   static_assert(ACT == ACT_NONE || J == 2, "gate and up rows meet in one workgroup");
   __shared__ __attribute__((aligned(16))) float red[NW * MT * 16 * RS];
-  static_assert(NX == 0 || (MT == 1 && SZ == 2 && !STAGE), "whole lines: 16-bit rows");
+  static_assert(NX == 0 || (MT == (NX + 1) / 2 && SZ == 2 && !STAGE), "whole lines: 16-bit rows");
   constexpr int PASS = NX == 1 ? 8 : 16 * MT;  // tokens per pass over the weights
   constexpr int XP = 144;         // bytes of a row of the corner (128 + 16: spreads the banks)
-  __shared__ __attribute__((aligned(16))) unsigned char turn[NX > 0 ? NW * 2 * 16 * XP : 16];
+  constexpr int CORNER = 8 * NX * XP, NC = NX <= 2 ? 2 : 1;  // two corners a wave where they are small
+  __shared__ __attribute__((aligned(16))) unsigned char turn[NX > 0 ? NW * NC * CORNER : 16];
   extern __shared__ __attribute__((aligned(16))) unsigned char xs[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -155,15 +155,18 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
       if constexpr (NX > 0) {
         // (the LDS operations of one wave run in order: the reads see the writes, and the next
         // writes to this half come after these reads)
-        unsigned char* t = turn + (wave * 2 + (u & 1)) * 16 * XP;
+        unsigned char* t = turn + (wave * NC + (u % NC)) * CORNER;
 #pragma unroll
         for (int i = 0; i < NX; ++i)
           *(u32x4*)(t + (8 * i + (lane >> 3)) * XP + (lane & 7) * 16) = st.line[i];
         asm volatile("" ::: "memory");
-        const int r = NX == 1 ? r16 & 7 : r16;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-          st.x[0][s] = load_frag<DT>((const T*)(t + r * XP + (c0 + 2 * s) * 16));
+        for (int i = 0; i < MT; ++i) {
+          const int r = NX == 1 ? r16 & 7 : 16 * i + r16;
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            st.x[i][s] = load_frag<DT>((const T*)(t + r * XP + (c0 + 2 * s) * 16));
+        }
         asm volatile("" ::: "memory");
       }
 #pragma unroll
@@ -284,16 +287,25 @@ static int launch(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
       } else {
         if (max_rows <= 8) SQMP_GV(1, 2, 8, 4, false, N1); else SQMP_GV(1, 2, 8, 4, false, N2);
       }
-    } else if (max_rows <= 32) {
-      SQMP_GV(2, 2, 8, 2, false, 0);
     } else {
-      SQMP_GV(4, 2, 8, 1, false, 0);
+      SQMP_GV(2, 2, 8, 2, false, (DT::id == SQMP_F32 ? 0 : 4));
     }
   } else {
 #define SQMP_GVX(J, NW)                                                                            \
   if (a.amap) SQMP_GV(1, J, NW, 4, true, 0);                                                       \
   else if (a.M <= 8) SQMP_GV(1, J, NW, 4, false, N1);                                              \
   else SQMP_GV(1, J, NW, 4, false, N2)
+    if constexpr (DT::id != SQMP_F32) {
+      // 17 .. 64 rows where groups of 16 are more than the CUs: groups of 32, a decoded fragment feeds
+      // two MFMAs (16 / 32 a group, fp16: 64 rows x 4096 x 4096 9.8 / 7.7 us, x 11008 x 4096 25.9 / 17.0; 32
+      // x 32000 x 4096 39.6 / 26.3; but 32 x 4096 x 4096 5.8 / 7.4, 64 x 1024 x 4096 5.4 / 7.1)
+      if (a.M > 16 && !a.amap && nb * groups > 256) {
+        const int groups = cdiv(a.M, 32);
+        SQMP_GV(2, 2, 8, 2, false, 4);
+        SQMP_LAUNCH_CHECK();
+        return SQMP_OK;
+      }
+    }
     const int blocks = nb * groups;
     if (blocks <= 192) { SQMP_GVX(1, 8); }
     else if (blocks <= 320) { SQMP_GVX(2, 16); }
@@ -313,6 +325,12 @@ static int by_group(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
   return SQMP_EUNSUPPORTED;
 }
 
+// Whether a single weight goes to the expert tiles: more than 32 rows of a wide one (64 rows, few-row
+// kernel / tiles: N 11008 17.0 / 24.6 us, 32000 43.9 / 38.5; 32 rows of 32000 26.3 / 34.6)
+static bool gemv_takes_tiles(int dtype, int M, int N) {
+  return dtype != SQMP_F32 && M > 32 && cdiv(N, 32) > 700;
+}
+
 static int check_operand(const void* x, long ldx, int dtype, int N, int Kp, int S_pad, int Gw,
                          int ngw, bool gathered = false) {
   if (N <= 0 || Kp <= 0 || Kp % 128 || S_pad < 0 || S_pad % 64 || Gw <= 0 || ngw <= 0)
@@ -328,12 +346,12 @@ static int check_operand(const void* x, long ldx, int dtype, int N, int Kp, int 
 
 // (0 where the few-row kernel runs, which splits K inside a workgroup)
 extern "C" size_t sqmp_gemv_workspace_bytes(int dtype, int M, int N, int Kp) {
-  if (M <= 16 || N <= 0 || Kp <= 0 || dtype == SQMP_F32) return 0;
+  if (N <= 0 || Kp <= 0 || !w4::gemv_takes_tiles(dtype, M, N)) return 0;
   return w4::expert_tiles_workspace(1, M, N, Kp);
 }
 
 extern "C" size_t sqmp_expert_workspace_bytes(int dtype, int E, int slots, int N, int Kp) {
-  if (E <= 0 || slots < 8 * (long)E || N <= 0 || Kp <= 0 || dtype == SQMP_F32) return 0;
+  if (E <= 0 || slots < 12L * E || N <= 0 || Kp <= 0 || dtype == SQMP_F32) return 0;
   return w4::expert_tiles_workspace(E, slots, N, Kp);
 }
 
@@ -363,8 +381,7 @@ extern "C" int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const 
   a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
   w4::set_groups(a);
   hipStream_t s = (hipStream_t)stream;
-  const char* k = knob("SQMP_EXPERT_ROWS");
-  if (M > 16 && !(k && atoi(k) == 0) && w4::expert_tiles_ok(a, dtype, 1, M))
+  if (w4::gemv_takes_tiles(dtype, M, N) && w4::expert_tiles_ok(a, dtype, 1, M))
     return w4::launch_expert_tiles(a, dtype, 1, M, w4::ACT_NONE,
                                    workspace && ws_bytes >= w4::expert_tiles_workspace(1, M, N, Kp)
                                        ? (float*)workspace : nullptr, s);
@@ -395,10 +412,11 @@ extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* row
   a.rows = rows, a.offsets = offsets, a.top_k = top_k;
   w4::set_groups(a);
   hipStream_t s = (hipStream_t)stream;
-  // tiles from 8 rows per expert on (few-row kernel / 64-row tiles: 64 experts of 6 rows 56 / 71 us,
-  // 8 of 16 rows 147 / 115 us); SQMP_EXPERT_ROWS = 0 / a tile height overrides (A/B)
+  // tiles from 12 rows per expert on (few-row kernel / tiles, 8 experts, 4096 -> 2 x 11008 gated: 8 rows
+  // each 111 / 133 us, 16: 124 / 115, 24: 184 / 150; 64 of 2048 -> 2 x 1408: 6 rows 48 / 63, 12: 73 / 60);
+  // SQMP_EXPERT_ROWS = 0 / a tile height overrides (A/B)
   const char* k = knob("SQMP_EXPERT_ROWS");
-  if (w4::expert_tiles_ok(a, dtype, E, x_rows) && (k ? atoi(k) > 0 : slots >= 8L * E))
+  if (w4::expert_tiles_ok(a, dtype, E, x_rows) && (k ? atoi(k) > 0 : slots >= 12L * E))
     return w4::launch_expert_tiles(a, dtype, E, slots, act,
                                    workspace && ws_bytes >= w4::expert_tiles_workspace(E, slots, N, Kp)
                                        ? (float*)workspace : nullptr, s);

@@ -1176,7 +1176,7 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
         x = pack_rows(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
         xp, ld = x.data_ptr(), L
     wp, wn = None, 0
-    if M > 16:
+    if M > 32:
         wn = workspace_bytes("gemv", code, M, N, pw.Kp)
         if wn:
             ws = torch.empty(wn, dtype=torch.uint8, device=device)
