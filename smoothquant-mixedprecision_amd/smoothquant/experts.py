@@ -246,15 +246,17 @@ def _operand(x: torch.Tensor, pe: PackedExperts, r: Routing, by_slot: bool):
         return x, rows
     if x.stride(1) != 1 or x.stride(0) == 0:  # (0: rows of an expanded tensor)
         x = x.contiguous()
-    L = pe.Kp + pe.S_pad
     own = pe.amap.dim() == 2
     n = r.rows.shape[0] if own else x.shape[0]
-    out = torch.empty((n, L), dtype=x.dtype, device=x.device)
-    p = ops._p
-    check(load().sqmp_pack_rows(p(x), max(x.stride(0), 1), ops._dtype_code(x.dtype), n, p(pe.amap),
-                                pe.Kp, p(pe.salient), pe.S, pe.S_pad, p(rows) if own else None,
-                                r.top_k, p(r.offsets) if own else None, pe.num_experts,
-                                pe.Kp if own else 0, p(out), ops._stream(x)), "pack_rows")
+    out = x.new_empty((n, pe.Kp + pe.S_pad))
+    status = load().sqmp_pack_rows(x.data_ptr(), max(x.stride(0), 1), ops.DTYPE_CODE[x.dtype], n,
+                                   pe.amap.data_ptr(), pe.Kp, _ptr(pe.salient), pe.S, pe.S_pad,
+                                   _ptr(rows) if own else None, r.ids.shape[1],
+                                   r.offsets.data_ptr() if own else None, pe.num_experts,
+                                   pe.Kp if own else 0, out.data_ptr(),
+                                   ops._raw_stream(x.device.index))
+    if status:
+        check(status, "pack_rows")
     return out, None if own else rows
 
 

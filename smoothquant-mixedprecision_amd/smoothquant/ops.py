@@ -1119,12 +1119,18 @@ def pack_rows(x2: torch.Tensor, amap: torch.Tensor, Kp: int, salient: Optional[t
               S: int, S_pad: int) -> torch.Tensor:
     """x [M, K] -> [M, Kp + S_pad]: the unquantized activation operand (columns gathered by amap,
     then the salient columns)."""
+    if not x2.is_cuda:
+        _require_gpu(x2, "pack_rows")
     if x2.stride(1) != 1 or x2.stride(0) == 0:  # (0: rows of an expanded tensor)
         x2 = x2.contiguous()
-    out = torch.empty((x2.shape[0], Kp + S_pad), dtype=x2.dtype, device=x2.device)
-    check(load().sqmp_pack_rows(_p(x2), max(x2.stride(0), 1), _dtype_code(x2.dtype), x2.shape[0],
-                                _p(amap), Kp, _p(salient), S, S_pad, None, 1, None, 0, 0, _p(out),
-                                _stream(x2)), "pack_rows")
+    M = x2.shape[0]
+    out = x2.new_empty((M, Kp + S_pad))
+    status = load().sqmp_pack_rows(x2.data_ptr(), max(x2.stride(0), 1), _dtype_code(x2.dtype), M,
+                                   amap.data_ptr(), Kp,
+                                   None if salient is None else salient.data_ptr(), S, S_pad, None,
+                                   1, None, 0, 0, out.data_ptr(), _raw_stream(x2.device.index))
+    if status:
+        check(status, "pack_rows")
     return out
 
 
@@ -1173,7 +1179,7 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
     elif s1 == 1 and ld > 0 and lib.sqmp_gemv_gathers(code, M, pw.Kp, pw.S_pad):
         amap, sal = pw.amap.data_ptr(), None if pw.salient is None else pw.salient.data_ptr()
     else:
-        x = pack_rows(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
+        x = pack_rows.__wrapped__(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
         xp, ld = x.data_ptr(), L
     wp, wn = None, 0
     if M > 32:
