@@ -423,11 +423,13 @@ int sqmp_gemm_h2d(const void* a2, int ldr, const int* aexp, const void* wt, cons
 /* workspace: in it the fp32 sums of tiles whose K is split meet (no need to clear it; NULL or a
  * smaller one than asked for: no tile is split, the same values in another order of summation) */
 size_t sqmp_gemv_workspace_bytes(int dtype, int M, int N, int Kp);
+/* cols: the leading coded positions that x's rows hold: Kp, or, without salient columns, a multiple
+ * of 64 below it (the positions behind are padding, whose codes are 0; they are not read). */
 /* amap (int32 [Kp], with salient int32 [S]): x holds the columns in their own order, rows of any
  * stride and alignment; operand position p is column amap[p] (zero where < 0) -- where
  * sqmp_gemv_gathers says so (few rows; else SQMP_EUNSUPPORTED: sqmp_pack_rows first). */
 int sqmp_gemv_gathers(int dtype, int M, int Kp, int S_pad);
-int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const int32_t* salient, int S,
+int sqmp_gemv_w4(const void* x, long ldx, int cols, const int32_t* amap, const int32_t* salient, int S,
                  const void* codes_t, const void* scale_t, const void* sal_t, const void* bias,
                  void* y, int dtype, int M, int N, int Kp, int S_pad, int Gw, int ngw,
                  void* workspace, size_t ws_bytes, void* stream);
@@ -455,7 +457,7 @@ int sqmp_plan_routes(const int32_t* ids, int T, int E, int top_k, int32_t* offse
  * slots = rows of z (an upper bound of offsets[E]); rows of z behind offsets[E] are left as they
  * were.  x_rows: rows of x. */
 size_t sqmp_expert_workspace_bytes(int dtype, int E, int slots, int N, int Kp);
-int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* rows, int top_k,
+int sqmp_expert_linear_w4(const void* x, long ldx, int cols, const int32_t* rows, int top_k,
                           const int32_t* offsets, int E, const void* codes_t, const void* scale_t,
                           const void* sal_t, void* y, int dtype, int slots, int x_rows, int N,
                           int n_out, int Kp, int S_pad, int Gw, int ngw, int act, void* workspace,

@@ -165,7 +165,7 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int r16 = lane & 15, q = lane >> 4;
   const int e = t.e, m0 = t.m0, nm = t.m1 - t.m0, tn = t.tn;
-  const int nks_all = a.S_pad / 64, nkm_all = a.Kp / 64;
+  const int nks_all = a.S_pad / 64, nkm_all = a.nk;
   // this part's stages: codes [k0, nkm), then (last part) the salient ones up to nkt
   const int k0 = (int)((long)nkm_all * t.part / t.parts) & ~3;
   const bool last = t.part + 1 == t.parts;
@@ -216,7 +216,7 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
 
   // weights
   const long wb = (long)e * ((a.N + 255) / 256 * 8) + tn * 8 + wave;
-  const __amdgpu_buffer_rsrc_t rW = rsrc_of(a.codes + wb * nkm_all * 256);
+  const __amdgpu_buffer_rsrc_t rW = rsrc_of(a.codes + wb * (a.Kp / 64) * 256);
   const __amdgpu_buffer_rsrc_t rS = rsrc_of((const T*)a.scale + wb * a.ngw * 32);
   struct Codes {
     u32x4 w;
@@ -286,7 +286,7 @@ __device__ inline void run_tile(const GemvArgs& a, int act, const Tile& t, unsig
   for (int kt = k0; kt < nkm; kt += DW)
 #pragma unroll
     for (int u = 0; u < DW; ++u)
-      if (u < 2 || kt + u < nkm) step(kt + u, cs[u], cs[(u + 1) % DW]);  // (nkm is even)
+      if (kt + u < nkm) step(kt + u, cs[u], cs[(u + 1) % DW]);
   // the exact salient columns: fragments as they are
   for (int kd = 0; kd < nks; ++kd) {
     const int kt = nkm + kd;

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
     if (nb * 32 + half * 16 >= a.N) return;
   }
   const int nblk = (a.N + 255) / 256 * 8;  // 32-row blocks of one weight's operands
-  const int nkm = a.Kp / 64, nks = a.S_pad / 64;
+  const int nkp = a.Kp / 64, nkm = a.nk, nks = a.S_pad / 64;
   // one weight: every pass of tokens has workgroups of its own (blockIdx.y)
   int lo = (int)blockIdx.y * PASS, hi = min(a.M, lo + PASS);
   long wb = nb;
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
     hi = a.offsets[blockIdx.y + 1];
     wb += (long)blockIdx.y * nblk;
   }
-  const __amdgpu_buffer_rsrc_t rW = rsrc_of(a.codes + wb * nkm * 256);
+  const __amdgpu_buffer_rsrc_t rW = rsrc_of(a.codes + wb * nkp * 256);
   const __amdgpu_buffer_rsrc_t rS = rsrc_of((const T*)a.scale + wb * a.ngw * 32);
   const T* sal = (const T*)a.sal + wb * nks * 2048 + lane * 32 + half * 16;
   const uint32_t vw = (uint32_t)lane * 16 + half * 8, vs = (uint32_t)(r16 * 2 + half) * SZ;
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(NW * 64) void gemv_kernel(const GemvArgs a) {
       for (int s = 0; s < 2; ++s) {
         Frag<DT> x[MT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) x[i] = load_frag<DT>(xp[i] + (long)(nkm + kd) * 64 + 16 * s);
+        for (int i = 0; i < MT; ++i) x[i] = load_frag<DT>(xp[i] + (long)(nkp + kd) * 64 + 16 * s);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const Frag<DT> w = load_frag<DT>(sal + (long)kd * 2048 + j * 16 + s * 8);
@@ -331,14 +331,15 @@ static bool gemv_takes_tiles(int dtype, int M, int N) {
   return dtype != SQMP_F32 && M > 32 && cdiv(N, 32) > 700;
 }
 
-static int check_operand(const void* x, long ldx, int dtype, int N, int Kp, int S_pad, int Gw,
-                         int ngw, bool gathered = false) {
+static int check_operand(const void* x, long ldx, int cols, int dtype, int N, int Kp, int S_pad,
+                         int Gw, int ngw, bool gathered = false) {
   if (N <= 0 || Kp <= 0 || Kp % 128 || S_pad < 0 || S_pad % 64 || Gw <= 0 || ngw <= 0)
     return SQMP_EINVAL;
   if (dtype != SQMP_F32 && dtype != SQMP_F16 && dtype != SQMP_BF16) return SQMP_EUNSUPPORTED;
-  if (gathered) return ldx > 0 ? SQMP_OK : SQMP_EINVAL;
+  if (gathered) return ldx > 0 && cols == Kp ? SQMP_OK : SQMP_EINVAL;
+  if (cols != Kp && (cols <= 0 || cols > Kp || cols % 64 || S_pad > 0)) return SQMP_EINVAL;
   const long per16 = dtype == SQMP_F32 ? 4 : 8;  // whole 16-byte loads of x
-  if (ldx < (long)Kp + S_pad || ldx % per16 || (size_t)x % 16) return SQMP_EINVAL;
+  if (ldx < (long)cols + S_pad || ldx % per16 || (size_t)x % 16) return SQMP_EINVAL;
   return SQMP_OK;
 }
 
@@ -361,8 +362,8 @@ extern "C" int sqmp_gemv_gathers(int dtype, int M, int Kp, int S_pad) {
          w4::stage_bytes(dtype, M, Kp, S_pad) <= w4::STAGE_BYTES;
 }
 
-extern "C" int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const int32_t* salient,
-                            int S, const void* codes_t, const void* scale_t,
+extern "C" int sqmp_gemv_w4(const void* x, long ldx, int cols, const int32_t* amap,
+                            const int32_t* salient, int S, const void* codes_t, const void* scale_t,
                             const void* sal_t, const void* bias, void* y, int dtype, int M, int N,
                             int Kp, int S_pad, int Gw, int ngw, void* workspace, size_t ws_bytes,
                             void* stream) {
@@ -370,7 +371,7 @@ extern "C" int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const 
   if (!x || !codes_t || !scale_t || !y || (S_pad > 0 && !sal_t)) return SQMP_EINVAL;
   if (M < 0 || M > SQMP_GEMV_MAX_ROWS) return SQMP_EINVAL;
   if (S < 0 || S > S_pad || (S > 0 && amap && !salient)) return SQMP_EINVAL;
-  const int st = w4::check_operand(x, ldx, dtype, N, Kp, S_pad, Gw, ngw, amap != nullptr);
+  const int st = w4::check_operand(x, ldx, cols, dtype, N, Kp, S_pad, Gw, ngw, amap != nullptr);
   if (st != SQMP_OK) return st;
   if (amap && !sqmp_gemv_gathers(dtype, M, Kp, S_pad)) return SQMP_EUNSUPPORTED;
   if (M == 0) return SQMP_OK;
@@ -378,7 +379,7 @@ extern "C" int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const 
   a.x = x, a.ldx = ldx, a.codes = (const uint32_t*)codes_t, a.scale = scale_t, a.sal = sal_t;
   a.bias = bias, a.y = y, a.M = M, a.N = N, a.n_out = N;
   a.amap = amap, a.salient = salient, a.S = S;
-  a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
+  a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw, a.nk = cols / 64;
   w4::set_groups(a);
   hipStream_t s = (hipStream_t)stream;
   if (w4::gemv_takes_tiles(dtype, M, N) && w4::expert_tiles_ok(a, dtype, 1, M))
@@ -390,7 +391,7 @@ extern "C" int sqmp_gemv_w4(const void* x, long ldx, const int32_t* amap, const 
   return w4::by_group<BF16, false, w4::ACT_NONE>(a, 1, M, s);
 }
 
-extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* rows, int top_k,
+extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, int cols, const int32_t* rows, int top_k,
                                      const int32_t* offsets, int E, const void* codes_t,
                                      const void* scale_t, const void* sal_t, void* y, int dtype,
                                      int slots, int x_rows, int N, int n_out, int Kp, int S_pad, int Gw,
@@ -403,12 +404,12 @@ extern "C" int sqmp_expert_linear_w4(const void* x, long ldx, const int32_t* row
   // gated: blocks of 16 gate and 16 up rows, n_out of the outputs kept
   if (act != w4::ACT_NONE ? (N % 32 || n_out <= N / 2 - 16 || n_out > N / 2) : n_out != N)
     return SQMP_EINVAL;
-  const int st = w4::check_operand(x, ldx, dtype, N, Kp, S_pad, Gw, ngw);
+  const int st = w4::check_operand(x, ldx, cols, dtype, N, Kp, S_pad, Gw, ngw);
   if (st != SQMP_OK) return st;
   if (slots == 0) return SQMP_OK;
   w4::GemvArgs a{};
   a.x = x, a.ldx = ldx, a.codes = (const uint32_t*)codes_t, a.scale = scale_t, a.sal = sal_t;
-  a.y = y, a.N = N, a.n_out = n_out, a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw;
+  a.y = y, a.N = N, a.n_out = n_out, a.Kp = Kp, a.S_pad = S_pad, a.Gw = Gw, a.ngw = ngw, a.nk = cols / 64;
   a.rows = rows, a.offsets = offsets, a.top_k = top_k;
   w4::set_groups(a);
   hipStream_t s = (hipStream_t)stream;

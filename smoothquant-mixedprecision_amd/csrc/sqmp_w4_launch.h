@@ -16,6 +16,7 @@ struct GemvArgs {
   void* y;                // D [M][N_out]
   int M, N;               // rows (dense form); weight rows (gated: gate and up rows together)
   int Kp, S_pad, Gw, ngw;
+  int nk;                  // stages of codes that x holds: Kp / 64, or fewer (the rest is padding)
   // x in an order of its own (STAGE): operand position p is column amap[p] (< 0: zero), position
   // Kp + j the column salient[j], j < S
   const int32_t *amap, *salient;

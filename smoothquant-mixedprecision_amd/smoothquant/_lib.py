@@ -97,13 +97,13 @@ SIGNATURES = {
     "sqmp_gemm_h2d": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp]),
     "sqmp_gemv_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "sqmp_gemv_gathers": (_i, [_i, _i, _i, _i]),
-    "sqmp_gemv_w4": (_i, [_vp, _l, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
+    "sqmp_gemv_w4": (_i, [_vp, _l, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
                           _i, _vp, _sz, _vp]),
     "sqmp_expert_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "sqmp_route_workspace_bytes": (_sz, [_i, _i]),
     "sqmp_route": (_i, [_vp, _l, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "sqmp_plan_routes": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "sqmp_expert_linear_w4": (_i, [_vp, _l, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i,
+    "sqmp_expert_linear_w4": (_i, [_vp, _l, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i,
                                    _i, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "sqmp_combine": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "sqmp_pack_rows": (_i, [_vp, _l, _i, _i, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _l, _vp,

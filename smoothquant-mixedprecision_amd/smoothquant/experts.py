@@ -144,7 +144,7 @@ class PackedExperts:
     ngw: int
     dtype: torch.dtype
     gated: bool
-    identity: bool                   # the operand is x itself (columns' order, K == Kp)
+    identity: bool                   # the operand is x itself (columns' order, K % 64 == 0)
 
 
 def _interleave(t: torch.Tensor) -> torch.Tensor:
@@ -179,8 +179,8 @@ def _pack_all(weights, E: int, rows: int, gated: bool) -> PackedExperts:
     amap = torch.stack(maps)
     if bool((amap == amap[0]).all()):  # (also on the first use of another stream: a sync)
         amap = amap[0].contiguous()
-        pe.identity = pe.S == 0 and pe.Kp == pe.K and bool(
-            torch.equal(amap, torch.arange(pe.K, dtype=torch.int32, device=amap.device)))
+        pe.identity = pe.S == 0 and pe.K % 64 == 0 and bool(
+            torch.equal(amap[:pe.K], torch.arange(pe.K, dtype=torch.int32, device=amap.device)))
     pe.amap = amap
     return pe
 
@@ -234,16 +234,16 @@ def pack_expert_codes(codes: torch.Tensor, scales: torch.Tensor, group_size: int
     one = ops.tile_major(pw.codes, pw.wscale, pw.wsal, E * pad, pw.Kp, 0, pw.ngw, pw.dtype)
     return PackedExperts(one[0].view(E, -1), one[1].view(E, -1), None, pw.amap, None, E,
                          n_rows // 2 if gated else n_rows, N, K, pw.Kp, 0, 0, pw.Gw, pw.ngw,
-                         pw.dtype, gated, pw.Kp == K)
+                         pw.dtype, gated, K % 64 == 0)
 
 
 # ------------------------------------------------------------------ products
 def _operand(x: torch.Tensor, pe: PackedExperts, r: Routing, by_slot: bool):
-    """(operand, its slot -> pair list or None): x itself where the kernels can read it, a packed
+    """(operand, its slot -> pair list or None, its coded columns): x itself where the kernels can read it, a packed
     copy of its rows, or -- where every expert has its own column order -- of every slot's row."""
     rows = None if by_slot else r.rows
-    if pe.identity and ops._operand_rows(x, pe.Kp):
-        return x, rows
+    if pe.identity and ops._operand_rows(x, pe.K):
+        return x, rows, pe.K
     if x.stride(1) != 1 or x.stride(0) == 0:  # (0: rows of an expanded tensor)
         x = x.contiguous()
     own = pe.amap.dim() == 2
@@ -257,7 +257,7 @@ def _operand(x: torch.Tensor, pe: PackedExperts, r: Routing, by_slot: bool):
                                    ops._raw_stream(x.device.index))
     if status:
         check(status, "pack_rows")
-    return out, None if own else rows
+    return out, None if own else rows, pe.Kp
 
 
 @ops.on_tensor_device
@@ -285,12 +285,12 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
         raise ValueError(f"expert_linear: out must be contiguous {pe.dtype} [{S}, {pe.n_out}] on {dev}")
     if S == 0:
         return out
-    a, pairs = _operand(x, pe, routing, by_slot)
+    a, pairs, cols = _operand(x, pe, routing, by_slot)
     lib, dt = load(), ops.DTYPE_CODE[pe.dtype]
     n = ops.workspace_bytes("expert", dt, pe.num_experts, S, pe.N, pe.Kp)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     status = lib.sqmp_expert_linear_w4(
-        a.data_ptr(), a.stride(0) if a.shape[0] > 1 else pe.Kp + pe.S_pad, _ptr(pairs),
+        a.data_ptr(), a.stride(0) if a.shape[0] > 1 else pe.Kp + pe.S_pad, cols, _ptr(pairs),
         routing.ids.shape[1], routing.offsets.data_ptr(), pe.num_experts, pe.codes_t.data_ptr(),
         pe.scale_t.data_ptr(), _ptr(pe.sal_t), out.data_ptr(), dt, S, a.shape[0], pe.N, pe.n_out,
         pe.Kp, pe.S_pad, pe.Gw, pe.ngw, code, _ptr(ws), n, ops._raw_stream(dev.index))

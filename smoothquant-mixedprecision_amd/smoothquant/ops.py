@@ -1170,24 +1170,26 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
     ld, s1 = x.stride()
     xp = x.data_ptr()
     amap = sal = None
-    if (packed or ident) and s1 == 1 and xp % 16 == 0 and (M == 1 or (ld >= L and ld % per == 0)):
+    cols = pw.Kp if packed else ident or pw.Kp
+    if (packed or ident) and s1 == 1 and xp % 16 == 0 and (M == 1 or (ld >= C and ld % per == 0)):
         if M == 1:
             ld = L
     elif packed:
         x = x.clone(memory_format=torch.contiguous_format)
         xp, ld = x.data_ptr(), L
     elif s1 == 1 and ld > 0 and lib.sqmp_gemv_gathers(code, M, pw.Kp, pw.S_pad):
+        cols = pw.Kp
         amap, sal = pw.amap.data_ptr(), None if pw.salient is None else pw.salient.data_ptr()
     else:
         x = pack_rows.__wrapped__(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
-        xp, ld = x.data_ptr(), L
+        xp, ld, cols = x.data_ptr(), L, pw.Kp
     wp, wn = None, 0
     if M > 32:
         wn = workspace_bytes("gemv", code, M, N, pw.Kp)
         if wn:
             ws = torch.empty(wn, dtype=torch.uint8, device=device)
             wp = ws.data_ptr()
-    status = lib.sqmp_gemv_w4(xp, ld, amap, sal, pw.S, codes_t, scale_t, sal_t, bp, y.data_ptr(),
+    status = lib.sqmp_gemv_w4(xp, ld, cols, amap, sal, pw.S, codes_t, scale_t, sal_t, bp, y.data_ptr(),
                               code, M, N, *tail, wp, wn, _raw_stream(device.index))
     if status:
         check(status, "gemv")
@@ -1202,6 +1204,19 @@ def _gemv_refuse(x: torch.Tensor, dtype: torch.dtype, device: torch.device):
     raise RuntimeError(f"gemv: x on {x.device}, the weight on {device}")
 
 
+def own_columns(pw: PackedWeight):
+    """K where x's rows are the operand as they are -- the identity order, no salient columns, whole
+    64-position stages --, 0 where not, None where a capture forbids to look."""
+    if pw.S or pw.S_pad or pw.K % 64:
+        return 0
+    if pw.ident:
+        return pw.K
+    if torch.cuda.is_current_stream_capturing():
+        return None
+    arange = torch.arange(pw.K, dtype=torch.int32, device=pw.amap.device)
+    return pw.K if torch.equal(pw.amap[:pw.K], arange) else 0
+
+
 def _gemv_args(pw: PackedWeight):
     """gemv's arguments that depend on the weight alone; kept on it once its operands and order are
     known for good (not inside a capture)."""
@@ -1209,12 +1224,12 @@ def _gemv_args(pw: PackedWeight):
         raise ValueError(f"gemv: needs 4-bit codes in groups of a multiple of 8 columns (n_bits "
                          f"{pw.n_bits}, group {pw.Gw})")
     t = gemv_operands(pw)
-    ident = identity_layout(pw)
+    ident = own_columns(pw)
     dev = pw.codes.device
     a = (pw.dtype, dev, _dtype_code(pw.dtype), pw.Kp + pw.S_pad, pw.K,
          4 if pw.dtype == torch.float32 else 8, ident, t[0].data_ptr(), t[1].data_ptr(),
          t[2].data_ptr() if pw.S_pad else None, pw.N, (pw.Kp, pw.S_pad, pw.Gw, pw.ngw))
-    if pw.gemv is t and pw.ident is not None:
+    if pw.gemv is t and ident is not None:
         pw.gemv_args = a
     else:
         a = a[:7] + (_Keep(t, a[7]), _Keep(t, a[8]), None if a[9] is None else _Keep(t, a[9])) + a[10:]

@@ -16,14 +16,15 @@ def lib():
 
 
 def test_gemv_refusals(lib):
-    def call(x=P, ldx=128, amap=None, salient=None, S=0, codes=P, scale=P, sal=None, bias=None, y=P, dtype=1,
+    def call(x=P, ldx=128, cols=None, amap=None, salient=None, S=0, codes=P, scale=P, sal=None, bias=None, y=P, dtype=1,
              M=1, N=32, Kp=128, S_pad=0, Gw=64, ngw=2):
-        return lib.sqmp_gemv_w4(x, ldx, amap, salient, S, codes, scale, sal, bias, y, dtype, M, N, Kp, S_pad, Gw, ngw, None, 0, None)
-    assert call(M=0) == 0                                   # nothing to do
+        return lib.sqmp_gemv_w4(x, ldx, Kp if cols is None else cols, amap, salient, S, codes, scale, sal, bias, y, dtype, M, N, Kp, S_pad, Gw, ngw, None, 0, None)
+    assert call(M=0) == 0 and call(M=0, cols=64, ldx=64) == 0   # nothing to do
     for bad in (dict(x=None), dict(codes=None), dict(scale=None), dict(y=None), dict(S_pad=64, ldx=192),
                 dict(M=-1), dict(M=65), dict(N=0), dict(Kp=64), dict(Kp=100), dict(S_pad=-64),
                 dict(S_pad=32, sal=P), dict(Gw=0), dict(ngw=0), dict(ldx=127), dict(ldx=132),
-                dict(x=P + 2), dict(ldx=64)):
+                dict(x=P + 2), dict(ldx=64), dict(cols=32), dict(cols=192), dict(cols=0), dict(cols=-64),
+                dict(cols=64, S_pad=64, sal=P, ldx=192), dict(cols=64, ldx=56), dict(cols=64, amap=P)):
         assert call(**bad) == -1, bad
     assert call(dtype=3) == -2
     assert call(Gw=12) == -2                                # groups of whole 8 positions only
@@ -37,9 +38,9 @@ def test_gemv_refusals(lib):
 
 
 def test_expert_linear_refusals(lib):
-    def call(x=P, ldx=128, rows=None, top_k=2, offsets=P, E=4, codes=P, scale=P, sal=None, y=P, dtype=1, slots=8,
+    def call(x=P, ldx=128, cols=None, rows=None, top_k=2, offsets=P, E=4, codes=P, scale=P, sal=None, y=P, dtype=1, slots=8,
              x_rows=4, N=32, n_out=32, Kp=128, S_pad=0, Gw=64, ngw=2, act=0):
-        return lib.sqmp_expert_linear_w4(x, ldx, rows, top_k, offsets, E, codes, scale, sal, y, dtype, slots,
+        return lib.sqmp_expert_linear_w4(x, ldx, Kp if cols is None else cols, rows, top_k, offsets, E, codes, scale, sal, y, dtype, slots,
                                          x_rows, N, n_out, Kp, S_pad, Gw, ngw, act, None, 0, None)
     assert call(slots=0) == 0
     for bad in (dict(x=None), dict(offsets=None), dict(y=None), dict(E=0), dict(E=65536), dict(top_k=0),

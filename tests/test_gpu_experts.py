@@ -170,7 +170,8 @@ def plain_experts(x, w, r, by_slot):
 SHAPES = [(1, 8, 2, 64, 128, 64), (9, 3, 1, 33, 100, 32), (130, 5, 3, 96, 256, 64),
           (300, 40, 6, 50, 192, 64), (40, 2, 2, 300, 1000, 8), (1100, 4, 2, 264, 384, 128),
           (500, 2, 1, 130, 256, 32), (256, 1, 1, 257, 128, 64), (777, 3, 3, 512, 640, 640),
-          (260, 256, 4, 16, 128, 128), (330, 3, 1, 512, 2048, 128), (64, 8, 2, 96, 4096, 64)]
+          (260, 256, 4, 16, 128, 128), (330, 3, 1, 512, 2048, 128), (64, 8, 2, 96, 4096, 64), (300, 2, 1, 64, 64, 64),
+          (700, 3, 2, 288, 1344, 64), (9, 4, 2, 64, 448, 32), (400, 2, 1, 130, 4160, 128)]
 
 
 @pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])

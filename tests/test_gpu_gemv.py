@@ -20,7 +20,8 @@ def _int_case(M, N, K, G, dt, seed):
 @pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 32, 33, 49, 64])
 @pytest.mark.parametrize("N,K,G", [(32, 128, 64), (40, 192, 32), (257, 1000, 8), (1, 64, 64),
-                                   (33, 1, 128), (96, 2304, 256), (2600, 256, 64), (22500, 192, 64)])
+                                   (33, 1, 128), (96, 2304, 256), (2600, 256, 64), (22500, 192, 64),
+                                   (64, 64, 64), (70, 448, 32), (40, 1344, 192)])
 def test_exact_sums(M, N, K, G, dt):
     x, codes, scales, pw = _int_case(M, N, K, G, DT[dt], M * 1000 + N)
     want = (x.double() @ values(codes, scales, G).T).float().to(DT[dt])
