@@ -13,24 +13,12 @@ in elementary torch operations, and the calls a user makes of this framework's k
 `own` selects the framework's kernels; `run` takes what `prepare` gives either way.
 """
 import math
-import os
-import sys
 
 import torch
 
 own = False
 
 DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
-
-
-def _kernels():
-    """The framework's modules with the operators (its folder is no package name: the path of it
-    is what a user exports as PYTHONPATH)."""
-    path = os.path.abspath("smoothquant-mixedprecision_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
-    from smoothquant import experts, ops
-    return ops, experts
 
 
 # ---------------------------------------------------------------------------------- cases
@@ -161,7 +149,7 @@ def prepare(case, seed):
         st["scales"] = _scales((N, -(-K // c["G"])), g, dev, dt)
         st["bias"] = torch.randn(N, generator=g, device=dev).to(dt) if c["bias"] else None
         if own:
-            ops, _ = _kernels()
+            from smoothquant import ops
             st["w"] = ops.pack_codes(st.pop("codes"), st.pop("scales"), c["G"])
         return st
     logits = _logits(c, g, dev)
@@ -184,7 +172,7 @@ def prepare(case, seed):
         st["codes"] = _codes((E, N, c["K"]), g, dev)
         st["scales"] = _scales((E, N, -(-c["K"] // c["G"])), g, dev, dt)
     if own:
-        _, experts = _kernels()
+        from smoothquant import experts
         st["routing"] = experts.plan_routes(ids, wts, E)
         if c["op"] == "experts":
             st["w"] = experts.pack_expert_codes(st.pop("codes"), st.pop("scales"), c["G"],
@@ -219,7 +207,7 @@ def run(st):
 
 
 def _run_own(st, c):
-    ops, experts = _kernels()
+    from smoothquant import experts, ops
     if c["op"] == "gemv":
         return ops.gemv(st["x"], st["w"], st["bias"])
     if c["op"] == "route":
