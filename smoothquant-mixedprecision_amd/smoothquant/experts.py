@@ -278,7 +278,8 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
             or x.shape[0] != (S if by_slot else routing.ids.shape[0]) or x.shape[1] != pe.K
             or x.dtype is not pe.dtype or dev != pe.codes_t.device or routing.rows.device != dev):
         _expert_refuse(x, pe, routing, act, rows)
-    if out is None:
+    given = out is not None
+    if not given:
         out = x.new_empty((S, pe.n_out))
     elif (tuple(out.shape) != (S, pe.n_out) or out.dtype != pe.dtype or out.device != dev
           or not out.is_contiguous()):
@@ -296,7 +297,7 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
         pe.Kp, pe.S_pad, pe.Gw, pe.ngw, code, _ptr(ws), n, ops._raw_stream(dev.index))
     if status:
         check(status, "expert_linear")
-    return out
+    return ops.written(out) if given else out
 
 
 def _expert_refuse(x, pe, routing, act, rows):
@@ -337,7 +338,8 @@ def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = Non
     if not z.is_contiguous():
         z = z.contiguous()
     H = z.shape[1]
-    if out is None:
+    given = out is not None
+    if not given:
         out = z.new_empty((T, H))
     elif (tuple(out.shape) != (T, H) or out.dtype != z.dtype or out.device != dev
           or not out.is_contiguous()):
@@ -349,7 +351,7 @@ def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = Non
                                  ops._raw_stream(dev.index))
     if status:
         check(status, "combine")
-    return out
+    return ops.written(out) if given else out
 
 
 # ------------------------------------------------------------------ the module

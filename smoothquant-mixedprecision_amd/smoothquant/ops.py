@@ -60,6 +60,14 @@ def on_tensor_device(fn):
     return call
 
 
+def written(t: torch.Tensor) -> torch.Tensor:
+    """t, after a kernel wrote it through its address: its version counter rises as for a write of
+    torch's own, so that what is kept for its former contents (statistics, operands and outputs of
+    layers on the same tensor) is not used for the new ones."""
+    torch.autograd.graph.increment_version(t)
+    return t
+
+
 def _require_gpu(t: torch.Tensor, what: str):
     if t.device.type != "cuda":
         raise RuntimeError(
@@ -1067,6 +1075,8 @@ def tile_major(codes: torch.Tensor, wscale: torch.Tensor, wsal: torch.Tensor, N:
     check(load().sqmp_pack_fq7(_p(codes), _p(wscale), _p(wsal) if S_pad else None,
                                _dtype_code(dtype), N, Kp, S_pad, ngw, 2, *[_p(t) for t in out],
                                _stream(codes)), "pack_fq7")
+    for t in out:
+        written(t)
     return out
 
 

@@ -1,0 +1,86 @@
+"""The expert calls up to their kernels, without a GPU: host tensors that say they are on one, and a
+library that records the calls and does nothing."""
+import pytest
+import torch
+
+from smoothquant import experts, ops
+
+CUDA0 = torch.device("cuda", 0)
+
+
+class OnGpu(torch.Tensor):
+    """A host tensor that says that it is on the first GPU."""
+    is_cuda = True
+    device = CUDA0
+
+
+def gpu(t):
+    return t.as_subclass(OnGpu)
+
+
+class Library:
+    """Every entry succeeds; the calls are kept."""
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.calls.append((name, args))
+            return 0
+        return entry
+
+
+@pytest.fixture
+def library(monkeypatch):
+    lib = Library()
+    for m in (ops, experts):
+        monkeypatch.setattr(m, "load", lambda: lib)
+    monkeypatch.setattr(ops, "_SPLIT_WS", {})
+    monkeypatch.setattr(ops, "_current_device", lambda: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 0)
+    return lib
+
+
+def routing(T=4, k=2, E=3, dtype=torch.int32):
+    i32 = dict(dtype=dtype)
+    return experts.Routing(gpu(torch.zeros(T, k, **i32)), gpu(torch.ones(T, k)),
+                           gpu(torch.zeros(E + 1, **i32)), gpu(torch.zeros(T * k, **i32)),
+                           gpu(torch.zeros(T * k, **i32)), E)
+
+
+def weight(E=3, N=32, K=128, dtype=torch.float16):
+    return experts.PackedExperts(gpu(torch.zeros(E, 256, dtype=torch.uint8)), gpu(torch.zeros(E, 64, dtype=dtype)),
+                                 None, gpu(torch.arange(K, dtype=torch.int32)), None, E, N, N, K, K, 0, 0,
+                                 64, K // 64, dtype, False, True)
+
+
+def test_out_is_a_write_that_torch_sees(library):
+    """A kernel writes `out` through its address; its version counter, by which results kept for a
+    tensor are told from those for its former contents, has to rise as for a write of torch's own."""
+    r = routing()
+    base = torch.zeros(9, 64, dtype=torch.float16)
+    y = gpu(base[1:5])                                       # a view: one counter with its base
+    was = base._version
+    assert experts.combine(gpu(torch.zeros(8, 64, dtype=torch.float16)), r, out=y) is y
+    assert y._version > was and base._version > was
+    z = gpu(torch.zeros(8, 32, dtype=torch.float16))
+    was = z._version
+    assert experts.expert_linear(gpu(torch.zeros(4, 128, dtype=torch.float16)), weight(), r, out=z) is z
+    assert z._version > was
+    assert [c[0] for c in library.calls if "workspace" not in c[0]] == ["sqmp_combine", "sqmp_expert_linear_w4"]
+    was = z._version
+    with pytest.raises(ValueError):                          # refused: nothing written
+        experts.expert_linear(gpu(torch.zeros(4, 128, dtype=torch.float16)), weight(), r, act="silu", out=z)
+    assert z._version == was
+    with torch.inference_mode():                             # (tensors without a counter)
+        o = gpu(torch.zeros(4, 64, dtype=torch.float16))
+        assert experts.combine(gpu(torch.zeros(8, 64, dtype=torch.float16)), r, out=o) is o
+
+
+def test_packed_operands_written_into_tensors_of_the_caller(library, monkeypatch):
+    monkeypatch.setattr(ops, "_stream", lambda t: None)
+    out = tuple(gpu(torch.zeros(0, dtype=d)) for d in (torch.uint8, torch.float16, torch.float16))
+    was = [t._version for t in out]
+    ops.tile_major(gpu(torch.zeros(1, dtype=torch.uint8)), gpu(torch.zeros(1).half()), gpu(torch.zeros(1).half()),
+                   32, 128, 0, 2, torch.float16, out)
+    assert all(t._version > v for t, v in zip(out, was))
