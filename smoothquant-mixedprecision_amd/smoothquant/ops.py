@@ -120,13 +120,19 @@ class PackedWeight:
     sal_key: Optional[tuple] = field(default=None)        # identity of the salient set (host)
     w8: Optional[torch.Tensor] = field(default=None)     # uint8 [Np, Kp] e4m3 codes (f8 GEMM)
     ws32: Optional[torch.Tensor] = field(default=None)   # fp32 [ngw, Np] scales (f8 GEMM)
-    fq7: Optional[tuple] = field(default=None)           # (codes_t, scale_t, sal_t, J) of gemm_fq7
+    # (codes_t, scale_t, sal_t, J) of gemm_fq7; like gemv's below derived from the codes and not
+    # handed to the copy that dataclasses.replace makes, whose codes may be others
+    fq7: Optional[tuple] = field(default=None, init=False)
     h2: Optional[tuple] = field(default=None)            # (f16 [2, Np, L], int32 [Np]) (gemm_h2)
     h2d: Optional[torch.Tensor] = field(default=None)    # f16 tile-major planes (gemm_h2d)
     sib_maps: Optional[tuple] = field(default=None)      # sibling position map (sqmp_permute_act)
     ident: Optional[bool] = field(default=None)          # packed order == column order (identity_layout)
-    gemv: Optional[tuple] = field(default=None)          # (codes_t, scale_t, sal_t) of gemv
-    gemv_args: Optional[tuple] = field(default=None)     # what gemv passes for this weight
+    gemv: Optional[tuple] = field(default=None, init=False)       # (codes_t, scale_t, sal_t) of gemv
+    gemv_args: Optional[tuple] = field(default=None, init=False)  # what gemv passes for this weight
+
+    def __getstate__(self):
+        """Copies and pickles (another device, another process) gather gemv's arguments anew."""
+        return dict(self.__dict__, gemv_args=None)
 
     @property
     def gemm_operand(self):
@@ -1156,7 +1162,7 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
     are few, else copied first (sqmp_pack_rows)."""
     if not x.is_cuda:
         _require_gpu(x, "gemv")
-    dtype, device, code, L, K, per, ident, codes_t, scale_t, sal_t, N, tail = (
+    dtype, device, code, L, K, per, ident, (codes_t, scale_t, sal_t), N, tail = (
         pw.gemv_args or _gemv_args(pw))
     if x.dim() != 2 or x.dtype is not dtype or x.device != device:
         _gemv_refuse(x, dtype, device)
@@ -1199,8 +1205,9 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
         if wn:
             ws = torch.empty(wn, dtype=torch.uint8, device=device)
             wp = ws.data_ptr()
-    status = lib.sqmp_gemv_w4(xp, ld, cols, amap, sal, pw.S, codes_t, scale_t, sal_t, bp, y.data_ptr(),
-                              code, M, N, *tail, wp, wn, _raw_stream(device.index))
+    status = lib.sqmp_gemv_w4(xp, ld, cols, amap, sal, pw.S, codes_t.data_ptr(), scale_t.data_ptr(),
+                              sal_t.data_ptr() if pw.S_pad else None, bp, y.data_ptr(), code, M, N,
+                              *tail, wp, wn, _raw_stream(device.index))
     if status:
         check(status, "gemv")
     return y
@@ -1228,8 +1235,8 @@ def own_columns(pw: PackedWeight):
 
 
 def _gemv_args(pw: PackedWeight):
-    """gemv's arguments that depend on the weight alone; kept on it once its operands and order are
-    known for good (not inside a capture)."""
+    """gemv's arguments that depend on the weight alone (its operands as tensors: a call takes their
+    addresses); kept on it once its operands and order are known for good (not inside a capture)."""
     if not gemv_eligible(pw):
         raise ValueError(f"gemv: needs 4-bit codes in groups of a multiple of 8 columns (n_bits "
                          f"{pw.n_bits}, group {pw.Gw})")
@@ -1237,18 +1244,7 @@ def _gemv_args(pw: PackedWeight):
     ident = own_columns(pw)
     dev = pw.codes.device
     a = (pw.dtype, dev, _dtype_code(pw.dtype), pw.Kp + pw.S_pad, pw.K,
-         4 if pw.dtype == torch.float32 else 8, ident, t[0].data_ptr(), t[1].data_ptr(),
-         t[2].data_ptr() if pw.S_pad else None, pw.N, (pw.Kp, pw.S_pad, pw.Gw, pw.ngw))
+         4 if pw.dtype == torch.float32 else 8, ident, t, pw.N, (pw.Kp, pw.S_pad, pw.Gw, pw.ngw))
     if pw.gemv is t and ident is not None:
         pw.gemv_args = a
-    else:
-        a = a[:7] + (_Keep(t, a[7]), _Keep(t, a[8]), None if a[9] is None else _Keep(t, a[9])) + a[10:]
     return a
-
-
-class _Keep(int):
-    """A pointer that holds the tensors it points into (operands that nothing else keeps)."""
-    def __new__(cls, owner, ptr):
-        self = super().__new__(cls, ptr)
-        self.owner = owner
-        return self

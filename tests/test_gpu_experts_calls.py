@@ -40,3 +40,30 @@ def test_a_buffer_written_again_between_two_layers(linked):
     a(experts.expert_linear(x[0], pe, r, out=buf))
     got = b(experts.expert_linear(x[1], pe, r, out=buf))
     assert torch.equal(got, b(buf.clone()))
+
+
+def test_copies_of_a_layer_after_its_original_is_gone(tmp_path):
+    """Layers copied and saved after they ran on few rows, from a state dict too: each computes from its
+    own weight (the original's is overwritten, then freed)."""
+    import copy
+    D = torch.float16
+    src, = _layers(1, 128, 96, D)
+    loaded, = _layers(1, 128, 96, D)
+    loaded.load_state_dict(src.state_dict())
+    x = torch.randn(3, 128, device="cuda").to(D)
+    for q in (src, loaded):
+        q.kernel = "gemv"
+        want = q(x.clone())
+        pw = q.packed()
+        assert pw.gemv_args is not None
+        f = str(tmp_path / "q.pt")
+        torch.save(q, f)
+        others = [copy.deepcopy(q), torch.load(f, weights_only=False), copy.deepcopy(pw)]
+        for t in pw.gemv:
+            t.zero_()
+        assert torch.equal(q(x.clone()), q.bias.reshape(1, -1).expand(3, -1).to(D))   # (what a copy must not see)
+        del q, pw
+        a = ops.quant_act_fp(x, others[2], "per_group", 4, 32)
+        y = ops.gemv(a, others[2], others[0].bias, packed=True)
+        for got in (others[0](x.clone()), others[1](x.clone()), y):
+            assert torch.equal(got, want)
