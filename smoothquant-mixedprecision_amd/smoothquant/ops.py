@@ -60,6 +60,14 @@ def on_tensor_device(fn):
     return call
 
 
+def _keep(pw, name: str, value):
+    """value, kept as pw.<name> for later calls -- not inside a HIP-graph capture, where what was
+    built is written at the graph's replays only."""
+    if not torch.cuda.is_current_stream_capturing():
+        setattr(pw, name, value)
+    return value
+
+
 def written(t: torch.Tensor) -> torch.Tensor:
     """t, after a kernel wrote it through its address: its version counter rises as for a write of
     torch's own, so that what is kept for its former contents (statistics, operands and outputs of
@@ -329,8 +337,7 @@ def _sibling_map(src: PackedWeight, dst: PackedWeight) -> torch.Tensor:
         return c[2]
     col = dst.amap.long()
     m = torch.where(col >= 0, src.posmap.long()[col.clamp(min=0)], -1).to(torch.int32)
-    dst.sib_maps = (weakref.ref(src), ver, m)  # one source per layer (its sibling leader)
-    return m
+    return _keep(dst, "sib_maps", (weakref.ref(src), ver, m))[2]  # one source per layer (its leader)
 
 
 def _sibling_ok(src: PackedWeight, dst: PackedWeight) -> bool:
@@ -378,9 +385,9 @@ def quant_act_fp(x2: torch.Tensor, pw: PackedWeight, act_quant: str, n_bits: int
                 and la[1] == skey + (n_bits, group_size)
                 and la[2]() is not None and _sibling_ok(la[2](), pw)):
             # a sibling of the layer that produced la[3] on this same input
-            check(lib.sqmp_permute_act(_p(la[3]), _p(a), _p(_sibling_map(la[2](), pw)),
-                                       _dtype_code(x2.dtype), M, pw.Kp, pw.S_pad,
-                                       ctypes.c_void_p(stream)), "permute_act")
+            moves = _sibling_map(la[2](), pw)
+            check(lib.sqmp_permute_act(_p(la[3]), _p(a), _p(moves), _dtype_code(x2.dtype), M, pw.Kp,
+                                       pw.S_pad, ctypes.c_void_p(stream)), "permute_act")
             return a
         st = e["stats"]
         # only a DIFFERENT layer on the same input reuses them: calling one layer again
@@ -465,9 +472,10 @@ def gemm_fq7_group(As, pws, biases):
     p0 = pws[0]
     n = len(pws)
     probs = (_lib.Fq7Problem * n)()
-    ys = []
+    ys, held = [], []  # (operands that a capture builds live in this call alone)
     for o, (a, pw, b) in enumerate(zip(As, pws, biases)):
-        bt, st, salt, J = fq7_operands(pw)
+        held.append(fq7_operands(pw))
+        bt, st, salt, J = held[-1]
         y = torch.empty((M, pw.N), dtype=pw.dtype, device=a.device)
         ys.append(y)
         _require_gpu(a, "gemm_fq7_group")
@@ -717,7 +725,7 @@ def fq7_eligible(pw: PackedWeight) -> bool:
 
 
 def fq7_operands(pw: PackedWeight):
-    """(codes_t, scale_t, sal_t) of gemm_fq7: tile-major copies of the packed weight, built
+    """(codes_t, scale_t, sal_t, J) of gemm_fq7: tile-major copies of the packed weight, built
     once per packed weight."""
     if pw.fq7 is None or pw.fq7[3] != FQ7_J:
         sizes = [ctypes.c_size_t() for _ in range(3)]
@@ -730,7 +738,7 @@ def fq7_operands(pw: PackedWeight):
         check(load().sqmp_pack_fq7(_p(pw.codes), _p(pw.wscale), _p(pw.wsal) if pw.S_pad else None,
                                    _dtype_code(pw.dtype), pw.N, pw.Kp, pw.S_pad, pw.ngw, FQ7_J,
                                    _p(bt), _p(st), _p(salt), _stream(pw.codes)), "pack_fq7")
-        pw.fq7 = (bt, st, salt, FQ7_J)
+        return _keep(pw, "fq7", (bt, st, salt, FQ7_J))
     return pw.fq7
 
 
@@ -770,7 +778,7 @@ def h2_operand(pw: PackedWeight):
         bexp = torch.empty(Np, dtype=torch.int32, device=full.device)
         check(load().sqmp_split2_f16(_p(full), pw.N, L, Np, _p(planes), _p(bexp), _stream(full)),
               "split2_f16")
-        pw.h2 = (planes, bexp)
+        return _keep(pw, "h2", (planes, bexp))
     return pw.h2
 
 
@@ -788,7 +796,7 @@ def h2d_operand(pw: PackedWeight) -> torch.Tensor:
         wt = torch.empty_like(planes)
         check(load().sqmp_pack_h2d(_p(planes), planes.shape[1], planes.shape[2], _p(wt),
                                    _stream(planes)), "pack_h2d")
-        pw.h2d = wt
+        return _keep(pw, "h2d", wt)
     return pw.h2d
 
 
@@ -898,19 +906,20 @@ def _ws32(pw: PackedWeight) -> torch.Tensor:
         ws32 = torch.empty((pw.ngw, pad_n(pw.N)), dtype=torch.float32, device=pw.codes.device)
         check(load().sqmp_pack_f8(_p(pw.codes), _p(pw.wscale), _dtype_code(pw.dtype), pw.N,
                                   pw.Kp, pw.ngw, None, _p(ws32), _stream(pw.codes)), "pack_f8")
-        pw.ws32 = ws32
+        return _keep(pw, "ws32", ws32)
     return pw.ws32
 
 
 def f8_operands(pw: PackedWeight):
     """(w8, ws32) of the f8 GEMM, built once per packed weight."""
+    ws32 = _ws32(pw)
     if pw.w8 is None:
         w8 = torch.empty((pad_n(pw.N), pw.Kp), dtype=torch.uint8, device=pw.codes.device)
         check(load().sqmp_pack_f8(_p(pw.codes), _p(pw.wscale), _dtype_code(pw.dtype), pw.N,
-                                  pw.Kp, pw.ngw, _p(w8), _p(_ws32(pw)), _stream(pw.codes)),
+                                  pw.Kp, pw.ngw, _p(w8), _p(ws32), _stream(pw.codes)),
               "pack_f8")
-        pw.w8 = w8
-    return pw.w8, _ws32(pw)
+        return _keep(pw, "w8", w8), ws32
+    return pw.w8, ws32
 
 
 def quant_act_f8(x2: torch.Tensor, pw: PackedWeight, act_quant: str, n_bits: int,

@@ -67,3 +67,32 @@ def test_copies_of_a_layer_after_its_original_is_gone(tmp_path):
         y = ops.gemv(a, others[2], others[0].bias, packed=True)
         for got in (others[0](x.clone()), others[1](x.clone()), y):
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("linked", [False, True])
+def test_layers_first_used_in_a_capture(linked):
+    """A prompt captured before any eager call, then a decoding step: the step does not take the
+    operands that only the graph's replays write."""
+    from smoothquant.fake_quant import link_siblings
+    D = torch.float16
+    warm, cold = _layers(2, 128, 96, D), _layers(2, 128, 96, D)
+    if linked:
+        link_siblings(*warm), link_siblings(*cold)
+    x = torch.randn(300, 128, device="cuda").to(D)
+    for q in warm:                                            # (the quantizers' workspaces)
+        q(x)
+    want = [q(x) for q in warm]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = [q(x) for q in cold]
+    step = x[:3].clone()
+    for a, b in zip(warm, cold):
+        a.kernel = b.kernel = "gemv"
+        assert torch.equal(b(step), a(step))
+        a.kernel = b.kernel = "auto"
+        assert torch.equal(b(step), a(step))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, w) for p, w in zip(y, want))
+        assert all(torch.equal(q(x), w) for q, w in zip(cold, want))

@@ -116,3 +116,89 @@ def test_layer_loaded_from_a_state_dict():
     torch.save(loaded, buf)
     buf.seek(0)
     check_copy(src, torch.load(buf, weights_only=False).packed())
+
+
+class Library:
+    """Every entry succeeds and does nothing; the calls are kept."""
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.calls.append((name, args))
+            if name == "sqmp_fq7_sizes":
+                for a, n in zip(args[-3:], (4096, 512, 0)):
+                    a._obj.value = n
+            return 0
+        return entry
+
+
+@pytest.fixture
+def library(monkeypatch):
+    lib = Library()
+    monkeypatch.setattr(ops, "load", lambda: lib)
+    monkeypatch.setattr(ops, "_stream", lambda t: None)
+    monkeypatch.setattr(ops, "_p", lambda t: None)
+    return lib
+
+
+def test_operands_first_built_in_a_capture_are_not_kept(library, monkeypatch):
+    """The copies that a capture builds are written at its replays only: neither gemm_fq7 nor gemv,
+    which share them, may use them outside of it."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    pw = packed()
+    first = ops.fq7_operands(pw)
+    assert pw.fq7 is None and first[3] == ops.FQ7_J
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    t = ops.gemv_operands(pw)
+    assert not {v.data_ptr() for v in t if v.numel()} & {v.data_ptr() for v in first[:3] if v.numel()}
+    kept = ops.fq7_operands(pw)
+    assert pw.fq7 is kept and kept[0] is t[0]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    assert ops.fq7_operands(pw) is kept                       # built before: used
+
+
+@pytest.mark.parametrize("name,build", [
+    ("w8", lambda pw: ops.f8_operands(pw)), ("ws32", lambda pw: ops.f8_operands(pw)),
+    ("h2", lambda pw: ops.h2_operand(pw)), ("h2d", lambda pw: ops.h2d_operand(pw)),
+    ("sib_maps", lambda pw: ops._sibling_map(LEADER, pw))])
+def test_nothing_that_a_capture_builds_is_kept(library, monkeypatch, name, build):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    pw = packed(torch.float32 if name.startswith("h2") else torch.float16)
+    assert build(pw) is not None and getattr(pw, name) is None
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    build(pw)
+    kept = getattr(pw, name)
+    assert kept is not None
+    build(pw)
+    assert getattr(pw, name) is kept
+
+
+LEADER = packed()
+
+
+def test_grouped_products_hold_their_operands_until_the_launch(library, monkeypatch):
+    """In a capture each weight's copies live in the call alone: all of them until the one launch."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(ops, "_require_gpu", lambda *a: None)
+    import weakref
+    born = []
+    build = ops.fq7_operands
+
+    def watched(pw):
+        o = build(pw)
+        born.append(weakref.ref(o[0]))
+        return o
+    monkeypatch.setattr(ops, "fq7_operands", watched)
+    alive = []
+
+    class Lib(Library):
+        def __getattr__(self, name):
+            if name == "sqmp_gemm_fq7_group":
+                return lambda *a: alive.extend(r() is not None for r in born) or 0
+            return super().__getattr__(name)
+    lib = Lib()
+    monkeypatch.setattr(ops, "load", lambda: lib)
+    a = [torch.zeros(4, K, dtype=torch.float16) for _ in range(3)]
+    ops.gemm_fq7_group(a, [packed() for _ in range(3)], [None] * 3)
+    assert alive == [True] * 3
