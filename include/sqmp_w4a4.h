@@ -112,6 +112,8 @@ enum sqmp_act_out {
 
 /* Library identity. */
 const char* sqmp_version(void);
+/* A number that names the graph capture `stream` is in (no two captures share one), 0: in none. */
+unsigned long long sqmp_capture_id(void* stream);
 const char* sqmp_status_string(int status);
 
 /* Host-only geometry of a packed weight (no GPU work).

@@ -2,7 +2,7 @@
 #include "sqmp_common.h"
 
 extern "C" const char* sqmp_version(void) {
-  return "sqmp_w4a4 0.7.0 (gfx950; W4A4 mixed-precision linear, smoothquant-mixedprecision)";
+  return "sqmp_w4a4 0.7.1 (gfx950; W4A4 mixed-precision linear, smoothquant-mixedprecision)";
 }
 
 extern "C" const char* sqmp_status_string(int status) {
@@ -14,4 +14,12 @@ extern "C" const char* sqmp_status_string(int status) {
     case SQMP_EWORKSPACE: return "workspace missing or too small";
     default: return "unknown status";
   }
+}
+
+extern "C" unsigned long long sqmp_capture_id(void* stream) {
+  SQMP_DEVICE_GUARD(stream);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (!stream || hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) return 0;
+  return status == hipStreamCaptureStatusActive ? id + 1 : 0;
 }

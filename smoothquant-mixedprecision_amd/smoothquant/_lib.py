@@ -47,6 +47,7 @@ class Fq7Problem(ctypes.Structure):
 # name -> (restype, argtypes); the authoritative list of exported symbols
 SIGNATURES = {
     "sqmp_version": (ctypes.c_char_p, []),
+    "sqmp_capture_id": (ctypes.c_ulonglong, [_vp]),
     "sqmp_status_string": (ctypes.c_char_p, [_i]),
     "sqmp_weight_geometry": (_i, [_i, _i, _i, _i, _ip, _ip, _ip, _ip]),
     "sqmp_pack_workspace_bytes": (_sz, [_i, _i]),

@@ -653,7 +653,9 @@ class SiblingGroup:
 
     @staticmethod
     def _key(x):
-        return (x.data_ptr(), tuple(x.shape), tuple(x.stride()), x.dtype, x._version)
+        # (the capture: outputs of a graph are written at its replays only)
+        return (x.data_ptr(), tuple(x.shape), tuple(x.stride()), x.dtype, x._version,
+                ops.capture_id(ops._raw_stream(x.device.index)) if x.is_cuda else 0)
 
     @staticmethod
     def _sig(m):

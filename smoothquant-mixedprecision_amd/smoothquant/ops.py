@@ -289,7 +289,10 @@ def _act_workspace(M: int, K: int, Kp: int, device):
 # (allocated zeroed; every call leaves its statistics regions zero), plus the identity of
 # the batch statistics each currently holds (for SQMP_QA_REUSE_STATS).  The region layout
 # depends on (K, Kp), so one workspace per (device, stream, K, Kp): a region one layout
-# leaves non-zero is never a must-be-zero region of another.
+# leaves non-zero is never a must-be-zero region of another.  A HIP-graph capture has
+# workspaces of its own, cleared by every replay: graphs are replayed in any order and on any
+# stream, behind this bookkeeping, and share neither memory nor statistics with each other or with
+# eager calls (the clearing costs a replay 2-3 us per layout).
 _WS = {}
 _SORTED = ("per_group", "per_group_mean3std")
 
@@ -305,15 +308,27 @@ def _ws_bytes(M: int, K: int, Kp: int) -> int:
     return n
 
 
+def capture_id(stream_ptr: int) -> int:
+    """Which HIP-graph capture the stream is in (0: none)."""
+    return load().sqmp_capture_id(stream_ptr) if stream_ptr else 0
+
+
 def _act_ws(device, stream_ptr: int, K: int, Kp: int, nbytes: int, tag: str = "in"):
     # tag "out": the in-place output quantizer has workspaces of its own, so quantizing a
     # layer's output (OPT q/k/v) leaves the input statistics for its sibling layers intact
-    key = (device.index, stream_ptr, K, Kp, tag)
+    capture = capture_id(stream_ptr)
+    key = (device.index, stream_ptr, K, Kp, tag, capture != 0)
     e = _WS.get(key)
-    if e is None or e["buf"].numel() < nbytes:
-        e = {"buf": torch.zeros(nbytes, dtype=torch.uint8, device=device), "stats": None}
+    if e is None or e["buf"].numel() < nbytes or e["capture"] != capture:
+        e = {"buf": torch.zeros(nbytes, dtype=torch.uint8, device=device), "stats": None,
+             "capture": capture}
         _WS[key] = e
     return e
+
+
+def _discard_ws(e):
+    """A failed call may have left the workspace dirty: the next one starts with another."""
+    e["capture"] = None
 
 
 # Sibling operand reuse (sqmp_permute_act): a layer that quantizes the same input as the
@@ -404,7 +419,7 @@ def quant_act_fp(x2: torch.Tensor, pw: PackedWeight, act_quant: str, n_bits: int
                                    _p(aexp) if h2 else None, None, _p(e["buf"]),
                                    e["buf"].numel(), ctypes.c_void_p(stream))
     if status != _lib.SQMP_OK:
-        _WS.pop((x2.device.index, stream, K, pw.Kp, "in"), None)  # it may be left dirty
+        _discard_ws(e)
         check(status, "quant_act")
     if skey is not None:
         e["stats"] = (weakref.ref(stats_of if stats_of is not None else x2), skey,
@@ -454,7 +469,7 @@ def quant_act_fp_group(x2: torch.Tensor, pws, act_quant: str, n_bits: int,
                                       _lib.QA_CLEAN_WS, optr, _p(e["buf"]), e["buf"].numel(),
                                       vp(stream))
     if status != _lib.SQMP_OK:
-        _WS.pop((x2.device.index, stream, K, p0.Kp, "in"), None)  # it may be left dirty
+        _discard_ws(e)
         check(status, "quant_act_group")
     # the workspace's sorted column list now describes x2 (a later sibling call on x2 may
     # reuse it); no operand is kept for sqmp_permute_act
@@ -631,7 +646,7 @@ def quant_act_c4(x2: torch.Tensor, pw: PackedWeight, act_quant: str, n_bits: int
                                    pw.N, pw.Gw, pw.ngw, _p(wp), _p(e["buf"]), e["buf"].numel(),
                                    ctypes.c_void_p(stream))
     if status != _lib.SQMP_OK:
-        _WS.pop((dev.index, stream, K, pw.Kp, "in"), None)
+        _discard_ws(e)
         check(status, "quant_act_c4")
     if act_quant in _SORTED:
         e["stats"] = (weakref.ref(src), skey, pw.codes.data_ptr())
@@ -685,21 +700,17 @@ def fake_quant_inplace(t2: torch.Tensor, act_quant: str, n_bits: int, group_size
     # salient set): with no salient column the list is 0 .. C-1 (build_maps / pack_weight), so
     # every such call on this workspace builds the same table -- consecutive in-place
     # quantizers (the ppl_eval flow's inputs and q/k/v outputs) skip its launch
-    # (SQMP_QA_TABLE_READY).  Never across a HIP-graph capture: a workspace a capture used is
-    # rewritten by every replay, behind this bookkeeping.
+    # (SQMP_QA_TABLE_READY).  Not inside a HIP-graph capture.
     tab = (("list", C) if (S == 0 and M > 0 and act_quant in ("per_token", "per_group_unsorted"))
            else None)
-    capturing = torch.cuda.is_current_stream_capturing()
-    if capturing:
-        e["captured"] = True
-    if tab is not None and not e.get("captured") and e.get("tab") == tab:
+    if tab is not None and not e["capture"] and e.get("tab") == tab:
         flags |= _lib.QA_TABLE_READY
     status = lib.sqmp_quant_act_v2(_p(t2), _dtype_code(t2.dtype), M, C, ACT_MODES[act_quant],
                                    n_bits, group_size, _p(amap_fq), C, _p(nonsal), None, S, 0,
                                    None, flags, _lib.OUT_INPLACE, None, None, None,
                                    _p(e["buf"]), e["buf"].numel(), ctypes.c_void_p(stream))
     if status != _lib.SQMP_OK:
-        _WS.pop((t2.device.index, stream, C, C, "out"), None)
+        _discard_ws(e)
         check(status, "fake_quant")
     e["tab"] = tab  # (any other mode rebuilt or overwrote the table region)
     e["stats"] = None  # the sorted-column list now describes t2, not a layer input
@@ -946,7 +957,7 @@ def quant_act_f8(x2: torch.Tensor, pw: PackedWeight, act_quant: str, n_bits: int
                                    _p(a8), _p(sa), _p(xs), _p(e["buf"]), e["buf"].numel(),
                                    ctypes.c_void_p(stream))
     if status != _lib.SQMP_OK:
-        _WS.pop((x2.device.index, stream, K, pw.Kp, "in"), None)
+        _discard_ws(e)
         check(status, "quant_act")
     if write_x:
         torch.autograd.graph.increment_version(x2)  # (x was rewritten through a raw pointer)

@@ -84,3 +84,43 @@ def test_packed_operands_written_into_tensors_of_the_caller(library, monkeypatch
     ops.tile_major(gpu(torch.zeros(1, dtype=torch.uint8)), gpu(torch.zeros(1).half()), gpu(torch.zeros(1).half()),
                    32, 128, 0, 2, torch.float16, out)
     assert all(t._version > v for t, v in zip(out, was))
+
+
+def test_every_capture_has_its_own_workspaces(library, monkeypatch):
+    """A graph's workspace is cleared inside the graph (it is allocated in its capture) and belongs to
+    it alone: not the eager one of the stream, not that of another capture."""
+    capture = [0]
+    monkeypatch.setattr(ops, "capture_id", lambda stream: capture[0])
+    monkeypatch.setattr(ops, "_WS", {})
+    dev = torch.device("cpu")
+
+    def ws():
+        return ops._act_ws(dev, 7, 64, 128, 1024)
+    eager = ws()
+    eager["stats"] = "of an eager call"
+    capture[0] = 3
+    first = ws()
+    assert first is not eager and first["stats"] is None and ws() is first
+    capture[0] = 4
+    second = ws()
+    assert second is not first and second["buf"].data_ptr() != eager["buf"].data_ptr()
+    capture[0] = 0
+    assert ws() is eager and eager["stats"] == "of an eager call"
+    ops._discard_ws(eager)                                    # after a failure
+    assert ws() is not eager
+
+
+def test_outputs_kept_for_siblings_do_not_leave_their_capture(monkeypatch):
+    from smoothquant.fake_quant import SiblingGroup
+    capture = [0]
+    monkeypatch.setattr(ops, "capture_id", lambda stream: capture[0])
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 7)
+    x = gpu(torch.zeros(2, 8))
+    key = SiblingGroup._key(x)
+    assert SiblingGroup._key(x) == key
+    capture[0] = 3
+    assert SiblingGroup._key(x) != key
+
+
+def test_capture_id_outside_of_a_capture():
+    assert ops.capture_id(0) == 0

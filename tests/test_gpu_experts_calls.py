@@ -96,3 +96,124 @@ def test_layers_first_used_in_a_capture(linked):
         torch.cuda.synchronize()
         assert all(torch.equal(p, w) for p, w in zip(y, want))
         assert all(torch.equal(q(x), w) for q, w in zip(cold, want))
+
+
+def _captured(fn):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fn()
+    return graph, y
+
+
+@pytest.mark.parametrize("kernel", ["gemv", "auto"])
+def test_graphs_of_decoding_steps_share_nothing(kernel):
+    """Graphs of two batch sizes, captured one after the other without a warm-up on the capture's
+    stream: replayed in the other order, in turns, and side by side on two streams."""
+    D, g = torch.float16, gen(4)
+    a, b = _layers(2, 256, 96, D)
+    for q in (a, b):
+        q.kernel = kernel
+    ins = [torch.randn(M, 256, generator=g, device="cuda").to(D) for M in (1, 7)]
+    want = [[(a(x.roll(i, 1)), b(x.roll(i, 1))) for x in ins] for i in range(4)]
+    xs = [x.clone() for x in ins]
+    graphs = [_captured(lambda x=x: (a(x), b(x))) for x in xs]
+
+    def check(i, picks, streams=None):
+        for p in picks:
+            xs[p].copy_(ins[p].roll(i, 1))
+        torch.cuda.synchronize()
+        for n, p in enumerate(picks):
+            with torch.cuda.stream(streams[n] if streams else torch.cuda.current_stream()):
+                graphs[p][0].replay()
+        torch.cuda.synchronize()
+        for p in picks:
+            for got, w in zip(graphs[p][1], want[i][p]):
+                assert torch.equal(got, w)
+    check(1, [1])                                             # the second graph before the first
+    a(ins[0])
+    check(2, [0, 1])
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        check(3, [0, 1], side)
+        check(0, [1, 0], side)
+
+
+def test_a_graph_does_not_take_statistics_from_outside_of_it():
+    """A layer captured alone, after eager calls (and another capture) of its sibling on the same
+    tensor: its graph computes its own statistics and operand of new contents."""
+    D, g = torch.float16, gen(5)
+    a, b = _layers(2, 128, 96, D)
+    x = torch.randn(5, 128, generator=g, device="cuda").to(D)
+    xs = x.clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a(xs), b(xs)
+        a.kernel = b.kernel = "gemv"
+        a(xs), b(xs)
+    torch.cuda.synchronize()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first, stream=s):
+        ya = a(xs)
+    with torch.cuda.graph(second, stream=s):
+        yb = b(xs)
+    for i in range(3):
+        new = x.roll(i + 1, 1) * (1 + i)
+        xs.copy_(new)
+        second.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(yb, b(new.clone()))
+        first.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(ya, a(new.clone()))
+
+
+def test_siblings_captured_one_by_one():
+    """Linked layers, each captured in a graph of its own on the same tensor: every graph computes its
+    layer's output."""
+    from smoothquant.fake_quant import link_siblings
+    D, g = torch.float16, gen(6)
+    a, b = _layers(2, 128, 96, D)
+    link_siblings(a, b)
+    x = torch.randn(300, 128, generator=g, device="cuda").to(D)
+    a(x), b(x)
+    xs = x.clone()
+    a(xs)                                                     # (b's output of it is kept for b)
+    graphs = [_captured(lambda q=q: q(xs)) for q in (a, b)]
+    assert torch.equal(a(xs), a(x.clone()))                   # not the graph's, which has not run
+    for i in range(3):
+        new = x.roll(i + 1, 1)
+        xs.copy_(new)
+        for (graph, y), q in zip(reversed(graphs), (b, a)):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, q(new.clone()))
+
+
+@pytest.mark.parametrize("p", [0.0, 0.05])
+def test_graphs_of_expert_modules_side_by_side(p):
+    """Two expert modules with salient columns of their own, captured without a warm-up, replayed on two
+    streams at once."""
+    import copy
+    from test_gpu_mixtral import _model
+    base = copy.deepcopy(_model(3).model.layers[0].mlp.experts).to("cuda", torch.float16)
+    H, g = base.hidden_dim, gen(7)
+    mods, ins = [], []
+    for i in range(2):
+        imp = torch.rand(H, generator=g, device="cuda").cpu()
+        mods.append(experts.W4A4Experts.from_float(base, "per_channel", "per_token", imp, p, 4, 32))
+        T = 40 + 30 * i
+        ins.append((torch.randn(T, H, generator=g, device="cuda").half(),
+                    torch.rand(T, base.num_experts, generator=g, device="cuda").topk(2, dim=1).indices,
+                    torch.rand(T, 2, generator=g, device="cuda")))
+    want = [m(*i) for m, i in zip(mods, ins)]
+    graphs = [_captured(lambda m=m, i=i: m(*i)) for m, i in zip(mods, ins)]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        torch.cuda.synchronize()
+        for s, (graph, _y) in zip(side, reversed(graphs)):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_g, y), w in zip(graphs, want):
+            assert torch.equal(y, w)
