@@ -31,7 +31,8 @@ ACTS = {None: 0, "silu": 1, "gelu": 2}
 @dataclass
 class Routing:
     """Which experts the tokens go to, and the (token, expert) pairs in expert order.  A pair is
-    f = token * top_k + j; an id of -1 means that nothing was chosen there."""
+    f = token * top_k + j; an id of -1 means that nothing was chosen there.  The three lists are a
+    plan as plan_routes makes it: the kernels follow them without looking whether they agree."""
     ids: torch.Tensor       # int32 [T, top_k]
     weights: torch.Tensor   # fp32 [T, top_k]
     offsets: torch.Tensor   # int32 [E + 1]: slots of expert e are offsets[e] .. offsets[e + 1]
@@ -46,6 +47,28 @@ class Routing:
     @property
     def top_k(self) -> int:
         return self.ids.shape[1]
+
+
+_I32 = torch.int32
+
+
+def _misfit(t, n: int, dev) -> bool:
+    """Whether a kernel would misread t as n contiguous int32 on dev."""
+    return not (t is not None and t.dtype is _I32 and t.numel() == n and t.device == dev
+                and t.is_contiguous())
+
+
+def _refuse_list(what: str, name: str, t, n: int, dev):
+    if t is not None and t.device != dev:
+        raise RuntimeError(f"{what}: x on {dev}, routing.{name} on {t.device}")
+    raise ValueError(f"{what}: routing.{name} must be {n} contiguous int32 on {dev}, got "
+                     + ("None" if t is None else f"{t.dtype} {tuple(t.shape)} of strides {t.stride()}"))
+
+
+def _shape_of(what: str, r: Routing):
+    if r.ids.dim() != 2:
+        raise ValueError(f"{what}: routing.ids must be [tokens, top_k], got {tuple(r.ids.shape)}")
+    return r.ids.shape
 
 
 def _plan_buffers(T: int, k: int, E: int, dev, n_ids: int):
@@ -272,12 +295,17 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
         ops._require_gpu(x, "expert_linear")
     code = ACTS.get(act, -1)
     by_slot = rows == "slot"
-    S, dev = routing.rows.shape[0], x.device
+    T, k = _shape_of("expert_linear", routing)
+    S, dev = T * k, x.device
     if (code < 0 or (code > 0) != pe.gated or not (by_slot or rows == "token")
             or routing.num_experts != pe.num_experts or x.dim() != 2
-            or x.shape[0] != (S if by_slot else routing.ids.shape[0]) or x.shape[1] != pe.K
-            or x.dtype is not pe.dtype or dev != pe.codes_t.device or routing.rows.device != dev):
+            or x.shape[0] != (S if by_slot else T) or x.shape[1] != pe.K
+            or x.dtype is not pe.dtype or dev != pe.codes_t.device):
         _expert_refuse(x, pe, routing, act, rows)
+    if _misfit(routing.rows, S, dev):
+        _refuse_list("expert_linear", "rows", routing.rows, S, dev)
+    if _misfit(routing.offsets, pe.num_experts + 1, dev):
+        _refuse_list("expert_linear", "offsets", routing.offsets, pe.num_experts + 1, dev)
     given = out is not None
     if not given:
         out = x.new_empty((S, pe.n_out))
@@ -292,7 +320,7 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     status = lib.sqmp_expert_linear_w4(
         a.data_ptr(), a.stride(0) if a.shape[0] > 1 else pe.Kp + pe.S_pad, cols, _ptr(pairs),
-        routing.ids.shape[1], routing.offsets.data_ptr(), pe.num_experts, pe.codes_t.data_ptr(),
+        k, routing.offsets.data_ptr(), pe.num_experts, pe.codes_t.data_ptr(),
         pe.scale_t.data_ptr(), _ptr(pe.sal_t), out.data_ptr(), dt, S, a.shape[0], pe.N, pe.n_out,
         pe.Kp, pe.S_pad, pe.Gw, pe.ngw, code, _ptr(ws), n, ops._raw_stream(dev.index))
     if status:
@@ -311,13 +339,12 @@ def _expert_refuse(x, pe, routing, act, rows):
     if routing.num_experts != pe.num_experts:
         raise ValueError(f"expert_linear: routing over {routing.num_experts} experts, weight of "
                          f"{pe.num_experts}")
-    want = (routing.rows.shape[0] if rows == "slot" else routing.tokens, pe.K)
+    want = (routing.tokens * (routing.top_k if rows == "slot" else 1), pe.K)
     if tuple(x.shape) != want:
         raise ValueError(f"expert_linear: x must be {list(want)}, got {list(x.shape)}")
     if x.dtype != pe.dtype:
         raise RuntimeError(f"expected input dtype {pe.dtype}, got {x.dtype}")
-    raise RuntimeError(f"expert_linear: x on {x.device}, weight on {pe.codes_t.device}, routing on "
-                       f"{routing.rows.device}")
+    raise RuntimeError(f"expert_linear: x on {x.device}, weight on {pe.codes_t.device}")
 
 
 @ops.on_tensor_device
@@ -326,15 +353,22 @@ def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = Non
     order of j; a token that goes nowhere gets zeros."""
     if not z.is_cuda:
         ops._require_gpu(z, "combine")
-    T, k = routing.ids.shape
+    T, k = _shape_of("combine", routing)
     if z.dim() != 2 or z.shape[0] != T * k or z.shape[1] == 0:
         raise ValueError(f"combine: z must be [{T * k}, H], got {tuple(z.shape)}")
     dt = ops.DTYPE_CODE.get(z.dtype)
     if dt is None:
         ops._dtype_code(z.dtype)
     dev = z.device
-    if routing.slots.device != dev:
-        raise RuntimeError(f"combine: z on {dev}, routing on {routing.slots.device}")
+    if _misfit(routing.slots, T * k, dev):
+        _refuse_list("combine", "slots", routing.slots, T * k, dev)
+    w = routing.weights
+    if w.shape != routing.ids.shape:
+        raise ValueError(f"combine: routing.weights must be {[T, k]}, got {list(w.shape)}")
+    if w.device != dev:
+        raise RuntimeError(f"combine: z on {dev}, routing.weights on {w.device}")
+    if w.dtype is not torch.float32 or not w.is_contiguous():  # (a caller's, as in plan_routes)
+        w = w.float().contiguous()
     if not z.is_contiguous():
         z = z.contiguous()
     H = z.shape[1]
@@ -347,7 +381,7 @@ def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = Non
     if T == 0:
         return out
     status = load().sqmp_combine(z.data_ptr(), dt, T, k, H, routing.slots.data_ptr(),
-                                 routing.weights.data_ptr(), out.data_ptr(),
+                                 w.data_ptr(), out.data_ptr(),
                                  ops._raw_stream(dev.index))
     if status:
         check(status, "combine")

@@ -124,3 +124,61 @@ def test_outputs_kept_for_siblings_do_not_leave_their_capture(monkeypatch):
 
 def test_capture_id_outside_of_a_capture():
     assert ops.capture_id(0) == 0
+
+
+# ------------------------------------------------------------------ routings by hand
+def _combine(r, T=4, k=2):
+    return experts.combine(gpu(torch.zeros(T * k, 64, dtype=torch.float16)), r)
+
+
+def _linear(r, T=4):
+    return experts.expert_linear(gpu(torch.zeros(T, 128, dtype=torch.float16)), weight(), r)
+
+
+@pytest.mark.parametrize("name,call", [("rows", _linear), ("offsets", _linear), ("slots", _combine)])
+@pytest.mark.parametrize("bad", [lambda t: gpu(t.long()), lambda t: gpu(t.float()), lambda t: gpu(t[:-1]),
+                                 lambda t: gpu(torch.zeros(2 * len(t), dtype=torch.int32))[::2],
+                                 lambda t: gpu(t.view(-1, 1)[:0]), lambda t: torch.zeros(t.shape, dtype=torch.int32),
+                                 lambda t: None], ids=["int64", "float", "short", "strided", "empty", "host", "none"])
+def test_lists_that_the_kernels_would_misread(library, name, call, bad):
+    """The kernels read a routing's lists as contiguous int32 of the routing's size on x's device: any
+    other tensor there is refused before a launch."""
+    r = routing()
+    call(r)
+    assert library.calls
+    library.calls.clear()
+    t = getattr(r, name)
+    setattr(r, name, bad(torch.Tensor(t) if t.dtype.is_floating_point else t.as_subclass(torch.Tensor)))
+    with pytest.raises((ValueError, RuntimeError), match=name):
+        call(r)
+    assert not [c for c in library.calls if "workspace" not in c[0]]
+
+
+def test_weights_of_another_type_or_stride(library):
+    """Router weights cast to the model's type, or strided, are converted as plan_routes converts them;
+    of another shape or on another device, refused."""
+    def passed():
+        return [c for c in library.calls if c[0] == "sqmp_combine"][-1][1][6]
+    for w in (torch.rand(4, 2).half(), torch.rand(4, 2).bfloat16(), torch.rand(4, 2).double(),
+              torch.rand(2, 4).t(), torch.rand(4, 4)[:, ::2], torch.rand(1, 2).expand(4, 2)):
+        r = routing()
+        r.weights = gpu(w)
+        before = r.weights
+        _combine(r)
+        assert passed() != w.data_ptr()                       # a converted copy
+        assert r.weights is before
+    r = routing()
+    _combine(r)
+    assert passed() == r.weights.data_ptr()
+    for w in (torch.rand(8), torch.rand(4, 1), torch.rand(2, 4), torch.rand(0, 2)):
+        r.weights = gpu(w)
+        with pytest.raises(ValueError, match="weights"):
+            _combine(r)
+    r.weights = torch.rand(4, 2)
+    with pytest.raises(RuntimeError, match="weights"):
+        _combine(r)
+    r = routing()
+    r.ids = gpu(torch.zeros(8, dtype=torch.int32))
+    for call in (_combine, _linear):
+        with pytest.raises(ValueError, match="ids"):
+            call(r)

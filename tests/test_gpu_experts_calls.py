@@ -217,3 +217,32 @@ def test_graphs_of_expert_modules_side_by_side(p):
         torch.cuda.synchronize()
         for (_g, y), w in zip(graphs, want):
             assert torch.equal(y, w)
+
+
+# ------------------------------------------------------------------ routings by hand
+@pytest.mark.parametrize("T", [5, 300])
+def test_router_weights_cast_by_the_caller(T):
+    """routing.weights in the model's type, as a model's own router casts them, and strided: the sums
+    of the converted weights."""
+    D, g = torch.bfloat16, gen(T)
+    E, k, H = 8, 2, 96
+    r = experts.route(torch.randn(T, E, generator=g, device="cuda"), k)
+    z = torch.randn(T * k, H, generator=g, device="cuda").to(D)
+    w16 = r.weights.to(D)
+    want = experts.combine(z, experts.plan_routes(r.ids, w16, E))
+    for w in (w16, w16.double(), w16.t().contiguous().t(), w16.float()[:, None, :].expand(T, 3, k)[:, 1]):
+        r.weights = w
+        assert torch.equal(experts.combine(z, r), want)
+    r.weights = w16.cpu()
+    with pytest.raises(RuntimeError, match="weights"):
+        experts.combine(z, r)
+    codes, scales = int_weight((E, 32, 64), 64, D, g)
+    pe = experts.pack_expert_codes(codes, scales, 64)
+    x = int_rows(T, 64, D, g)
+    good, wide = r.rows, r.rows.long()
+    for bad in (wide, good[:-1], good.cpu()):
+        r.rows = bad
+        with pytest.raises((ValueError, RuntimeError), match="rows"):
+            experts.expert_linear(x, pe, r)
+    r.rows = good
+    assert experts.expert_linear(x, pe, r).shape == (T * k, 32)
