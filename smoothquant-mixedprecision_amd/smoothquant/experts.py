@@ -180,14 +180,30 @@ def _interleave(t: torch.Tensor) -> torch.Tensor:
     return halves.view(E, 2, pad // 16, 16, X).transpose(1, 2).reshape(E, 2 * pad, X)
 
 
+def _packed_rows(pw: ops.PackedWeight, gated: bool):
+    """(codes, wscale, wsal, N) of the packed rows, interleaved where gated: after the quantization,
+    whose statistics (the mean and spread of a column) see the weight's own rows alone."""
+    if not gated:
+        return pw.codes, pw.wscale, pw.wsal, pw.N
+
+    def rows(t):
+        return _interleave(t[None, :pw.N])[0]
+    codes, scale, sal = rows(pw.codes), rows(pw.wscale.t()), rows(pw.wsal)
+    N = codes.shape[0]
+    more = (0, 0, 0, ops.pad_n(N) - N)
+    return (torch.nn.functional.pad(codes, more),
+            torch.nn.functional.pad(scale, more).t().contiguous(), sal.contiguous(), N)
+
+
 def _pack_all(weights, E: int, rows: int, gated: bool) -> PackedExperts:
-    """weights: iterator over the E experts' PackedWeight (rows interleaved where gated)."""
+    """weights: iterator over the E experts' PackedWeight (gated: of [gate; up] rows)."""
     pe, maps = None, []
     for e, pw in enumerate(weights):
         if not ops.gemv_eligible(pw):
             raise ValueError("pack_experts: needs 4-bit codes in groups of a multiple of 8 columns "
                              f"(n_bits {pw.n_bits}, group {pw.Gw})")
-        one = ops.tile_major(pw.codes, pw.wscale, pw.wsal, pw.N, pw.Kp, pw.S_pad, pw.ngw, pw.dtype,
+        codes, wscale, wsal, N = _packed_rows(pw, gated)
+        one = ops.tile_major(codes, wscale, wsal, N, pw.Kp, pw.S_pad, pw.ngw, pw.dtype,
                              None if pe is None else (pe.codes_t[e], pe.scale_t[e],
                                                       all_sal[e]))
         if pe is None:
@@ -196,7 +212,7 @@ def _pack_all(weights, E: int, rows: int, gated: bool) -> PackedExperts:
                 st[0] = t
             all_sal = stacks[2]
             pe = PackedExperts(stacks[0], stacks[1], all_sal if pw.S_pad else None, pw.amap,
-                               pw.salient, E, rows // 2 if gated else rows, pw.N, pw.K, pw.Kp,
+                               pw.salient, E, rows // 2 if gated else rows, N, pw.K, pw.Kp,
                                pw.S, pw.S_pad, pw.Gw, pw.ngw, pw.dtype, gated, False)
         maps.append(pw.amap)
     amap = torch.stack(maps)
@@ -227,9 +243,7 @@ def pack_experts(w: torch.Tensor, weight_quant: str = "per_channel", group_size:
     _check_stack("pack_experts", w, gated)
     if weight_quant == "none":
         raise ValueError("pack_experts: needs a quantized weight")
-    it = (ops.pack_weight(_interleave(w[e:e + 1])[0] if gated else w[e], weight_quant, 4, group_size,
-                          salient)
-          for e in range(w.shape[0]))
+    it = (ops.pack_weight(w[e], weight_quant, 4, group_size, salient) for e in range(w.shape[0]))
     return _pack_all(it, w.shape[0], w.shape[1], gated)
 
 

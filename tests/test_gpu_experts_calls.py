@@ -246,3 +246,52 @@ def test_router_weights_cast_by_the_caller(T):
             experts.expert_linear(x, pe, r)
     r.rows = good
     assert experts.expert_linear(x, pe, r).shape == (T * k, 32)
+
+
+# ------------------------------------------------------------------ gated weights
+def unpacked(pe, e):
+    """W_hat of expert e's packed rows [rows, K] from the operands' documented layout (csrc/sqmp_w4.h):
+    32-row blocks, 64-position stages, lane (r, q) holding rows r and 16 + r, chunk 4 (q & 1) + 2 s + q / 2."""
+    nb, nk = (pe.N + 255) // 256 * 8, pe.Kp // 64
+    words = pe.codes_t[e].cpu().view(torch.int32).view(nb, nk, 4, 16, 2, 2)       # block, stage, q, r, j, s
+    nib = torch.stack([(words >> ((16 if v & 1 else 0) + 4 * (v >> 1))) & 15 for v in range(8)], -1) - 8
+    codes = torch.zeros(nb, 2, 16, nk, 8, 8, dtype=torch.int32)                   # block, j, r, stage, chunk, element
+    sal = None if pe.sal_t is None else pe.sal_t[e].cpu().view(nb, pe.S_pad // 64, 4, 16, 2, 2, 8)
+    exact = None if sal is None else torch.zeros(nb, 2, 16, pe.S_pad // 64, 8, 8, dtype=pe.dtype)
+    for q in range(4):
+        for s in range(2):
+            c = 4 * (q & 1) + 2 * s + (q >> 1)
+            codes[:, :, :, :, c] = nib[:, :, q, :, :, s].permute(0, 3, 2, 1, 4)
+            if sal is not None:
+                exact[:, :, :, :, c] = sal[:, :, q, :, :, s].permute(0, 3, 2, 1, 4)
+    group = torch.clamp(torch.arange(pe.Kp) // pe.Gw, max=pe.ngw - 1)
+    scale = pe.scale_t[e].cpu().view(nb, pe.ngw, 16, 2).permute(0, 3, 2, 1).reshape(nb * 32, pe.ngw)[:, group]
+    w = (codes.reshape(nb * 32, pe.Kp).double() * scale.double()).to(pe.dtype)
+    amap = (pe.amap if pe.amap.dim() == 1 else pe.amap[e]).cpu().long()
+    out = torch.zeros(nb * 32, pe.K, dtype=pe.dtype)
+    out[:, amap[amap >= 0]] = w[:, amap >= 0]
+    if exact is not None:
+        out[:, pe.salient.cpu().long()] = exact.reshape(nb * 32, pe.S_pad)[:, :pe.S]
+    return out[:pe.N]
+
+
+@pytest.mark.parametrize("dt", ["fp16", "fp32"])
+@pytest.mark.parametrize("wq", ["per_channel", "per_tensor", "per_group", "per_group_unsorted", "per_group_mean3std"])
+@pytest.mark.parametrize("I,p", [(5, 0.0), (33, 0.0), (33, 0.06), (48, 0.0)])
+def test_gated_weights_are_those_of_their_own_rows(I, p, wq, dt):
+    """A gated weight is quantized as one weight of 2 I rows, whatever I is padded to: the very values
+    of ops.pack_weight of those rows."""
+    D, g = DT[dt], gen(I)
+    E, K, G = 3, 192, 32
+    # columns whose mean and spread differ: rows of zeros among the statistics change their order
+    w = (torch.randn(E, 2 * I, K, generator=g, device="cuda") * 0.02
+         * torch.rand(K, generator=g, device="cuda") + 0.02 * torch.rand(K, generator=g, device="cuda")).to(D)
+    sal = torch.randperm(K, generator=g, device="cuda")[:int(p * K)] if p else None
+    pe = experts.pack_experts(w, wq, G, sal, gated=True)
+    assert pe.n_out == I and pe.gated
+    n = torch.arange(I)
+    gate = 32 * (n // 16) + n % 16
+    for e in range(E):
+        want = ops.dequant_weight(ops.pack_weight(w[e], wq, 4, G, sal)).cpu()
+        got = unpacked(pe, e)
+        assert torch.equal(got[gate], want[:I]) and torch.equal(got[gate + 16], want[I:])
