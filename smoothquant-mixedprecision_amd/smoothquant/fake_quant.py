@@ -480,6 +480,12 @@ class W4A4Linear(nn.Module):
         return self
 
     # ------------------------------------------------------------------ forward
+    def _kernel_for(self, rows: int, pw: PackedWeight) -> str:
+        """The kernel of a batch: "gemv" is "auto" where the few-row product does not take it."""
+        if self.kernel == "gemv" and not (rows <= ops.GEMV_MAX_ROWS and ops.gemv_eligible(pw)):
+            return "auto"
+        return self.kernel
+
     @torch.no_grad()
     def forward(self, x):
         if self.kernel not in KERNELS:
@@ -523,9 +529,10 @@ class W4A4Linear(nn.Module):
         if bias is not None and bias.device != x.device:
             raise RuntimeError(f"bias on {bias.device}, input on {x.device}: move the module "
                                "to the input's device")
-        use_gemv = (self.kernel == "gemv" and x2.shape[0] <= ops.GEMV_MAX_ROWS
-                    and ops.gemv_eligible(pw))
-        kernel = "fq" if use_gemv else "auto" if self.kernel == "gemv" else self.kernel
+        kernel = self._kernel_for(x2.shape[0], pw)
+        use_gemv = kernel == "gemv"
+        if use_gemv:
+            kernel = "fq"  # (the operand)
         use_f8 = kernel == "f8" or (
             kernel == "auto" and ops.f8_auto(pw, amode, bits) and ops.f8_input_ok(xc))
         use_fqt = (not use_f8 and kernel in ("auto", "fqt")
@@ -672,7 +679,7 @@ class SiblingGroup:
         every member for this input, else None."""
         spec, pws, biases = None, [], []
         for m in self.members:
-            if m.kernel != "auto" or resolve_quantizer(m.output_quant) is not None:
+            if m.kernel not in ("auto", "gemv") or resolve_quantizer(m.output_quant) is not None:
                 return None
             sp = resolve_quantizer(m.act_quant)
             if spec is None:
@@ -680,6 +687,8 @@ class SiblingGroup:
             elif sp != spec:
                 return None
             pw = m.packed()
+            if m._kernel_for(x2.shape[0], pw) != "auto":
+                return None
             b = None if m.bias is None else m.bias.reshape(-1)
             if x2.dtype != pw.dtype or (b is not None and (b.dtype != pw.dtype
                                                             or b.device != x2.device)):
@@ -731,7 +740,8 @@ def link_siblings(*modules):
 
 def use_gemv(model: nn.Module, enable: bool = True) -> int:
     """Switch the W4A4Linear layers of `model` whose kernel is "auto" to "gemv" (enable=False:
-    back) and return how many changed: a model that decodes a few tokens at a time."""
+    every "gemv" layer to "auto", one set by hand too) and return how many changed: a model that
+    decodes a few tokens at a time."""
     was, now = ("auto", "gemv") if enable else ("gemv", "auto")
     n = 0
     for m in model.modules():

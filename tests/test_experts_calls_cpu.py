@@ -182,3 +182,24 @@ def test_weights_of_another_type_or_stride(library):
     for call in (_combine, _linear):
         with pytest.raises(ValueError, match="ids"):
             call(r)
+
+
+@pytest.mark.parametrize("rows,eligible,grouped", [(65, True, True), (64, True, False), (1, True, False), (3, False, True)])
+def test_linked_layers_switched_to_gemv_stay_a_group_on_prompts(monkeypatch, rows, eligible, grouped):
+    """"gemv" is "auto" for more rows than the few-row product takes, and for weights that it does not:
+    linked layers share their quantizer pass and product there, as with "auto"."""
+    from smoothquant import fake_quant
+    layers = [fake_quant.W4A4Linear(64, 32, bias=False, act_quant="per_group") for _ in range(2)]
+    pw = type("Pw", (), dict(dtype=torch.float16))()
+    for m in layers:
+        monkeypatch.setattr(m, "packed", lambda: pw)
+    monkeypatch.setattr(ops, "gemv_eligible", lambda p: eligible)
+    monkeypatch.setattr(ops, "group_eligible", lambda *a: True)
+    g = fake_quant.link_siblings(*layers)
+    x = torch.zeros(max(rows, 8), 64, dtype=torch.float16)[:rows]
+    monkeypatch.setattr(ops, "f8_input_ok", lambda x: True)
+    assert g._plan(x) is not None
+    assert fake_quant.use_gemv(torch.nn.ModuleList(layers)) == 2
+    assert (g._plan(x) is not None) == grouped
+    layers[1].kernel = "fq"
+    assert g._plan(x) is None

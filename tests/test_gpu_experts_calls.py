@@ -5,7 +5,7 @@ import torch
 
 from smoothquant import experts, ops
 from smoothquant.fake_quant import W4A4Linear
-from w4_cases import DT, gen, int_rows, int_weight
+from w4_cases import DT, gen, int_rows, int_weight, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -14,7 +14,7 @@ def _layers(n, K, N, D, **kw):
     """Sorted per_group layers of one input width, whose statistics and operands are kept per input."""
     torch.manual_seed(6)
     return [W4A4Linear.from_float(torch.nn.Linear(K, N).to("cuda", D), weight_quant="per_group",
-                                  act_quant="per_group", group_size=32, **kw) for _ in range(n)]
+                                  act_quant="per_group", group_size=64, **kw) for _ in range(n)]
 
 
 @pytest.mark.parametrize("linked", [False, True])
@@ -63,7 +63,7 @@ def test_copies_of_a_layer_after_its_original_is_gone(tmp_path):
             t.zero_()
         assert torch.equal(q(x.clone()), q.bias.reshape(1, -1).expand(3, -1).to(D))   # (what a copy must not see)
         del q, pw
-        a = ops.quant_act_fp(x, others[2], "per_group", 4, 32)
+        a = ops.quant_act_fp(x, others[2], "per_group", 4, 64)
         y = ops.gemv(a, others[2], others[0].bias, packed=True)
         for got in (others[0](x.clone()), others[1](x.clone()), y):
             assert torch.equal(got, want)
@@ -295,3 +295,33 @@ def test_gated_weights_are_those_of_their_own_rows(I, p, wq, dt):
         want = ops.dequant_weight(ops.pack_weight(w[e], wq, 4, G, sal)).cpu()
         got = unpacked(pe, e)
         assert torch.equal(got[gate], want[:I]) and torch.equal(got[gate + 16], want[I:])
+
+
+@pytest.mark.parametrize("M", [64, 65, 300, 2048])
+def test_linked_layers_after_use_gemv(M):
+    """A model switched for decoding computes prompts as before: one grouped pass, the bits of "auto"."""
+    from smoothquant import fake_quant
+    D = torch.float16
+    layers = _layers(3, 512, 256, D)
+    group = fake_quant.link_siblings(*layers)
+    x = torch.randn(M, 512, device="cuda").to(D)
+    want = [q(x) for q in layers]
+    launches = []
+    real = ops.gemm_fq7_group
+    fake_quant.use_gemv(torch.nn.ModuleList(layers))
+    try:
+        ops.gemm_fq7_group = lambda *a: launches.append(len(a[0])) or real(*a)
+        got = [q(x) for q in layers]
+    finally:
+        ops.gemm_fq7_group = real
+    assert launches == ([3] if M > 64 else []) and not group._stash
+    for y, w, q in zip(got, want, layers):
+        if M > 64:
+            assert torch.equal(y, w)
+            continue
+        pw = q.packed()
+        a = ops.quant_act_fp(x.clone(), pw, "per_group", 4, 64)
+        w_hat = ops.dequant_weight_packed(pw).double()
+        exact = a.double() @ w_hat.T + q.bias.reshape(-1).double()
+        tol = tolerance(a, w_hat, exact, D, extra=2.0 ** -24 * exact.abs())
+        assert ((y.double() - exact).abs() <= tol).all()
