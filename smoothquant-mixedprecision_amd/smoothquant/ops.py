@@ -51,12 +51,15 @@ _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.curre
 
 def on_tensor_device(fn):
     """fn(tensor, ...) with the tensor's device current."""
+    first = fn.__code__.co_varnames[0]
+
     @functools.wraps(fn)
-    def call(t, *args, **kw):
+    def call(*args, **kw):
+        t = args[0] if args else kw.get(first)
         if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != _current_device():
             with torch.cuda.device(t.device):
-                return fn(t, *args, **kw)
-        return fn(t, *args, **kw)
+                return fn(*args, **kw)
+        return fn(*args, **kw)
     return call
 
 

@@ -203,3 +203,35 @@ def test_linked_layers_switched_to_gemv_stay_a_group_on_prompts(monkeypatch, row
     assert (g._plan(x) is not None) == grouped
     layers[1].kernel = "fq"
     assert g._plan(x) is None
+
+
+def test_calls_by_keyword(library, monkeypatch):
+    """The tensor by whose device a call goes may be given by its name, as any argument."""
+    r = routing()
+    assert experts.combine(z=gpu(torch.zeros(8, 64).half()), routing=r).shape == (4, 64)
+    assert experts.combine(routing=r, z=gpu(torch.zeros(8, 64).half())).shape == (4, 64)
+    assert experts.expert_linear(x=gpu(torch.zeros(4, 128).half()), pe=weight(), routing=r).shape == (8, 32)
+    for call in (lambda: experts.route(top_k=2, logits=torch.zeros(4, 3)),       # (reached: host tensors)
+                 lambda: experts.plan_routes(num_experts=3, weights=torch.zeros(4, 2), ids=torch.zeros(4, 2)),
+                 lambda: ops.gemv(x=torch.zeros(1, 8), pw=None),
+                 lambda: experts.pack_experts(w=torch.zeros(2, 8, 8))):
+        with pytest.raises(RuntimeError, match="ROCm GPU"):
+            call()
+    for name in ("pack_codes", "pack_rows", "tile_major"):
+        with pytest.raises(TypeError, match="missing"):
+            getattr(ops, name)()
+    entered = []
+    monkeypatch.setattr(ops, "_current_device", lambda: 1)
+
+    class Ctx:
+        def __init__(self, dev):
+            entered.append(dev)
+
+        def __enter__(self):
+            return self
+
+        def __exit__(self, *exc):
+            return False
+    monkeypatch.setattr(torch.cuda, "device", Ctx)
+    experts.combine(routing=r, z=gpu(torch.zeros(8, 64).half()))
+    assert entered == [CUDA0]
