@@ -71,6 +71,14 @@ def _shape_of(what: str, r: Routing):
     return r.ids.shape
 
 
+def _refuse_overlap(what: str, out: torch.Tensor, x: torch.Tensor):
+    """Workgroups read rows of x that others' outputs would have taken the place of."""
+    a, b = ((t.data_ptr(), t.data_ptr() + t.element_size() * (
+        1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))) for t in (out, x))
+    if out.numel() and x.numel() and a[0] < b[1] and b[0] < a[1]:
+        raise ValueError(f"{what}: out overlaps the operand in memory")
+
+
 def _plan_buffers(T: int, k: int, E: int, dev, n_ids: int):
     """(ids, rows, slots, offsets, workspace, its size): the first four, int32, from one
     allocation in this order."""
@@ -304,7 +312,8 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
     D(act(gate) * up) of a gated weight (act "silu" / "gelu"; fp32 up to the one rounding).
 
     x: [tokens, K] (rows="token") or [tokens * top_k, K] already in expert order (rows="slot").
-    Rows of z behind routing.offsets[-1] (tokens that go nowhere) are left as they were."""
+    Rows of z behind routing.offsets[-1] (tokens that go nowhere) are left as they were.  `out` may not
+    share memory with x."""
     if not x.is_cuda:
         ops._require_gpu(x, "expert_linear")
     code = ACTS.get(act, -1)
@@ -326,6 +335,8 @@ def expert_linear(x: torch.Tensor, pe: PackedExperts, routing: Routing, act: Opt
     elif (tuple(out.shape) != (S, pe.n_out) or out.dtype != pe.dtype or out.device != dev
           or not out.is_contiguous()):
         raise ValueError(f"expert_linear: out must be contiguous {pe.dtype} [{S}, {pe.n_out}] on {dev}")
+    if given:
+        _refuse_overlap("expert_linear", out, x)
     if S == 0:
         return out
     a, pairs, cols = _operand(x, pe, routing, by_slot)
@@ -364,7 +375,7 @@ def _expert_refuse(x, pe, routing, act, rows):
 @ops.on_tensor_device
 def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y [tokens, H]: y[t] = D(sum_j weights[t, j] * z[slot of pair (t, j)]), fp32 sums in the
-    order of j; a token that goes nowhere gets zeros."""
+    order of j; a token that goes nowhere gets zeros.  `out` may not share memory with z."""
     if not z.is_cuda:
         ops._require_gpu(z, "combine")
     T, k = _shape_of("combine", routing)
@@ -392,6 +403,8 @@ def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = Non
     elif (tuple(out.shape) != (T, H) or out.dtype != z.dtype or out.device != dev
           or not out.is_contiguous()):
         raise ValueError(f"combine: out must be contiguous {z.dtype} [{T}, {H}] on {dev}")
+    if given:
+        _refuse_overlap("combine", out, z)
     if T == 0:
         return out
     status = load().sqmp_combine(z.data_ptr(), dt, T, k, H, routing.slots.data_ptr(),

@@ -235,3 +235,27 @@ def test_calls_by_keyword(library, monkeypatch):
     monkeypatch.setattr(torch.cuda, "device", Ctx)
     experts.combine(routing=r, z=gpu(torch.zeros(8, 64).half()))
     assert entered == [CUDA0]
+
+
+# ------------------------------------------------------------------ calls to refuse
+def test_out_in_the_memory_of_the_operand(library):
+    """A product reads its rows while it writes others': `out` may not share memory with them."""
+    r = routing()
+    buf = torch.zeros(40, 64, dtype=torch.float16)
+    z = gpu(buf[:8])
+    for at in (0, 3, 7):
+        with pytest.raises(ValueError, match="overlap"):
+            experts.combine(z, r, out=gpu(buf[at:at + 4]))
+    assert experts.combine(z, r, out=gpu(buf[8:12])) is not None
+    assert experts.combine(gpu(buf[4:12]), r, out=gpu(buf[:4])) is not None
+    pe = weight(N=128)
+    buf = torch.zeros(40, 128, dtype=torch.float16)
+    with pytest.raises(ValueError, match="overlap"):
+        experts.expert_linear(gpu(buf[:8]), pe, r, rows="slot", out=gpu(buf[:8]))
+    with pytest.raises(ValueError, match="overlap"):
+        experts.expert_linear(gpu(buf[7:11]), pe, r, out=gpu(buf[:8]))
+    with pytest.raises(ValueError, match="overlap"):          # rows apart, the last one inside
+        experts.expert_linear(gpu(buf[:40:10]), pe, r, out=gpu(buf[30:38]))
+    assert experts.expert_linear(gpu(buf[:31:10]), pe, r, out=gpu(buf[31:39])) is not None
+    n = len([c for c in library.calls if "workspace" not in c[0]])
+    assert n == 3
