@@ -24,6 +24,7 @@ from . import _lib, ops
 from ._lib import check, load
 
 MAX_EXPERTS, MAX_TOP_K = 256, 16
+MAX_PAIRS = 2 ** 31 - 4097  # slots and pairs are int32, the kernels' loops run at most a block past them
 ACTS = {None: 0, "silu": 1, "gelu": 2}
 
 
@@ -92,11 +93,13 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _check_sizes(what: str, E: int, k: int):
+def _check_sizes(what: str, T: int, E: int, k: int):
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError(f"{what}: {E} experts, supported are 1 .. {MAX_EXPERTS}")
     if not 1 <= k <= MAX_TOP_K:
         raise ValueError(f"{what}: top_k {k}, supported are 1 .. {MAX_TOP_K}")
+    if T * k > MAX_PAIRS:
+        raise ValueError(f"{what}: {T} tokens times {k} are more than {MAX_PAIRS} pairs")
 
 
 @ops.on_tensor_device
@@ -110,7 +113,7 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
     if logits.dim() != 2:
         raise ValueError(f"route: logits must be [tokens, experts], got {tuple(logits.shape)}")
     T, E = logits.shape
-    _check_sizes("route", E, top_k)
+    _check_sizes("route", T, E, top_k)
     if top_k > E:
         raise ValueError(f"route: top_k {top_k} of {E} experts")
     dt = ops._dtype_code(logits.dtype)
@@ -144,7 +147,7 @@ def plan_routes(ids: torch.Tensor, weights: torch.Tensor, num_experts: int) -> R
         raise ValueError(f"plan_routes: weights {tuple(weights.shape)} on {weights.device} do not "
                          f"match ids {tuple(ids.shape)} on {ids.device}")
     T, k = ids.shape
-    _check_sizes("plan_routes", num_experts, k)
+    _check_sizes("plan_routes", T, num_experts, k)
     if ids.dtype != torch.int32:
         ids = (ids.long().clamp(-1, num_experts)).to(torch.int32)  # (no id may wrap into range)
     ids = ids.contiguous()
@@ -381,6 +384,8 @@ def combine(z: torch.Tensor, routing: Routing, out: Optional[torch.Tensor] = Non
     T, k = _shape_of("combine", routing)
     if z.dim() != 2 or z.shape[0] != T * k or z.shape[1] == 0:
         raise ValueError(f"combine: z must be [{T * k}, H], got {tuple(z.shape)}")
+    if z.shape[1] > MAX_PAIRS:
+        raise ValueError(f"combine: {z.shape[1]} columns, at most {MAX_PAIRS}")
     dt = ops.DTYPE_CODE.get(z.dtype)
     if dt is None:
         ops._dtype_code(z.dtype)

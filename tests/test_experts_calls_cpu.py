@@ -259,3 +259,21 @@ def test_out_in_the_memory_of_the_operand(library):
     assert experts.expert_linear(gpu(buf[:31:10]), pe, r, out=gpu(buf[31:39])) is not None
     n = len([c for c in library.calls if "workspace" not in c[0]])
     assert n == 3
+
+
+@pytest.mark.parametrize("T,k", [(2 ** 32 + 5, 1), (2 ** 31, 1), (2 ** 28, 8)])
+def test_more_pairs_than_the_lists_can_number(library, T, k):
+    """Slots and pairs are 32-bit numbers: more of them are refused, not wrapped."""
+    with pytest.raises(ValueError, match="pairs"):
+        experts.route(gpu(torch.zeros(1, 8).expand(T, 8)), k)
+    with pytest.raises(ValueError, match="pairs"):
+        experts.plan_routes(gpu(torch.zeros(1, k, dtype=torch.int32).expand(T, k)),
+                            gpu(torch.zeros(1, k).expand(T, k)), 8)
+    assert not library.calls
+
+
+def test_rows_wider_than_the_kernels_count(library):
+    r = routing()
+    with pytest.raises(ValueError, match="columns"):
+        experts.combine(gpu(torch.zeros(1, 1, dtype=torch.float16).expand(8, 2 ** 32 + 8)), r)
+    assert not library.calls
