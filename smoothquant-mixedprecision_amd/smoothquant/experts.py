@@ -530,6 +530,9 @@ class W4A4Experts(nn.Module):
     @torch.no_grad()
     def forward(self, hidden_states, top_k_index, top_k_weights):
         ops._require_gpu(hidden_states, "W4A4Experts.forward")
+        if hidden_states.device.index != ops._current_device():
+            with torch.cuda.device(hidden_states.device):
+                return self.forward(hidden_states, top_k_index, top_k_weights)
         gate_up, down, maps = self.packed()
         x = hidden_states.reshape(-1, hidden_states.shape[-1])
         if x.shape[1] != gate_up.K:

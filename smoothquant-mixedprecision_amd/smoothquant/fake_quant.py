@@ -490,6 +490,9 @@ class W4A4Linear(nn.Module):
     def forward(self, x):
         if self.kernel not in KERNELS:
             raise ValueError(f"kernel must be one of {KERNELS}, got {self.kernel!r}")
+        if x.is_cuda and x.device.index != ops._current_device():
+            with torch.cuda.device(x.device):
+                return self.forward(x)
         x_shape = x.shape
         if len(x_shape) == 3:
             x2 = x.reshape(-1, x_shape[-1])

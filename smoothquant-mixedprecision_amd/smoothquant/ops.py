@@ -5,6 +5,7 @@ raises if a tensor is not on a ROCm device: the W4A4 operator has no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -45,8 +46,15 @@ def _stream(t: torch.Tensor):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 # A device's default stream has the null handle, which names no device: the few-row and expert
-# calls make their tensors' device current first where it is not
+# calls, the modules' forward and packing make their tensors' device current first where it is not
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def on_device(device: torch.device):
+    """A context in which `device` (a tensor's) is the current one."""
+    if device.type != "cuda" or device.index == _current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def on_tensor_device(fn):
@@ -163,11 +171,13 @@ def build_maps(K: int, salient: Optional[torch.Tensor], device, Kp: Optional[int
     amap_fq = torch.empty(K, **i32)
     nonsal = torch.empty(max(K - S, 1), **i32)
     ref = amap_fq
-    check(load().sqmp_build_maps(K, _p(salient), S, _p(perm), _p(amap), _p(amap_fq), _p(nonsal),
-                                 Kp, _stream(ref)), "build maps")
+    with on_device(ref.device):
+        check(load().sqmp_build_maps(K, _p(salient), S, _p(perm), _p(amap), _p(amap_fq), _p(nonsal),
+                                     Kp, _stream(ref)), "build maps")
     return perm, amap, amap_fq, nonsal
 
 
+@on_tensor_device
 def pack_weight(w: torch.Tensor, weight_quant: str, n_bits: int, group_size: int,
                 salient: Optional[torch.Tensor]) -> PackedWeight:
     """Quantize + pack W [N, K] (fake_quant.py:324-371 without the module bookkeeping)."""
@@ -253,9 +263,10 @@ def salient_key(K: int, salient: Optional[torch.Tensor]) -> tuple:
 
 def dequant_weight_packed(pw: PackedWeight) -> torch.Tensor:
     out = torch.empty((pw.N, pw.Kp), dtype=pw.dtype, device=pw.codes.device)
-    check(load().sqmp_dequant_weight_packed(_p(pw.codes), _p(pw.wscale), _dtype_code(pw.dtype),
-                                            pw.N, pw.Kp, pw.Gw, pw.ngw, pw.n_bits, _p(out),
-                                            _stream(out)), "dequant_weight_packed")
+    with on_device(pw.codes.device):
+        check(load().sqmp_dequant_weight_packed(_p(pw.codes), _p(pw.wscale), _dtype_code(pw.dtype),
+                                                pw.N, pw.Kp, pw.Gw, pw.ngw, pw.n_bits, _p(out),
+                                                _stream(out)), "dequant_weight_packed")
     return out
 
 
@@ -263,10 +274,11 @@ def dequant_weight(pw: PackedWeight) -> torch.Tensor:
     """The reference's `weight` buffer: W_hat [N, K] in D (salient columns exact)."""
     _require_gpu(pw.codes, "dequant_weight")
     w_hat = torch.zeros((pw.N, pw.K), dtype=pw.dtype, device=pw.codes.device)
-    check(load().sqmp_dequant_weight(_p(pw.codes), _p(pw.wscale), _p(pw.wsal) if pw.S_pad else None,
-                                     _p(pw.amap), _p(pw.salient), _dtype_code(pw.dtype), pw.N,
-                                     pw.K, pw.S, pw.n_bits, pw.Kp, pw.Gw, pw.ngw, pw.S_pad,
-                                     _p(w_hat), _stream(w_hat)), "dequant_weight")
+    with on_device(pw.codes.device):
+        check(load().sqmp_dequant_weight(_p(pw.codes), _p(pw.wscale), _p(pw.wsal) if pw.S_pad else None,
+                                         _p(pw.amap), _p(pw.salient), _dtype_code(pw.dtype), pw.N,
+                                         pw.K, pw.S, pw.n_bits, pw.Kp, pw.Gw, pw.ngw, pw.S_pad,
+                                         _p(w_hat), _stream(w_hat)), "dequant_weight")
     return w_hat
 
 

@@ -277,3 +277,52 @@ def test_rows_wider_than_the_kernels_count(library):
     with pytest.raises(ValueError, match="columns"):
         experts.combine(gpu(torch.zeros(1, 1, dtype=torch.float16).expand(8, 2 ** 32 + 8)), r)
     assert not library.calls
+
+
+@pytest.mark.parametrize("call", ["experts", "linear", "linear_group", "pack"])
+def test_modules_run_on_their_inputs_device(monkeypatch, call):
+    """A device's default stream is the null handle, which a C entry takes for the current device's: a
+    module called with a tensor of another device makes that one current for all of its launches."""
+    from smoothquant import fake_quant
+    current, seen = [0], []
+    monkeypatch.setattr(ops, "_current_device", lambda: current[0])
+
+    class Ctx:
+        def __init__(self, dev):
+            self.dev = torch.device(dev) if not isinstance(dev, torch.device) else dev
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.dev.index
+
+        def __exit__(self, *exc):
+            current[0] = self.was
+            return False
+    monkeypatch.setattr(torch.cuda, "device", Ctx)
+
+    class OnSecond(OnGpu):
+        device = torch.device("cuda", 1)
+    x = torch.zeros(2, 64, dtype=torch.float16).as_subclass(OnSecond)
+
+    class Reached(Exception):
+        pass
+
+    def reached(*a, **k):
+        seen.append(current[0])
+        raise Reached
+    if call == "experts":
+        m = experts.W4A4Experts()
+        monkeypatch.setattr(m, "packed", reached)
+        run = lambda: m(x, torch.zeros(2, 1, dtype=torch.long), torch.ones(2, 1))
+    elif call == "pack":
+        monkeypatch.setattr(ops, "geometry", reached)
+        run = lambda: ops.pack_weight(x, "per_channel", 4, 64, None)
+    else:
+        m = fake_quant.W4A4Linear(64, 8, bias=False)
+        if call == "linear_group":
+            fake_quant.link_siblings(m, fake_quant.W4A4Linear(64, 8, bias=False))
+            monkeypatch.setattr(fake_quant.SiblingGroup, "forward", reached)
+        monkeypatch.setattr(m, "packed", reached)
+        run = lambda: m(x)
+    with pytest.raises(Reached):
+        run()
+    assert seen == [1] and current == [0]
