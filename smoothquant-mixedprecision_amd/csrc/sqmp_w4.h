@@ -65,12 +65,13 @@ __device__ inline void mfma(f32x4& acc, const Frag<DT>& a, const Frag<DT>& b) {
   for (int i = 0; i < n; ++i) Mfma<DT>::run(acc, a.v[i], b.v[i]);
 }
 
-// 4 bytes 0 .. 15 -> floats, times 2^-9: as e4m3 such a byte is n 2^-9 (0 .. 7 the subnormals, 8 .. 15
-// the first binade, one step of 2^-9), so one conversion makes two of them
+// 4 bytes 0 .. 15 -> floats: as e4m3 such a byte is n 2^-9 (0 .. 7 the subnormals, 8 .. 15 the first
+// binade, one step of 2^-9), so one conversion with a scale of 2^9 makes two of them.  (The 2^9 in the
+// weight's scale instead overflows from 2^119 on)
 __device__ inline void nibbles_to_f32(uint32_t b, float (&n)[4]) {
   typedef float f2 __attribute__((ext_vector_type(2)));
-  const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)b, false);
-  const f2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)b, true);
+  const f2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(b, 512.0f, false);
+  const f2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(b, 512.0f, true);
   n[0] = lo[0], n[1] = lo[1], n[2] = hi[0], n[3] = hi[1];
 }
 
@@ -83,11 +84,11 @@ __device__ inline Frag<DT> decode(uint32_t w, typename DT::T s, const DecK& k) {
   f.v[0] = Dec<DT>::run(w, Dec<DT>::prep((uint32_t)b), k);
   return f;
 }
-// (n - 8) s = fma(n 2^-9, 2^9 s, -8 s): the scaled factors and 8 s are exact, so fp32 rounds once,
-// and bf16 s (8 + 4 significant bits) not before the cast
+// (n - 8) s = fma(n, s, -8 s): 8 s is exact, so fp32 rounds once, and bf16 s (8 + 4 significant bits)
+// not before the cast (scales below 2^125: 8 s is finite)
 template <>
 __device__ inline Frag<F32> decode<F32>(uint32_t w, float s, const DecK&) {
-  const float s9 = 512.f * s, m8 = -8.f * s;
+  const float m8 = -8.f * s;
   float b[4], c[4];  // nibbles 0, 2, 4, 6 and 1, 3, 5, 7
   nibbles_to_f32(w & 0x0F0F0F0Fu, b);
   nibbles_to_f32((w >> 4) & 0x0F0F0F0Fu, c);
@@ -95,7 +96,7 @@ __device__ inline Frag<F32> decode<F32>(uint32_t w, float s, const DecK&) {
   const float o[8] = {b[0], b[2], c[0], c[2], b[1], b[3], c[1], c[3]};
   Frag<F32> f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f.v[e >> 2][e & 3] = __float_as_uint(__builtin_fmaf(o[e], s9, m8));
+  for (int e = 0; e < 8; ++e) f.v[e >> 2][e & 3] = __float_as_uint(__builtin_fmaf(o[e], s, m8));
   return f;
 }
 // Half of decode: the values at dwords h and h + 2 of the fragment (elements 2h, 2h + 1, 2h + 4,
@@ -119,11 +120,11 @@ template <> struct DecHalf<BF16> {
   __device__ static inline void run(u32x4& f, uint32_t w, uint32_t prep, const DecK&, int h) {
     typedef float f2 __attribute__((ext_vector_type(2)));
     typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-    const float s = __uint_as_float(prep), s9 = 512.f * s, m8 = -8.f * s;
+    const float s = __uint_as_float(prep), m8 = -8.f * s;
     float n[4];
     nibbles_to_f32((h ? w >> 4 : w) & 0x0F0F0F0Fu, n);
-    const f2 lo = {__builtin_fmaf(n[0], s9, m8), __builtin_fmaf(n[2], s9, m8)};
-    const f2 hi = {__builtin_fmaf(n[1], s9, m8), __builtin_fmaf(n[3], s9, m8)};
+    const f2 lo = {__builtin_fmaf(n[0], s, m8), __builtin_fmaf(n[2], s, m8)};
+    const f2 hi = {__builtin_fmaf(n[1], s, m8), __builtin_fmaf(n[3], s, m8)};
     f[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(lo, bf2));
     f[h + 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(hi, bf2));
   }
