@@ -379,12 +379,12 @@ __global__ __launch_bounds__((OPT & 16) ? 1024 : 512, ((OPT & 8) && !(OPT & 16))
     for (int j = 0; j < J; ++j)
       bf[0][j] = DIAG == 3 ? u32x4{cd.w[j >> 1][(j & 1) * 2], sp[j], sp[j], sp[j]}
                            : (J == 4 ? Dec<DT>::run_lean(cd.w[j >> 1][(j & 1) * 2], sp[j], dk)
-                                     : Dec<DT>::run(cd.w[j >> 1][(j & 1) * 2], sp[j], dk));
+                                     : Dec<DT>::run_cvt(cd.w[j >> 1][(j & 1) * 2], sp[j], dk));
 #define SQMP_BF7(s, j) bf[s][j]
     SQMP_FQ7_BLOCKS(SQMP_BF7, ald,
                     if (t < J) bf[1][t] = DIAG == 3 ? u32x4{cd.w[t >> 1][(t & 1) * 2 + 1], sp[t], sp[t], sp[t]}
                                                     : (J == 4 ? Dec<DT>::run_lean(cd.w[t >> 1][(t & 1) * 2 + 1], sp[t], dk)
-                                                              : Dec<DT>::run(cd.w[t >> 1][(t & 1) * 2 + 1], sp[t], dk)));
+                                                              : Dec<DT>::run_cvt(cd.w[t >> 1][(t & 1) * 2 + 1], sp[t], dk)));
 #undef SQMP_BF7
   };
   // hook(t) runs after the MFMAs of block t (the mid-stage wait / issue at t = I - 1)
