@@ -280,9 +280,11 @@ static int launch(const GemvArgs& a, int E, int max_rows, hipStream_t s) {
   // / 10.6, 1000 of K 4096 19.7 / 21.6 / 20.8 / 28.8
   constexpr int N1 = DT::id == SQMP_F32 ? 0 : 1, N2 = DT::id == SQMP_F32 ? 0 : 2;
   if constexpr (EXP) {
-    // (many experts' blocks: 4 waves, 8 experts x 688 blocks of K 4096 61 us against 74 with 8)
+    // 8 / 4 waves by the blocks of all experts, 2 rows each: K 4096 (fp16) 256 blocks 6.7 / 7.7 us, 512 10.3 /
+    // 10.5, 1024 18.8 / 17.0, 1536 26.3 / 24.0, 2048 34.0 / 31.1, 5504 81 / 77; K 2048 (bf16) 1024 13.5 / 11.7,
+    // 2048 23.5 / 20.1, 5632 58 / 50
     if (max_rows <= 16) {
-      if ((long)nb * E >= 2048) {
+      if ((long)nb * E >= 1024) {
         if (max_rows <= 8) SQMP_GV(1, 2, 4, 4, false, N1); else SQMP_GV(1, 2, 4, 4, false, N2);
       } else {
         if (max_rows <= 8) SQMP_GV(1, 2, 8, 4, false, N1); else SQMP_GV(1, 2, 8, 4, false, N2);

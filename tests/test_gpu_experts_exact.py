@@ -207,3 +207,28 @@ def test_module(T, aq, p, dt):
         assert torch.equal(ha[ra.slots.long()], h[sl[t]])     # the very rows of the batch
         alone = mod(x[t:t + 1], ids[t:t + 1], wt[t:t + 1])
         assert ((alone.double() - y64[t]).abs() <= bound[t]).all()
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("T", [1, 8, 13])
+@pytest.mark.parametrize("E,N,K,G", [(64, 512, 320, 64), (8, 4102, 192, 32), (3, 11006, 1088, 64), (40, 864, 200, 8),
+                                     (2, 4096, 704, 128)])
+def test_few_rows_of_many_blocks(E, N, K, G, T, act, dt):
+    """Experts of a few rows: on either side of 1024 blocks of 32 weight rows, from which on workgroups have
+    4 waves; up to 8 rows of an expert, and more."""
+    D, g = DT[dt], gen(N + T)
+    codes, scales = int_weight((E, N, K), G, D, g)
+    scales = scales / 64 if act else scales
+    pe = experts.pack_expert_codes(codes, scales, G, gated=act is not None)
+    ids = torch.randint(0, E, (T, 1), generator=g, device="cuda")
+    ids[T // 2:] = 1                                          # an expert of most of the tokens
+    r = experts.plan_routes(ids, torch.ones(T, 1, device="cuda"), E)
+    x = int_rows(T, K, D, g)
+    u = plain_experts(x, values(codes, scales, G), r, False)
+    z = experts.expert_linear(x, pe, r, act=act)
+    if act is None:
+        assert torch.equal(z, u.float().to(D))
+    else:
+        want, tol = gated(u, N // 2, act)
+        assert ((z.double() - want).abs() <= rounded(tol, want, D)).all()
