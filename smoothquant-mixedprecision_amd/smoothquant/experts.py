@@ -467,14 +467,28 @@ class W4A4Experts(nn.Module):
 
     # -------------------------------------------------------------- packing
     @staticmethod
-    def from_float(module, weight_quant="per_channel", act_quant="per_token", importance=None,
-                   salient_prop=0, quant_bits=4, group_size=128):
-        """module: the fused experts.  importance [H] picks the salient columns of gate_up_proj
-        (one set for all experts, as W4A4Linear picks them)."""
+    def check(module, weight_quant="per_channel", act_quant="per_token", quant_bits=4, group_size=128):
+        """The module that would take over `module`, without its weights; ValueError where none can."""
         for n in ("gate_up_proj", "down_proj", "act_fn"):
             if not hasattr(module, n):
                 raise ValueError(f"W4A4Experts: {type(module).__name__} has no fused {n}")
         new = W4A4Experts(_act_name(module.act_fn), act_quant, quant_bits, group_size)
+        if weight_quant == "none" or weight_quant not in ops.WEIGHT_MODES:
+            raise ValueError(f"W4A4Experts: invalid weight_quant: {weight_quant}")
+        for w in (module.gate_up_proj, module.down_proj):
+            if w.shape[0] > MAX_EXPERTS:
+                raise ValueError(f"W4A4Experts: {w.shape[0]} experts, at most {MAX_EXPERTS}")
+            if ops.geometry(w.shape[2], 0, ops.WEIGHT_MODES[weight_quant], group_size)[1] % 8:
+                raise ValueError("W4A4Experts: needs groups of a multiple of 8 columns, got "
+                                 f"{group_size}")
+        return new
+
+    @staticmethod
+    def from_float(module, weight_quant="per_channel", act_quant="per_token", importance=None,
+                   salient_prop=0, quant_bits=4, group_size=128):
+        """module: the fused experts.  importance [H] picks the salient columns of gate_up_proj
+        (one set for all experts, as W4A4Linear picks them)."""
+        new = W4A4Experts.check(module, weight_quant, act_quant, quant_bits, group_size)
         if not torch.cuda.is_available():
             raise RuntimeError("W4A4Experts packing needs a ROCm GPU (no CPU implementation)")
         gate_up, down = module.gate_up_proj.data, module.down_proj.data

@@ -822,6 +822,10 @@ def quantize_mixtral(model, weight_quant="per_channel", act_quant="per_token",
     if quantize_experts:
         from .experts import W4A4Experts
         W4A4Experts(act_quant=act_quant, quant_bits=quant_bits)  # (refuses before anything is swapped)
+        for m in model.modules():
+            if (isinstance(m, mm.MixtralSparseMoeBlock)
+                    and hasattr(getattr(m, "experts", None), "gate_up_proj")):
+                W4A4Experts.check(m.experts, weight_quant, act_quant, quant_bits, group_size)
     expert_cls = getattr(mm, "MixtralBLockSparseTop2MLP", None) or getattr(mm, "MixtralBlockSparseTop2MLP", None)
     for name, m in list(model.model.named_modules()):
         pre = "model." + name + "."

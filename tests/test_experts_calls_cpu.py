@@ -326,3 +326,27 @@ def test_modules_run_on_their_inputs_device(monkeypatch, call):
     with pytest.raises(Reached):
         run()
     assert seen == [1] and current == [0]
+
+
+@pytest.mark.parametrize("config,kw,match", [
+    (dict(hidden_act="relu"), {}, "activation"),
+    (dict(hidden_act="gelu_new"), {}, "activation"),
+    ({}, dict(weight_quant="per_group", group_size=12), "multiple of 8"),
+    ({}, dict(weight_quant="none"), "weight_quant"),
+    (dict(num_local_experts=260), {}, "experts"),
+    ({}, dict(act_quant="per_group"), "row by row"),
+    ({}, dict(quant_bits=8), "4 bits")])
+def test_quantize_mixtral_refuses_before_it_swaps_anything(monkeypatch, config, kw, match):
+    """Experts that cannot be packed: the model is left whole, not with its first layers quantized."""
+    from transformers import MixtralConfig, MixtralForCausalLM
+    from smoothquant import fake_quant
+    c = dict(vocab_size=16, hidden_size=32, intermediate_size=24, num_hidden_layers=1, num_attention_heads=2,
+             num_key_value_heads=2, num_local_experts=2, num_experts_per_tok=1)
+    model = MixtralForCausalLM(MixtralConfig(**dict(c, **config)))
+    if not any(hasattr(m, "gate_up_proj") for m in model.modules()):
+        pytest.skip("experts are not fused in this version of transformers")
+    swapped = []
+    monkeypatch.setattr(fake_quant, "_swap", lambda *a, **k: swapped.append(a[1]))
+    with pytest.raises(ValueError, match=match):
+        fake_quant.quantize_model(model, quantize_experts=True, **kw)
+    assert not swapped
