@@ -266,7 +266,7 @@ def pack_expert_codes(codes: torch.Tensor, scales: torch.Tensor, group_size: int
     if scales.dim() != 3 or scales.shape[:2] != codes.shape[:2]:
         raise ValueError(f"pack_expert_codes: scales {tuple(scales.shape)} do not match codes "
                          f"{tuple(codes.shape)}")
-    n_rows = codes.shape[1]
+    n_rows, scales = codes.shape[1], scales.detach()
     if gated:
         codes, scales = _interleave(codes), _interleave(scales)
     # one weight whose rows are the experts', each padded to the operands' 256

@@ -1080,6 +1080,7 @@ def pack_codes(codes: torch.Tensor, scales: torch.Tensor, group_size: int) -> Pa
         raise ValueError(f"pack_codes: scales {tuple(scales.shape)} do not match codes "
                          f"{tuple(codes.shape)} in groups of {group_size}")
     dev, dt = codes.device, scales.dtype
+    scales = scales.detach()  # (the weight is a constant)
     wmode = _lib.W_PER_CHANNEL if scales.shape[1] == 1 else _lib.W_PER_GROUP_UNSORTED
     Kp, Gw, ngw, S_pad = geometry(K, 0, wmode, group_size)
     Np = pad_n(N)

@@ -325,3 +325,21 @@ def test_linked_layers_after_use_gemv(M):
         exact = a.double() @ w_hat.T + q.bias.reshape(-1).double()
         tol = tolerance(a, w_hat, exact, D, extra=2.0 ** -24 * exact.abs())
         assert ((y.double() - exact).abs() <= tol).all()
+
+
+def test_scales_that_require_a_gradient():
+    """Packed weights of parameters: constants without a graph, that copy as any other."""
+    import copy
+    D, g = torch.float16, gen(9)
+    codes, scales = int_weight((2, 64, 128), 64, D, g)
+    want = ops.pack_codes(codes[0], scales[0], 64)
+    p = torch.nn.Parameter(scales)
+    pw, pe = ops.pack_codes(codes[0], p[0], 64), experts.pack_expert_codes(codes, p, 64, gated=True)
+    assert not pw.wscale.requires_grad and not pe.scale_t.requires_grad
+    x = int_rows(3, 128, D, g)
+    assert torch.equal(ops.gemv(x, copy.deepcopy(pw)), ops.gemv(x, want))
+    r = experts.plan_routes(torch.tensor([[0], [1], [1]], device="cuda"), torch.ones(3, 1, device="cuda"), 2)
+    assert torch.equal(experts.expert_linear(x, copy.deepcopy(pe), r, act="silu"),
+                       experts.expert_linear(x, pe, r, act="silu"))
+    dense = ops.pack_codes(codes[0], torch.nn.Parameter(scales[0]).repeat_interleave(16, 1), 4)
+    assert not dense.dense.requires_grad
