@@ -75,8 +75,8 @@ __device__ inline void nibbles_to_f32(uint32_t b, float (&n)[4]) {
   n[0] = lo[0], n[1] = lo[1], n[2] = hi[0], n[3] = hi[1];
 }
 
-// one dword of codes and its scale -> 8 values D(code * s).  (bf16 by Dec: with e4m3 conversions the
-// few-row kernel runs 11.0 us instead of 10.6 at 8 x 11008 x 4096, the expert tiles 2 % faster)
+// one dword of codes and its scale -> 8 values D(code * s).  (bf16 by Dec::run: by scaled conversions
+// the few-row kernel runs 10.1 us instead of 8.8 at 8 x 11008 x 4096; the tiles use them, DecHalf)
 template <class DT>
 __device__ inline Frag<DT> decode(uint32_t w, typename DT::T s, const DecK& k) {
   Frag<DT> f;

@@ -1170,9 +1170,21 @@ def _operand_rows(x2: torch.Tensor, width: int):
 def pack_rows(x2: torch.Tensor, amap: torch.Tensor, Kp: int, salient: Optional[torch.Tensor],
               S: int, S_pad: int) -> torch.Tensor:
     """x [M, K] -> [M, Kp + S_pad]: the unquantized activation operand (columns gathered by amap,
-    then the salient columns)."""
+    then the salient columns).  amap int32 [Kp] and salient int32 [S] name columns of x (amap < 0: a
+    zero); they are not looked at here."""
     if not x2.is_cuda:
         _require_gpu(x2, "pack_rows")
+    if x2.dim() != 2 or Kp <= 0 or not 0 <= S <= S_pad:
+        raise ValueError(f"pack_rows: x {tuple(x2.shape)}, Kp {Kp}, {S} of {S_pad} salient columns")
+    for name, t, n in (("amap", amap, Kp), ("salient", salient, S)):
+        if n and (t is None or t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous()
+                  or t.device != x2.device):
+            raise ValueError(f"pack_rows: {name} must be {n} contiguous int32 on {x2.device}")
+    return _pack_rows(x2, amap, Kp, salient, S, S_pad)
+
+
+def _pack_rows(x2, amap, Kp, salient, S, S_pad) -> torch.Tensor:
+    """pack_rows with the maps of a packed weight."""
     if x2.stride(1) != 1 or x2.stride(0) == 0:  # (0: rows of an expanded tensor)
         x2 = x2.contiguous()
     M = x2.shape[0]
@@ -1233,7 +1245,7 @@ def gemv(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
         cols = pw.Kp
         amap, sal = pw.amap.data_ptr(), None if pw.salient is None else pw.salient.data_ptr()
     else:
-        x = pack_rows.__wrapped__(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
+        x = _pack_rows(x, pw.amap, pw.Kp, pw.salient, pw.S, pw.S_pad)
         xp, ld, cols = x.data_ptr(), L, pw.Kp
     wp, wn = None, 0
     if M > 32:

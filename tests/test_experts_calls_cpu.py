@@ -350,3 +350,25 @@ def test_quantize_mixtral_refuses_before_it_swaps_anything(monkeypatch, config, 
     with pytest.raises(ValueError, match=match):
         fake_quant.quantize_model(model, quantize_experts=True, **kw)
     assert not swapped
+
+
+def test_pack_rows_refuses_maps_it_would_misread(library):
+    """ops.pack_rows: int32 maps of the operand's size, on the rows' device."""
+    x = gpu(torch.zeros(3, 64, dtype=torch.float16))
+    amap, sal = gpu(torch.arange(128, dtype=torch.int32)), gpu(torch.arange(4, dtype=torch.int32))
+
+    def call(x=x, amap=amap, Kp=128, salient=None, S=0, S_pad=0):
+        return ops.pack_rows(x, amap, Kp, salient, S, S_pad)
+    assert call().shape == (3, 128) and call(salient=sal, S=4, S_pad=64).shape == (3, 192)
+    library.calls.clear()
+    for bad in (dict(amap=gpu(torch.arange(128))), dict(amap=gpu(torch.arange(127, dtype=torch.int32))),
+                dict(amap=gpu(torch.arange(256, dtype=torch.int32))[::2]), dict(amap=None), dict(Kp=0), dict(x=x[0]),
+                dict(salient=sal, S=5, S_pad=64), dict(S=4, S_pad=64), dict(salient=sal, S=4, S_pad=2),
+                dict(salient=gpu(torch.arange(4)), S=4, S_pad=64), dict(S=-1), dict(x=x.int())):
+        with pytest.raises(ValueError):
+            call(**bad)
+    for bad in (dict(amap=torch.arange(128, dtype=torch.int32)),
+                dict(salient=torch.arange(4, dtype=torch.int32), S=4, S_pad=64)):
+        with pytest.raises((ValueError, RuntimeError)):
+            call(**bad)
+    assert not library.calls
