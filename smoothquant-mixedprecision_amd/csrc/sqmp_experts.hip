@@ -18,10 +18,10 @@
 // The grid holds every tile that any split of `slots` over the experts can need; the tiles that
 // exist are found from the offsets on the GPU (no host synchronisation), the rest return.
 // Measured: 16384 x 4096 x 4096 as one expert 423 us (1300 TFLOP/s, 256-row tiles; a library product of
-// 8192^3 reaches 1200 on that card), 2 of 8 experts x 2048 tokens, 4096 -> 2 x 11008 gated 675 us
-// (1094 TFLOP/s; 616 us at the library's rate), 11008 -> 4096 355 us (1040; 308 us); 509 tokens x 6 of
-// 64, 2048 -> 1408 gated bf16 95 + 13 us of join (40 us of bytes at the rate of a large copy): there the
-// vector pipe decodes for 41 % and the MFMA runs for 27 % of the time.
+// 8192^3 reaches 1200 on that card), 2 of 8 experts x 2048 tokens, 4096 -> 2 x 11008 gated 710 us
+// (1040 TFLOP/s; 616 us at the library's rate), 11008 -> 4096 357 + 20 us of join (980; 295 us); 509
+// tokens x 6 of 64, 2048 -> 1408 gated bf16 97 + 13 us (40 us of bytes at the rate of a large copy):
+// there the vector pipe decodes for 41 % and the MFMA runs for 27 % of the time.
 #include "sqmp_w4_launch.h"
 
 namespace sqmp {

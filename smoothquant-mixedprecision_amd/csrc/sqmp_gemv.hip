@@ -12,10 +12,10 @@
 // in flight each; the NW partial sums meet in LDS and are added in a fixed order, so results do not
 // depend on timing.  x comes as 16-byte fragments from L2, or, where its rows are unaligned or the
 // weight has an order of its own, gathered into LDS while the first codes are on their way.
-// Measured in a captured graph: 1 x 4096 x 4096 fp16 4.4 us (8.7 MB: 2.0 TB/s, 1.7 us at the rate of a
-// large copy; latency), 8 x 11008 x 4096 bf16 9.5 us (2.5 TB/s; decoding, and 344 blocks on 256
-// CUs), 1 x 32000 x 4096 15.1 us (4.5 TB/s), 64 x 4096 x 11008 15 us (1.7 TB/s; two groups of tokens
-// decode everything twice), 8 experts of 2 rows, 22016 x 4096: 62 us (5.4 TB/s).
+// Measured (kernel alone): 1 x 4096 x 4096 fp16 4.5 us (8.7 MB: 1.9 TB/s, 1.7 us at the rate of a
+// large copy; latency), 8 x 11008 x 4096 bf16 9.3 us (2.6 TB/s; decoding, and 344 blocks on 256
+// CUs), 1 x 32000 x 4096 15.1 us (4.5 TB/s), 64 x 4096 x 11008 15.9 us (1.6 TB/s; two groups of tokens
+// decode everything twice), 8 tokens to 2 of 8 experts, 22016 x 4096: 67.8 us (335 MB: 4.9 TB/s).
 #include "sqmp_w4_launch.h"
 
 namespace sqmp {
