@@ -414,7 +414,7 @@ __global__ __launch_bounds__(128) void join_kernel(const GemvArgs a, int E, int 
 // 2 x 11008 gated, fp16, 128 rows each 275 / 367, 512: 694 / 725, 1024: 1293 / 1293, 2048: 2513 / 2490, 4096:
 // 5019 / 5081; bf16 512: 726 / 732, 1024: 1326 / 1283, 2048: 2576 / 2479, 4096: 5177 / 5043.  The way down has
 // fewer tiles and depends on how full their last round is: 11008 -> 4096 fp16 1024: 638 / 660, 2048: 1289 /
-// 1407, 3072: 1873 / 2003; bf16 1536: 964 / 937, 2048: 1301 / 1396, 3072: 1953 / 1963; 4096 -> 4096 fp16 2048:
+// 1407, 4096: 2453 / 2715; bf16 1536: 964 / 937, 2048: 1301 / 1396, 4096: 2552 / 2695; 4096 -> 4096 fp16 2048:
 // 470 / 449 and 472 / 502 on two cards.  SQMP_EXPERT_ROWS overrides (A/B)
 static int tile_rows(int E, int slots) {
   const char* k = knob("SQMP_EXPERT_ROWS");
